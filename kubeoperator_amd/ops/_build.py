@@ -64,6 +64,11 @@ FILE_FLAGS = {"flash_bwd_w1.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
               "flash_fwd4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true", "-fno-slp-vectorize", "-fno-honor-nans"]}
 
 
+# no packed fp32 instructions (v_pk_add / mul / fma_f32), which hipcc -O3 forms by itself from scalar float code: some of
+# their forms have returned wrong values on this hardware now and then, without an error. hipcc's host pass warns that it
+# does not know the feature
+BASE_HIPFLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
 # probe builds only (tools/build_ab.py --ablations): never set for the shipped extension
 EXTRA_HIPFLAGS: list[str] = []
 
@@ -83,7 +88,7 @@ def build(verbose: bool = False, jobs: int | None = None, force: bool = False) -
         objs.append(obj)
         if force or _needs(obj, src, hdr):
             jobs_list.append([hipcc, f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics",
-                              abi, *FILE_FLAGS.get(os.path.basename(src), []), *EXTRA_HIPFLAGS, "-I", CSRC, "-c", src,
+                              abi, *BASE_HIPFLAGS, *FILE_FLAGS.get(os.path.basename(src), []), *EXTRA_HIPFLAGS, "-I", CSRC, "-c", src,
                               "-o", obj])
     bsrc = os.path.join(CSRC, "bindings.cpp")
     bobj = os.path.join(BUILD_DIR, "bindings.cpp.o")
