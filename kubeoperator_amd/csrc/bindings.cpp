@@ -5,6 +5,7 @@
 // views whose rows may be strided (e.g. the Q, K and V column slices of the fused QKV output), so
 // the attention / RoPE paths never copy or transpose.
 #include <torch/extension.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include "kernels.h"
 
@@ -559,6 +560,233 @@ void decode_rope_append_(const Tensor& qkv, const Tensor& cos_t, const Tensor& s
      "decode_rope_append");
 }
 
+// ------------------------------------------------------------------ many requests on one model (serving, draft training)
+// Shared checks of the operators below: every operand on the first one's device (the launch goes to that device's current
+// stream, whatever the current device is), and no gradient expected of a forward-only operator.
+void check_same_device(const Tensor& t, const Tensor& first, const char* name) {
+  TORCH_CHECK(t.device() == first.device(), name, " is on ", t.device(), ", expected ", first.device());
+}
+void check_no_grad(const Tensor& t, const char* what) {
+  TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), what, " is forward only: it has no gradient");
+}
+void check_i32(const Tensor& t, const char* name) {
+  check_gpu(t, name);
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.is_contiguous(), name, " must be contiguous int32");
+}
+
+// whether the byte ranges that two 2-D row views span have anything in common
+bool spans_meet(const Tensor& a, const Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  auto lo = [](const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()); };
+  auto hi = [&](const Tensor& t) {
+    return lo(t) + ((t.size(0) - 1) * t.stride(0) + (t.size(1) - 1) * t.stride(1) + 1) * t.element_size();
+  };
+  return lo(a) < hi(b) && lo(b) < hi(a);
+}
+
+// q [B*T, Hq*D] rows; k_prefix / v_prefix [Hkv, P, D] (head and key strides multiples of 8); caches [B, Hkv, Smax, D]
+// contiguous; lens [B] int32. Row b*T+t is token t of sequence b.
+Tensor prefix_attn(const Tensor& q, const Tensor& k_prefix, const Tensor& v_prefix, const Tensor& k_cache,
+                   const Tensor& v_cache, const Tensor& lens, int64_t max_len, int64_t tokens, double scale) {
+  const std::pair<const Tensor*, const char*> ts[] = {
+      {&q, "q"}, {&k_prefix, "k_prefix"}, {&v_prefix, "v_prefix"}, {&k_cache, "k_cache"}, {&v_cache, "v_cache"}};
+  for (auto& [t, name] : ts) {
+    check_bf16(*t, name);
+    check_same_device(*t, q, name);
+    check_no_grad(*t, "prefix_attention");
+  }
+  check_rows(q, "q");
+  check_i32(lens, "lens");
+  check_same_device(lens, q, "lens");
+  TORCH_CHECK(k_cache.dim() == 4 && k_cache.is_contiguous() && v_cache.is_contiguous() &&
+                  k_cache.sizes() == v_cache.sizes(), "caches must be contiguous [B, Hkv, Smax, D] and equal");
+  check_aligned(k_cache, "k_cache");
+  check_aligned(v_cache, "v_cache");
+  const int64_t B = k_cache.size(0), Hkv = k_cache.size(1), Smax = k_cache.size(2), D = k_cache.size(3);
+  for (auto* t : {&k_prefix, &v_prefix}) {
+    TORCH_CHECK(t->dim() == 3 && t->size(0) == Hkv && t->size(2) == D && t->size(1) == k_prefix.size(1),
+                "prefix must be [Hkv, P, D] with the cache's heads and head dim, K and V alike");
+    TORCH_CHECK(t->numel() == 0 || (t->stride(2) == 1 && t->stride(0) % 8 == 0 && t->stride(1) % 8 == 0),
+                "prefix keys must be contiguous rows with strides that are multiples of 8");
+    check_aligned(*t, "prefix");
+  }
+  const int64_t P = k_prefix.size(1);
+  TORCH_CHECK(D == 64 || D == 128, "prefix_attention: head dim must be 64 or 128");
+  TORCH_CHECK(tokens >= 1 && q.size(0) == B * tokens && lens.numel() == B,
+              "prefix_attention: q must have B * tokens rows and lens B entries");
+  TORCH_CHECK(q.size(1) % D == 0 && q.size(1) > 0 && (q.size(1) / D) % Hkv == 0,
+              "prefix_attention: q width must be a multiple of Hkv * D");
+  TORCH_CHECK(max_len >= 0 && max_len <= Smax, "max_len must be in [0, Smax]");
+  TORCH_CHECK(P <= 0x7fffff00 && Smax <= 0x7fffff00 && B <= 0x7fffffff && tokens <= 0x7fffffff, "prefix_attention: too long");
+  const int64_t Hq = q.size(1) / D;
+  TORCH_CHECK(B * tokens * Hq <= 0x3fffffff, "prefix_attention: too many rows");
+  const c10::DeviceGuard guard(q.device());
+  auto o = at::empty({B * tokens, Hq * D}, q.options());
+  if (B == 0) return o;
+  auto ws = at::empty({kop::prefix_attn_workspace((int)B, (int)tokens, (int)Hq, (int)Hkv, (int)D, (int)P, (int)max_len)},
+                      q.options().dtype(at::kByte));
+  rc(kop::prefix_attn(bp(q), q.stride(0), bp(k_prefix), k_prefix.stride(0), k_prefix.stride(1), bp(v_prefix),
+                      v_prefix.stride(0), v_prefix.stride(1), (int)P, bp(k_cache), bp(v_cache), lens.data_ptr<int>(),
+                      (int)max_len, bp(o), o.stride(0), (int)B, (int)tokens, (int)Smax, (int)Hq, (int)Hkv, (int)D,
+                      (float)scale, ws.data_ptr(), cur_stream()),
+     "prefix_attn");
+  return o;
+}
+
+// y [M, N], x [M, K] rows; a [n, r, K], b [n, N, r] contiguous; index [M] int32; scale [n] fp32; out: y itself or a new tensor
+Tensor lora_add(const Tensor& y, const Tensor& x, const Tensor& a, const Tensor& b, const Tensor& index,
+                const Tensor& scale, const c10::optional<Tensor>& out_) {
+  const std::pair<const Tensor*, const char*> ts[] = {{&y, "y"}, {&x, "x"}, {&a, "a"}, {&b, "b"}};
+  for (auto& [t, name] : ts) {
+    check_bf16(*t, name);
+    check_same_device(*t, y, name);
+    check_no_grad(*t, "lora_add");
+  }
+  check_rows(y, "y");
+  check_rows(x, "x");
+  TORCH_CHECK(a.dim() == 3 && b.dim() == 3 && a.is_contiguous() && b.is_contiguous(),
+              "adapters must be contiguous a [n, r, K] and b [n, N, r]");
+  check_aligned(a, "a");
+  check_aligned(b, "b");
+  check_i32(index, "index");
+  check_same_device(index, y, "index");
+  check_f32(scale, "scale");
+  check_same_device(scale, y, "scale");
+  const int64_t M = x.size(0), K = x.size(1), N = y.size(1), n = a.size(0), r = a.size(1);
+  TORCH_CHECK(y.size(0) == M && index.dim() == 1 && index.numel() == M, "lora_add: x, y and index disagree on the rows");
+  TORCH_CHECK(a.size(2) == K && b.size(0) == n && b.size(1) == N && b.size(2) == r,
+              "lora_add: a must be [n, r, K] and b [n, N, r]");
+  TORCH_CHECK(scale.dim() == 1 && scale.numel() == n && scale.is_contiguous(), "lora_add: scale must be [n]");
+  TORCH_CHECK(r >= 8 && r % 8 == 0 && r <= kop::kLoraMaxRank, "lora_add: rank must be a multiple of 8 up to ",
+              kop::kLoraMaxRank, " (pad a and b with zeros)");
+  TORCH_CHECK(K % 8 == 0 && N % 8 == 0 && K > 0 && N > 0 && K <= 0x7fffff00 && N <= 0xffff00 && n <= 0x7fffffff,
+              "lora_add: widths must be multiples of 8");
+  const c10::DeviceGuard guard(y.device());
+  Tensor out;
+  if (out_.has_value() && out_->defined()) {
+    out = *out_;
+    check_bf16(out, "out");
+    check_rows(out, "out");
+    check_same_device(out, y, "out");
+    check_no_grad(out, "lora_add");
+    TORCH_CHECK(out.sizes() == y.sizes(), "lora_add: out must have y's shape");
+    TORCH_CHECK(out.stride(0) >= N || M <= 1, "lora_add: the rows of out overlap");
+    if (!(out.data_ptr() == y.data_ptr() && out.strides() == y.strides()))
+      TORCH_CHECK(!spans_meet(out, y), "lora_add: out overlaps y (pass y itself)");
+    TORCH_CHECK(!spans_meet(out, x), "lora_add: out overlaps x");
+  } else {
+    out = at::empty({M, N}, y.options());
+  }
+  if (M == 0) return out;
+  auto ws = at::empty({kop::lora_workspace(M, (int)K, (int)r)}, y.options().dtype(at::kByte));
+  rc(kop::lora_add(bp(y), y.stride(0), bp(x), x.stride(0), bp(a), bp(b), index.data_ptr<int>(), scale.data_ptr<float>(),
+                   bp(out), out.stride(0), M, (int)K, (int)N, (int)n, (int)r, ws.data_ptr(), cur_stream()),
+     "lora_add");
+  return out;
+}
+
+// target [B, T+1, V], draft [B, T, V] (None if T = 0 or temperature = 0), tokens [B, T] int64, u [B, T+1] fp32
+std::vector<Tensor> verify_draft(const Tensor& target, const c10::optional<Tensor>& draft, const Tensor& tokens,
+                                 const Tensor& u, double temperature, const c10::optional<Tensor>& n_draft) {
+  check_gpu(target, "target");
+  check_no_grad(target, "verify_draft");
+  const bool f32 = target.scalar_type() == at::kFloat;
+  TORCH_CHECK(f32 || target.scalar_type() == at::kBFloat16, "target must be float32 or bfloat16");
+  TORCH_CHECK(target.dim() == 3 && target.size(1) >= 1 && target.size(2) >= 1, "target must be [B, T+1, V]");
+  const int64_t B = target.size(0), T = target.size(1) - 1, V = target.size(2);
+  TORCH_CHECK(V == 1 || target.stride(2) == 1, "target must have a contiguous last dimension");
+  TORCH_CHECK(T <= kop::kVerifyMaxDraft, "verify_draft: at most ", kop::kVerifyMaxDraft, " drafted tokens");
+  TORCH_CHECK(V <= 0x3fffffff && B <= 65535, "verify_draft: vocabulary or batch too large");
+  TORCH_CHECK(temperature == 0.0 || (temperature >= 1e-4 && temperature <= 1e4),
+              "temperature must be 0 (greedy) or in [1e-4, 1e4]");
+  const void* dp = nullptr;
+  int64_t ds_b = 0, ds_t = 0;
+  if (T > 0 && temperature > 0.0) {
+    TORCH_CHECK(draft.has_value() && draft->defined(), "verify_draft: draft logits are needed unless temperature is 0");
+    check_gpu(*draft, "draft");
+    check_same_device(*draft, target, "draft");
+    check_no_grad(*draft, "verify_draft");
+    TORCH_CHECK(draft->scalar_type() == target.scalar_type(), "draft must have target's dtype");
+    TORCH_CHECK(draft->dim() == 3 && draft->size(0) == B && draft->size(1) == T && draft->size(2) == V,
+                "draft must be [B, T, V]");
+    TORCH_CHECK(V == 1 || draft->stride(2) == 1, "draft must have a contiguous last dimension");
+    dp = draft->data_ptr();
+    ds_b = draft->stride(0), ds_t = draft->stride(1);
+  }
+  check_gpu(tokens, "tokens");
+  check_same_device(tokens, target, "tokens");
+  TORCH_CHECK(tokens.scalar_type() == at::kLong && tokens.is_contiguous() && tokens.dim() == 2 && tokens.size(0) == B &&
+                  tokens.size(1) == T, "tokens must be contiguous int64 [B, T]");
+  check_f32(u, "u");
+  check_same_device(u, target, "u");
+  TORCH_CHECK(u.is_contiguous() && u.dim() == 2 && u.size(0) == B && u.size(1) == T + 1,
+              "u must be contiguous float32 [B, T+1]");
+  const int* nd = nullptr;
+  if (n_draft.has_value() && n_draft->defined()) {
+    check_i32(*n_draft, "n_draft");
+    check_same_device(*n_draft, target, "n_draft");
+    TORCH_CHECK(n_draft->dim() == 1 && n_draft->numel() == B, "n_draft must be [B]");
+    nd = n_draft->data_ptr<int>();
+  }
+  const c10::DeviceGuard guard(target.device());
+  auto out = at::empty({B, T + 1}, target.options().dtype(at::kLong));
+  auto accepted = at::empty({B}, target.options().dtype(at::kInt));
+  if (B == 0) return {out, accepted};
+  auto ws = at::empty({kop::verify_draft_workspace((int)B, (int)T, (int)V)}, target.options().dtype(at::kByte));
+  rc(kop::verify_draft(target.data_ptr(), target.stride(0), target.stride(1), dp, ds_b, ds_t, f32,
+                       tokens.data_ptr<int64_t>(), u.data_ptr<float>(), nd, (int)B, (int)T, (int)V, temperature,
+                       ws.data_ptr(), out.data_ptr<int64_t>(), accepted.data_ptr<int>(), cur_stream()),
+     "verify_draft");
+  return {out, accepted};
+}
+
+// logits [N, V] bf16 rows; index [N, K] int32; teacher [N, K] fp32; weight [N] fp32 or None; out: logits itself or a new
+// tensor -> loss [N], gradient [N, V]
+std::vector<Tensor> distill_topk(const Tensor& logits, const Tensor& index, const Tensor& teacher, double temperature,
+                                 const c10::optional<Tensor>& weight, const c10::optional<Tensor>& out_) {
+  check_bf16(logits, "logits");
+  TORCH_CHECK(!(logits.requires_grad() && at::GradMode::is_enabled()),
+              "distill_topk returns the gradient itself: detach the logits (distill_topk_lmhead has autograd)");
+  TORCH_CHECK(logits.dim() == 2 && logits.size(1) >= 1 && (logits.stride(1) == 1 || logits.size(1) == 1),
+              "logits must be [N, V] with a contiguous last dimension");
+  const int64_t N = logits.size(0), V = logits.size(1);
+  check_i32(index, "index");
+  check_f32(teacher, "teacher");
+  check_same_device(index, logits, "index");
+  check_same_device(teacher, logits, "teacher");
+  TORCH_CHECK(teacher.is_contiguous() && index.dim() == 2 && teacher.dim() == 2 && index.sizes() == teacher.sizes() &&
+                  index.size(0) == N, "index and teacher must be contiguous [N, K]");
+  const int64_t K = index.size(1);
+  TORCH_CHECK(K >= 1 && K <= kop::kDistillMaxK, "distill_topk: 1 to ", kop::kDistillMaxK, " teacher logits per row");
+  TORCH_CHECK(V <= 0x3fffffff && N <= 0x7fffffff, "distill_topk: too many rows or logits");
+  TORCH_CHECK(temperature >= 1e-4 && temperature <= 1e4, "temperature must be in [1e-4, 1e4]");
+  const float* wp = nullptr;
+  if (weight.has_value() && weight->defined()) {
+    check_f32(*weight, "weight");
+    check_same_device(*weight, logits, "weight");
+    TORCH_CHECK(weight->dim() == 1 && weight->numel() == N && weight->is_contiguous(), "weight must be [N]");
+    wp = weight->data_ptr<float>();
+  }
+  const c10::DeviceGuard guard(logits.device());
+  Tensor out;
+  if (out_.has_value() && out_->defined()) {
+    out = *out_;
+    check_bf16(out, "out");
+    check_same_device(out, logits, "out");
+    TORCH_CHECK(out.sizes() == logits.sizes() && (out.stride(1) == 1 || V == 1) && (out.stride(0) >= V || N <= 1),
+                "out must have logits' shape, contiguous rows and no overlap");
+    if (!(out.data_ptr() == logits.data_ptr() && out.strides() == logits.strides()))
+      TORCH_CHECK(!spans_meet(out, logits), "distill_topk: out overlaps logits (pass logits itself)");
+  } else {
+    out = at::empty({N, V}, logits.options());
+  }
+  auto loss = at::empty({N}, logits.options().dtype(at::kFloat));
+  rc(kop::distill_topk(bp(logits), logits.stride(0), N, (int)V, index.data_ptr<int>(), teacher.data_ptr<float>(), (int)K,
+                       wp, (float)temperature, loss.data_ptr<float>(), bp(out), out.stride(0), cur_stream()),
+     "distill_topk");
+  return {loss, out};
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "kubeoperator_amd gfx950 (MI355X) HIP kernels";
   m.attr("ARCH") = "gfx950";
@@ -593,6 +821,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("decode_attn", &decode_attn);
   m.def("decode_rope_append_", &decode_rope_append_);
   m.def("gemv", &gemv);
+  m.def("prefix_attn", &prefix_attn);
+  m.def("lora_add", &lora_add);
+  m.def("verify_draft", &verify_draft);
+  m.def("distill_topk", &distill_topk);
   m.def("flash_attn_bwd_workspace", &flash_attn_bwd_workspace);
   m.def("flash_attn_bwd", &flash_attn_bwd);
   m.def("flash_attn_set_dq_variant", [](int64_t v) { return (int64_t)kop::flash_attn_set_dq_variant((int)v); });

@@ -43,6 +43,37 @@ int cross_entropy_fwd(bf16_t* logits, int64_t ld, int64_t T, int V, const int64_
                       float* scale, float* loss_rows, float* lse_rows, bool write_grad, float grad_multiplier,
                       hipStream_t stream);
 
+// distill.hip: loss and gradient of bf16 logits against a teacher's top-K logits; grad may be the logits' own buffer.
+// index [N, K] int32 and teacher [N, K] fp32 contiguous, weight [N] fp32 or null
+constexpr int kDistillMaxK = 512;
+int distill_topk(const bf16_t* logits, int64_t ld, int64_t N, int V, const int* index, const float* teacher, int K,
+                 const float* weight, float temp, float* loss, bf16_t* grad, int64_t gld, hipStream_t stream);
+
+// verify.hip: accepted prefix of T drafted tokens per sequence and the token after it, from uniform numbers u [B, T+1];
+// temp 0: greedy. Row strides in elements; n_draft [B] or null; workspace: verify_draft_workspace() bytes, 8-byte aligned
+constexpr int kVerifyMaxDraft = 32;
+int64_t verify_draft_workspace(int B, int T, int V);
+int verify_draft(const void* target, int64_t ts_b, int64_t ts_t, const void* draft, int64_t ds_b, int64_t ds_t, bool f32,
+                 const int64_t* tokens, const float* u, const int* n_draft, int B, int T, int V, double temp,
+                 void* workspace, int64_t* out, int* accepted, hipStream_t stream);
+
+// lora.hip: out[i] = y[i] + scale[j] b[j] (a[j] x[i]) with j = index[i] (rows whose j is outside [0, n): out = y);
+// x [M, K], y / out [M, N] rows, a [n, r, K], b [n, N, r] contiguous, index [M] int32, scale [n] fp32.
+// workspace: lora_workspace() bytes. K, N, r multiples of 8, r <= kLoraMaxRank
+constexpr int kLoraMaxRank = 128;
+int64_t lora_workspace(int64_t M, int K, int r);
+int lora_add(const bf16_t* y, int64_t ys, const bf16_t* x, int64_t xs, const bf16_t* a, const bf16_t* b,
+             const int* index, const float* scale, bf16_t* out, int64_t os, int64_t M, int K, int N, int n, int r,
+             void* workspace, hipStream_t stream);
+
+// prefix_attn.hip: T newest tokens of each of B sequences against a prefix shared by all of them (kp / vp: P keys, head and
+// key strides in elements) and the sequence's own [B, Hkv, Smax, D] cache (lens[b] valid keys, max_len >= every lens on the
+// host); q / o rows b * T + t. workspace: prefix_attn_workspace() bytes
+int64_t prefix_attn_workspace(int B, int T, int Hq, int Hkv, int D, int P, int max_len);
+int prefix_attn(const bf16_t* q, int64_t qs, const bf16_t* kp, int64_t kph, int64_t kps, const bf16_t* vp, int64_t vph,
+                int64_t vps, int P, const bf16_t* kc, const bf16_t* vc, const int* lens, int max_len, bf16_t* o, int64_t os,
+                int B, int T, int Smax, int Hq, int Hkv, int D, float scale, void* workspace, hipStream_t stream);
+
 // adamw.hip
 int adamw_step(bf16_t* p, const bf16_t* g, float* master, float* m, float* v, int64_t n, float lr, float b1, float b2,
                float eps, float wd, int step, float gscale, const float* gscale_dev, hipStream_t stream);

@@ -55,14 +55,19 @@ def use_native(t=None) -> bool:
 
 from .functional import (  # noqa: E402
     cross_entropy_lmhead,
+    distill_topk,
+    distill_topk_lmhead,
     embedding,
     flash_attention,
     gelu,
     layer_norm,
     linear,
+    lora_add,
+    prefix_attention,
     rms_norm,
     rope_attention,
     swiglu,
+    verify_draft,
 )
 from .optim import FusedAdamW  # noqa: E402
 
@@ -78,5 +83,10 @@ __all__ = [
     "flash_attention",
     "rope_attention",
     "cross_entropy_lmhead",
+    "prefix_attention",
+    "lora_add",
+    "verify_draft",
+    "distill_topk",
+    "distill_topk_lmhead",
     "FusedAdamW",
 ]

@@ -864,6 +864,45 @@ def decode_attention(q, k_cache, v_cache, lens, max_len: int, scale=None):
     return _lib().decode_attn(q, k_cache, v_cache, lens, int(max_len), scale)
 
 
+def prefix_attention(q, k_prefix, v_prefix, k_cache, v_cache, lens, max_len: int, tokens: int = 1, scale=None):
+    """Serving: attention of the newest ``tokens`` tokens of every sequence over a prefix that the whole batch shares and
+    over the sequence's own cache, as one softmax. q [B * tokens, Hq*D] (row b * tokens + t; a row view of the fused QKV
+    output), k_prefix / v_prefix [Hkv, P, D] bf16 (strided heads and rows allowed, P = 0 too), caches [B, Hkv, Smax, D],
+    ``lens`` [B] int32 valid own keys with the new tokens' included, ``max_len`` >= every lens on the host (longer ones are
+    cut to it). Token t sees the prefix and the first lens - (tokens - 1 - t) own keys; a row that sees nothing is 0.
+    head dim 64 or 128. Forward only (csrc/prefix_attn.hip)."""
+    scale = scale if scale is not None else 1.0 / math.sqrt(k_cache.shape[-1])
+    if not q.is_cuda:
+        return ref.prefix_attention_ref(q, k_prefix, v_prefix, k_cache, v_cache, lens, int(max_len), int(tokens), scale)
+    return _lib().prefix_attn(q, k_prefix, v_prefix, k_cache, v_cache, lens, int(max_len), int(tokens), scale)
+
+
+def lora_add(y, x, a, b, index, scale, out=None):
+    """Serving: low-rank adapters of many requests beside one projection ``y = x W^T``: row i becomes
+    y[i] + scale[j] b[j] (a[j] x[i]) with j = index[i]; a row whose j is outside [0, n) keeps y. x [M, K], y [M, N] bf16
+    row views, a [n, r, K] and b [n, N, r] bf16 (r a multiple of 8 up to 128: pad with zeros), index [M] int32, scale [n]
+    fp32. Returns a new tensor, or writes ``out`` (``y`` itself for in place). Forward only (csrc/lora.hip)."""
+    if not y.is_cuda:
+        return ref.lora_add_ref(y, x, a, b, index, scale, out)
+    return _lib().lora_add(y, x, a, b, index, scale, out)
+
+
+def verify_draft(target, draft, tokens, u, temperature: float = 1.0, n_draft=None):
+    """Speculative decoding: how many of T drafted tokens the target model keeps, and the token that follows them.
+
+    target [B, T+1, V] and draft [B, T, V] logits (fp32 or bf16), tokens [B, T] int64 drawn from the draft's
+    distribution, u [B, T+1] uniform numbers in [0, 1). With p, q = softmax(logits / temperature): token t is kept while
+    u[t] q(x) < p(x); at the first refusal j the next token is drawn by u[T] from max(p_j - q_j, 0), after T kept
+    ones from p_T -- the outputs are then distributed as the target's own samples. ``temperature`` 0: a token is kept while
+    it is the target's argmax (lowest index on a tie), and the next one is the argmax (``draft`` is not read).
+    ``n_draft`` [B] int32: sequences with fewer drafted tokens. A token outside the vocabulary is refused; a logit of
+    -inf or NaN has probability 0; a row without any probability yields -1.
+    Returns (out [B, T+1] int64: the kept tokens, the next one, then -1; kept [B] int32). Forward only (csrc/verify.hip)."""
+    if not target.is_cuda:
+        return ref.verify_draft_ref(target, draft, tokens, u, float(temperature), n_draft)
+    return tuple(_lib().verify_draft(target, draft, tokens, u, float(temperature), n_draft))
+
+
 def rope_positions_(x, cos, sin, pos, nheads, D):
     """RoPE in place on the first ``nheads`` heads of each row of x at explicit positions ``pos`` [T] int32."""
     if not x.is_cuda:
@@ -956,3 +995,60 @@ def cross_entropy_lmhead(x, w, targets, ignore_index=-100):
         return F.cross_entropy(logits.float(), targets.reshape(-1), ignore_index=ignore_index)
     _gate(w)
     return _LMHeadCE.apply(x, w, targets, ignore_index)
+
+
+# ---------------------------------------------------------------------------------------------------
+# distillation from a teacher's top logits
+# ---------------------------------------------------------------------------------------------------
+def distill_topk(logits, index, teacher, temperature: float = 1.0, weight=None, out=None):
+    """Loss and gradient of a student's logits [N, V] (bf16) against a teacher's K top logits per row, in one launch.
+
+    ``index`` [N, K] int32 names the tokens, ``teacher`` [N, K] fp32 holds their logits (or log-probabilities); an index
+    outside [0, V) or a teacher logit of -inf / NaN is padding. With p = softmax(teacher / t) over the listed tokens
+    and q = softmax(logits / t) over the vocabulary: loss[i] = t^2 w_i sum_k p_k (log p_k - log q_k), and the second
+    result is d loss[i] / d logits (``out``: written there, ``logits`` itself for in place). ``weight`` [N] fp32 (default
+    1); rows of weight 0 or of padding only give 0. A token listed twice counts with the sum of its probabilities."""
+    if not logits.is_cuda:
+        return ref.distill_topk_ref(logits, index, teacher, float(temperature), weight, out)
+    return tuple(_lib().distill_topk(logits, index, teacher, float(temperature), weight, out))
+
+
+class _LMHeadDistill(Function):
+    @staticmethod
+    def forward(ctx, x, w, index, teacher, temperature, weight):
+        x2 = x.reshape(-1, x.shape[-1]).contiguous()
+        logits = torch.mm(x2, w.t())
+        rows, dlogits = distill_topk(logits, index, teacher, temperature, weight, out=logits)
+        ctx.save_for_backward(x2, w, dlogits)
+        ctx.in_shape = x.shape
+        return rows.sum()
+
+    @staticmethod
+    def backward(ctx, g):
+        dx, dw = _LMHeadCE.backward(ctx, g)[:2]
+        return dx, dw, None, None, None, None
+
+
+class _DistillCPU(Function):
+    @staticmethod
+    def forward(ctx, logits, index, teacher, temperature, weight):
+        rows, grad = distill_topk(logits, index, teacher, temperature, weight)
+        ctx.save_for_backward(grad)
+        return rows.sum()
+
+    @staticmethod
+    def backward(ctx, g):
+        return ctx.saved_tensors[0] * g, None, None, None, None
+
+
+def distill_topk_lmhead(x, w, index, teacher, temperature: float = 1.0, weight=None):
+    """Distillation loss of softmax(x @ w^T) against a teacher's top logits (``distill_topk``), summed with ``weight``
+    [N] (default 1 / N: the mean). The logits buffer is overwritten by its own gradient, as in
+    ``cross_entropy_lmhead``; index and teacher are [N, K] over the flattened rows of x."""
+    if weight is None:
+        n = x.numel() // x.shape[-1]
+        weight = torch.full((n,), 1.0 / max(n, 1), dtype=torch.float32, device=x.device)
+    if not x.is_cuda:
+        return _DistillCPU.apply(F.linear(x.reshape(-1, x.shape[-1]), w), index, teacher, float(temperature), weight)
+    _gate(w)
+    return _LMHeadDistill.apply(x, w, index, teacher, temperature, weight)

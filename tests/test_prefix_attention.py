@@ -1,0 +1,226 @@
+"""Attention behind a prefix that the whole batch shares (``ops.prefix_attention``) against one softmax in 64 bits over
+prefix and own keys: head layouts, one to many tokens, lengths on and around the 32-key blocks and 128-key steps,
+empty prefixes and sequences, stale and non-finite cache rows behind each length, strides, refusals, captured calls.
+
+Tolerance per output, with A = sum_j p_j |v_j|: P is rounded to bf16 before its product with V (2^-8 A), the output once more
+(2^-8 |o|); a score is an fp32 sum of D products, scaled (D + 4 roundings of sum |q||k| scale), and the exponential's
+argument carries two more roundings of its size, so p is off by e = ((D + 4) max_j sum |q k_j| scale + 4 max |s|) 2^-24 + 2^-22
+relative, in the numerator and in the denominator; sums over n keys in fp32 add n 2^-24 to each."""
+import math
+
+import pytest
+import torch
+
+from kubeoperator_amd.ops import functional as kf
+
+DEVS = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+U = 2.0 ** -24
+
+
+def make(B, T, Hq, Hkv, D, P, Smax, dev, seed=0, size=1.0):
+    g = torch.Generator().manual_seed(seed)
+    rnd = lambda *s: torch.randn(*s, generator=g).bfloat16()  # noqa: E731
+    qkv = size * rnd(B * T, (Hq + 2 * Hkv) * D)
+    return [t.to(dev) for t in (qkv, rnd(Hkv, P, D), rnd(Hkv, P, D), rnd(B, Hkv, Smax, D), rnd(B, Hkv, Smax, D))]
+
+
+def oracle(q, kp, vp, kc, vc, lens, max_len, T, scale):
+    B, Hkv, _, D = kc.shape
+    Hq = q.shape[1] // D
+    dev = q.device if q.numel() * (kp.shape[1] + max_len) > 1 << 20 else "cpu"
+    q, kp, vp, kc, vc = (t.to(dev).double() for t in (q, kp, vp, kc, vc))
+    out = torch.zeros(B * T, Hq, D, dtype=torch.float64, device=dev)
+    tol = torch.zeros_like(out)
+    for b in range(B):
+        n = min(max(int(lens[b]), 0), max_len)
+        for t in range(T):
+            own = max(n - (T - 1 - t), 0)
+            k = torch.cat([kp, kc[b, :, :own]], 1).repeat_interleave(Hq // Hkv, 0)
+            v = torch.cat([vp, vc[b, :, :own]], 1).repeat_interleave(Hq // Hkv, 0)
+            if not k.shape[1]:
+                continue
+            row = q[b * T + t].view(Hq, D, 1)
+            s = (k @ row).squeeze(-1) * scale
+            p = torch.softmax(s, -1).unsqueeze(1)
+            o, A = (p @ v).squeeze(1), (p @ v.abs()).squeeze(1)
+            e = ((D + 4) * (k.abs() @ row.abs()).squeeze(-1).amax(-1) * scale + 4 * s.abs().amax(-1)) * U + 2.0 ** -22 + k.shape[1] * U
+            out[b * T + t] = o
+            tol[b * T + t] = (2.0 ** -8 + 2 * e.unsqueeze(-1)) * A * (1 + 2.0 ** -7) + 2.0 ** -8 * o.abs()
+    return out.view(B * T, Hq * D).cpu(), tol.view(B * T, Hq * D).cpu()
+
+
+def check(q, kp, vp, kc, vc, lens, max_len, T, scale=None):
+    D = kc.shape[-1]
+    want, tol = oracle(q, kp, vp, kc, vc, lens, max_len, T, scale or 1 / math.sqrt(D))
+    got = kf.prefix_attention(q, kp, vp, kc, vc, lens, max_len, T, scale)
+    assert got.dtype == torch.bfloat16 and got.shape == want.shape
+    err = (got.double().cpu() - want).abs() - tol
+    assert err.max() <= 0, (err.max(), torch.nonzero(err > 0)[:5])
+    return got
+
+
+def run(B, T, Hq, Hkv, D, P, lens, dev, seed=0, stale=float("nan"), size=1.0):
+    Smax = max(max(lens), 1) + 5
+    qkv, kp, vp, kc, vc = make(B, T, Hq, Hkv, D, P, Smax, dev, seed, size)
+    for b, n in enumerate(lens):
+        kc[b, :, max(n, 0):] = stale
+        vc[b, :, max(n, 0):] = stale
+    return check(qkv[:, : Hq * D], kp, vp, kc, vc, torch.tensor(lens, dtype=torch.int32, device=dev), max(max(lens), 0), T)
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("Hq,Hkv,D", [(4, 2, 64), (12, 12, 64), (8, 2, 128), (6, 2, 128), (5, 1, 64), (16, 1, 128)])
+@pytest.mark.parametrize("P", [0, 1, 33, 200])
+@pytest.mark.parametrize("T", [1, 3])
+def test_heads_prefixes_and_tokens(dev, Hq, Hkv, D, P, T):
+    run(4, T, Hq, Hkv, D, P, [T, 31 + T, 128, 130], dev, seed=P + T)
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("T", [1, 2, 5, 8, 40])
+@pytest.mark.parametrize("n", [40, 63, 64, 65, 127, 128, 129, 161])
+def test_lengths_around_blocks(dev, T, n):
+    run(2, T, 8, 2, 64, n, [n, n + 1], dev, seed=n)
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("P", [0, 70])
+def test_empty_short_and_overlong_sequences(dev, P):
+    """Lengths of 0, below the token count (the first tokens see the prefix alone, or nothing: 0) and past max_len."""
+    T, Hq, Hkv, D = 4, 8, 4, 64
+    qkv, kp, vp, kc, vc = make(6, T, Hq, Hkv, D, P, 90, dev)
+    lens = torch.tensor([0, 1, 3, 4, 500, -3], dtype=torch.int32, device=dev)
+    got = check(qkv[:, : Hq * D], kp, vp, kc, vc, lens, 77, T)
+    if P == 0:
+        assert not got[:T].any() and not got[T:2 * T - 1].any() and got[2 * T - 1].any() and not got[-T:].any()
+    none = kf.prefix_attention(qkv[:, : Hq * D], kp, vp, kc, vc, lens * 0, 0, T)  # no own keys at all
+    if P == 0:
+        assert not none.any()
+    else:
+        check(qkv[:, : Hq * D], kp, vp, kc, vc, lens * 0, 0, T)
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_masked_keys_that_are_not_finite(dev, bad):
+    """Keys of later tokens hold NaN / inf: earlier tokens' rows are those of a finite cache, bit for bit."""
+    T, Hq, Hkv, D, P = 4, 8, 2, 128, 50
+    for n in (4, 33, 64, 100):
+        qkv, kp, vp, kc, vc = make(2, T, Hq, Hkv, D, P, 128, dev, seed=n)
+        q, lens = qkv[:, : Hq * D], torch.full((2,), n, dtype=torch.int32, device=dev)
+        want = kf.prefix_attention(q, kp, vp, kc, vc, lens, n, T).view(2, T, -1)
+        for what in ("k", "v", "both"):
+            k2, v2 = kc.clone(), vc.clone()
+            if what != "v":
+                k2[:, :, n - 2] = bad
+            if what != "k":
+                v2[:, :, n - 2] = bad
+            got = kf.prefix_attention(q, kp, vp, k2, v2, lens, n, T).view(2, T, -1)
+            assert torch.equal(got[:, :2], want[:, :2]), (n, what)  # tokens 0 and 1 do not see key n - 2
+            if what == "v":
+                assert not torch.isfinite(got[:, 2:].float()).any()
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_strided_prefix_and_slots(dev):
+    """The prefix as a slot of another cache ([Hkv, Smax, D] cut to P rows), and as rows of a fused [P, Hkv, D] tensor."""
+    Hq, Hkv, D, P = 8, 4, 64, 100
+    qkv, kp, vp, kc, vc = make(3, 1, Hq, Hkv, D, P, 64, dev)
+    lens = torch.tensor([5, 64, 33], dtype=torch.int32, device=dev)
+    q = qkv[:, : Hq * D]
+    want = check(q, kp, vp, kc, vc, lens, 64, 1)
+    slot = torch.full((2, 2, Hkv, P + 28, D), float("nan"), dtype=torch.bfloat16, device=dev)
+    slot[0, 1, :, :P], slot[1, 1, :, :P] = kp, vp
+    assert torch.equal(kf.prefix_attention(q, slot[0, 1, :, :P], slot[1, 1, :, :P], kc, vc, lens, 64), want)
+    rows = torch.stack([kp.transpose(0, 1), vp.transpose(0, 1)], 1).contiguous()  # [P, 2, Hkv, D]
+    assert torch.equal(kf.prefix_attention(q, rows[:, 0].transpose(0, 1), rows[:, 1].transpose(0, 1), kc, vc, lens, 64), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,T,Hq,Hkv,D,P,own", [(64, 1, 32, 8, 128, 2048, 500), (24, 5, 32, 8, 128, 3000, 300), (1, 1, 32, 8, 128, 8192, 2000),
+                                                (128, 1, 12, 12, 64, 777, 64), (3, 128, 8, 2, 64, 513, 128), (2, 300, 32, 8, 128, 130, 333),
+                                                (96, 8, 4, 2, 64, 5000, 40), (2, 1, 64, 8, 128, 1, 3000), (40, 2, 16, 2, 64, 1500, 200),
+                                                (33, 7, 6, 2, 128, 999, 77)])
+def test_serving_sizes(B, T, Hq, Hkv, D, P, own):
+    lens = [T + (b * (own - T)) // max(B - 1, 1) for b in range(B)]
+    run(B, T, Hq, Hkv, D, P, lens, "cuda", seed=B)
+
+
+@pytest.mark.gpu
+def test_large_scores():
+    """Scores of several hundred: one key holds nearly everything, maxima that move from block to block."""
+    run(8, 2, 8, 2, 128, 700, [2, 40, 90, 128, 129, 200, 300, 256], "cuda", size=32.0)
+
+
+@pytest.mark.gpu
+def test_agrees_with_decode_attention():
+    """Without a prefix and for one token it is the framework's decode attention; with the prefix copied in front of every
+    sequence's own keys, decode attention over the whole cache gives the same."""
+    B, Hq, Hkv, D, P = 5, 32, 8, 128, 300
+    qkv, kp, vp, kc, vc = make(B, 1, Hq, Hkv, D, P, 200, "cuda")
+    lens = torch.tensor([1, 50, 128, 199, 200], dtype=torch.int32, device="cuda")
+    q = qkv[:, : Hq * D]
+    full_k, full_v = (torch.cat([p.expand(B, Hkv, P, D), c], 2).contiguous() for p, c in ((kp, kc), (vp, vc)))
+    for a, b in ((kf.prefix_attention(q, kp[:, :0], vp[:, :0], kc, vc, lens, 200), kf.decode_attention(q, kc, vc, lens, 200)),
+                 (kf.prefix_attention(q, kp, vp, kc, vc, lens, 200), kf.decode_attention(q, full_k, full_v, lens + P, 200 + P))):
+        # both round P (2^-8 A, A <= max |v|) and the output
+        assert (a.float() - b.float()).abs().max() <= 4 * 2.0 ** -8 * float(max(vp.abs().max(), vc.abs().max()))
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_refusals(dev):
+    Hq, Hkv, D, P, B = 4, 2, 64, 20, 3
+    qkv, kp, vp, kc, vc = make(B, 1, Hq, Hkv, D, P, 32, dev)
+    q, lens = qkv[:, : Hq * D], torch.tensor([1, 2, 3], dtype=torch.int32, device=dev)
+    f = kf.prefix_attention
+    bad = [
+        lambda: f(q, kp, vp[:, :19], kc, vc, lens, 32),
+        lambda: f(q, kp[:1], vp[:1], kc, vc, lens, 32),
+        lambda: f(q, kp, vp, kc, vc[:, :, :31], lens, 32),
+        lambda: f(q, kp, vp, kc, vc, lens, 33),
+        lambda: f(q, kp, vp, kc, vc, lens, -1),
+        lambda: f(q, kp, vp, kc, vc, lens.long(), 32),
+        lambda: f(q, kp, vp, kc, vc, lens[:2], 32),
+        lambda: f(q, kp, vp, kc, vc, lens, 32, 2),
+        lambda: f(q, kp, vp, kc, vc, lens, 32, 0),
+        lambda: f(q[:, :192], kp, vp, kc, vc, lens, 32),
+        lambda: f(q[:2], kp, vp, kc, vc, lens, 32),
+        lambda: f(q.reshape(B, Hq, D), kp, vp, kc, vc, lens, 32),
+        lambda: f(q[:, :64 * 2], kp[..., :32], vp[..., :32], kc[..., :32].contiguous(), vc[..., :32].contiguous(), lens, 32),
+        lambda: f(q.clone().requires_grad_(), kp, vp, kc, vc, lens, 32),
+    ]
+    if dev == "cuda":
+        bad += [lambda: f(q.float(), kp, vp, kc, vc, lens, 32), lambda: f(q, kp.cpu(), vp, kc, vc, lens, 32),
+                lambda: f(q, kp, vp, kc, vc, lens.cpu(), 32), lambda: f(q, kp, vp, kc[:, :, ::2], vc[:, :, ::2], lens, 16),
+                lambda: f(q, kp.transpose(1, 2).contiguous().transpose(1, 2), vp, kc, vc, lens, 32)]
+    for g in bad:
+        with pytest.raises(RuntimeError):
+            g()
+    assert f(q[:0], kp, vp, kc[:0], vc[:0], lens[:0], 32).shape == (0, Hq * D)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,T,P", [(4, 1, 500), (48, 4, 700)])
+def test_captured_call_replays_and_another_stream(B, T, P):
+    Hq, Hkv, D = 8, 2, 128
+    qkv, kp, vp, kc, vc = make(B, T, Hq, Hkv, D, P, 200, "cuda")
+    lens = torch.randint(T, 201, (B,), dtype=torch.int32, device="cuda")
+    args = (qkv[:, : Hq * D], kp, vp, kc, vc, lens, 200, T)
+    want = kf.prefix_attention(*args)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        other = kf.prefix_attention(*args)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(other, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = kf.prefix_attention(*args)
+    for seed in range(3):
+        for a, b in zip((qkv, kp, vp, kc, vc), make(B, T, Hq, Hkv, D, P, 200, "cuda", seed=seed)):
+            a.copy_(b)
+        lens.copy_(torch.randint(0, 201, (B,), dtype=torch.int32, device="cuda"))
+        eager = kf.prefix_attention(*args)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, eager)
