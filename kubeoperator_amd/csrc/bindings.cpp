@@ -678,7 +678,7 @@ Tensor lora_add(const Tensor& y, const Tensor& x, const Tensor& a, const Tensor&
     out = at::empty({M, N}, y.options());
   }
   if (M == 0) return out;
-  auto ws = at::empty({kop::lora_workspace(M, (int)K, (int)r)}, y.options().dtype(at::kByte));
+  auto ws = at::empty({kop::lora_workspace(M, (int)K, (int)N, (int)n, (int)r)}, y.options().dtype(at::kByte));
   rc(kop::lora_add(bp(y), y.stride(0), bp(x), x.stride(0), bp(a), bp(b), index.data_ptr<int>(), scale.data_ptr<float>(),
                    bp(out), out.stride(0), M, (int)K, (int)N, (int)n, (int)r, ws.data_ptr(), cur_stream()),
      "lora_add");

@@ -15,136 +15,262 @@ namespace kop {
 namespace {
 constexpr float kL2E = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-}  // namespace
 
-// one workgroup per row, two passes: running (max, sum) in the log2 domain, then the gradient
-template <int NT, bool VEC>
-__global__ void __launch_bounds__(NT) distill_kernel(const bf16_t* logits, int64_t ld, int V,
-                                                     const int* __restrict__ index, const float* __restrict__ teacher,
-                                                     int K, const float* __restrict__ weight, float temp,
-                                                     float* __restrict__ loss, bf16_t* grad, int64_t gld) {
-  __shared__ float red[NT / 64];
-  __shared__ int s_idx[kDistillMaxK];
-  __shared__ float s_p[kDistillMaxK], s_x[kDistillMaxK];
-  const int64_t row = blockIdx.x;
-  const bf16_t* x = logits + row * ld;
-  bf16_t* gx = grad + row * gld;
-  const int t = threadIdx.x;
-  const float w = weight ? weight[row] : 1.f;
-  const float c = kL2E / temp;
-  // teacher: the row's maximum over its real entries
-  float tm = -INFINITY;
-  for (int k = t; k < K; k += NT) {
-    const int i = index[row * K + k];
-    float v = teacher[row * K + k];
-    const bool real = i >= 0 && i < V && v == v && v > -INFINITY;
-    if (!real) v = -INFINITY;
-    s_idx[k] = real ? i : -1;
-    s_p[k] = v;
-    s_x[k] = real ? bf2f(x[i]) : 0.f;
-    tm = fmaxf(tm, v);
+// 8 logits of a row at element i, a multiple of 8 (rows may start off the 16-byte grid: global accesses take any element's
+// alignment); 32-bit byte offsets keep the row's base in scalar registers
+struct __attribute__((packed, aligned(2))) U16 {
+  u32x4 v;
+};
+__device__ __forceinline__ u32x4 load8(const bf16_t* x, uint32_t i) {
+  return reinterpret_cast<const U16*>(reinterpret_cast<const char*>(x) + 2 * i)->v;
+}
+__device__ __forceinline__ void store8(bf16_t* x, uint32_t i, const float* f) {
+  reinterpret_cast<U16*>(reinterpret_cast<char*>(x) + 2 * i)->v = pack8(f);
+}
+__device__ __forceinline__ float max8(const float* f) {
+  return fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
+}
+
+// The teacher's side of a row and the listed tokens' logits, in LDS.
+template <int NT>
+struct Teacher {
+  int idx[kDistillMaxK];    // -1: padding
+  float p[kDistillMaxK];    // logit, then probability
+  float x[kDistillMaxK];    // the student's logit of the token
+  float red[NT / 64];
+
+  // the row's entries; returns the largest teacher logit (-inf: all padding), in every thread
+  __device__ __forceinline__ float load(const bf16_t* xr, int V, const int* index, const float* teacher, int K) {
+    float m = -INFINITY;
+    for (int k = threadIdx.x; k < K; k += NT) {
+      const int i = index[k];
+      float v = teacher[k];
+      const bool real = i >= 0 && i < V && v > -INFINITY;  // false for NaN
+      v = real ? v : -INFINITY;
+      idx[k] = real ? i : -1;
+      p[k] = v;
+      x[k] = real ? bf2f(xr[i]) : 0.f;
+      m = fmaxf(m, v);
+    }
+    return block_max<NT / 64>(m, red);
   }
-  tm = block_max<NT / 64>(tm, red);
-  const bool live = tm > -INFINITY && w != 0.f;  // uniform over the workgroup
-  if (!live) {
-    if (t == 0) loss[row] = 0.f;
-    const int V8 = VEC ? V >> 3 : 0;
-    for (int i = t; i < V8; i += NT) reinterpret_cast<u32x4*>(gx)[i] = u32x4{0u, 0u, 0u, 0u};
-    for (int i = V8 * 8 + t; i < V; i += NT) gx[i] = 0;
+  // p = softmax; returns the loss in units of log2 without its factors. lse2: log2 of the student's sum, c = log2 e / temp
+  __device__ __forceinline__ float finish(int K, float tm, float c, float lse2, bool some) {
+    float s = 0.f;
+    for (int k = threadIdx.x; k < K; k += NT) s += idx[k] >= 0 ? __builtin_amdgcn_exp2f((p[k] - tm) * c) : 0.f;
+    __syncthreads();  // red may still be read
+    s = block_sum<NT / 64>(s, red);
+    const float ls = __log2f(s);
+    float part = 0.f;
+    for (int k = threadIdx.x; k < K; k += NT) {
+      const float lp = (p[k] - tm) * c - ls;
+      const float e = idx[k] >= 0 ? __builtin_amdgcn_exp2f(lp) : 0.f;
+      p[k] = e;
+      if (e > 0.f) part += e * (lp - (some ? fmaf(x[k], c, -lse2) : -INFINITY));
+    }
+    __syncthreads();
+    return block_sum<NT / 64>(part, red);
+  }
+  // the listed tokens' own elements, once every element of the row has been written. A token listed more than once: its
+  // entries' sum, written by the first of them
+  __device__ __forceinline__ void patch(int K, float c, float lse2, float gw, bf16_t* gx) {
+    __syncthreads();
+    for (int k = threadIdx.x; k < K; k += NT) {
+      const int i = idx[k];
+      if (i < 0) continue;
+      float sum = 0.f;
+      bool first = true;
+      for (int j = 0; j < K; ++j) {
+        const bool same = idx[j] == i;
+        sum += same ? p[j] : 0.f;
+        first = first && !(same && j < k);
+      }
+      if (first) gx[i] = f2bf(gw * (__builtin_amdgcn_exp2f(fmaf(x[k], c, -lse2)) - sum));
+    }
+  }
+};
+
+struct Args {
+  const bf16_t* logits;
+  int64_t ld;
+  int V, K;
+  const int* index;
+  const float *teacher, *weight;
+  float temp;
+  float* loss;
+  bf16_t* grad;
+  int64_t gld;
+};
+// rows without a loss: zeros
+template <int NT>
+__device__ __forceinline__ void no_loss(const Args& a, int64_t row, bf16_t* gx) {
+  const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const uint32_t V8 = a.V & ~7u;
+  if (threadIdx.x == 0) a.loss[row] = 0.f;
+  for (uint32_t i = threadIdx.x * 8; i < V8; i += NT * 8) store8(gx, i, z);
+  if (V8 + threadIdx.x < (uint32_t)a.V) gx[V8 + threadIdx.x] = 0;
+}
+
+// keeps the compiler from carrying a pass's unpacked floats (twice the registers) over to the next pass
+template <int N>
+__device__ __forceinline__ void repack(u32x4* v) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) asm volatile("" : "+v"(v[j]));
+}
+
+// One workgroup per row that holds the whole row: CR 16-byte pieces per thread in registers, CL more in LDS, so every
+// logit is read once and every gradient element written once. Two plain reductions, no running rescale.
+template <int NT, int CR, int CL>
+__global__ void __launch_bounds__(NT, CL > 0 ? 4 : 1) distill_row_kernel(Args a) {
+  __shared__ Teacher<NT> s_t;
+  __shared__ u32x4 s_w[CL > 0 ? CL * NT : 1];
+  const int t = threadIdx.x;
+  const int64_t row = blockIdx.x;
+  const bf16_t* x = a.logits + row * a.ld;
+  bf16_t* gx = a.grad + row * a.gld;
+  const float w = a.weight ? a.weight[row] : 1.f;
+  const float c = kL2E / a.temp;
+  // pieces j * NT + t of 8 logits; the up to 7 logits behind the last whole piece: one each for the first threads
+  const uint32_t V8 = a.V & ~7u;
+  const bool tail = V8 + t < (uint32_t)a.V;
+  constexpr uint32_t kPad = 0xff80ff80u;  // two bf16 -inf
+  u32x4 v[CR];
+  static_assert(CL % 3 == 0, "LDS pieces are loaded three at a time");
+#pragma unroll 1
+  for (int j = 0; j < CL; j += 3) {
+    u32x4 q[3];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      const uint32_t i = ((CR + j + k) * NT + t) * 8;
+      q[k] = u32x4{kPad, kPad, kPad, kPad};
+      if (i < V8) q[k] = load8(x, i);
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) s_w[(j + k) * NT + t] = q[k];
+  }
+#pragma unroll
+  for (int j = 0; j < CR; ++j) {
+    const uint32_t i = (j * NT + t) * 8;
+    v[j] = u32x4{kPad, kPad, kPad, kPad};
+    if (i < V8) v[j] = load8(x, i);
+  }
+  const float xt = tail ? bf2f(x[V8 + t]) : -INFINITY;
+  const float tm = s_t.load(x, a.V, a.index + row * a.K, a.teacher + row * a.K, a.K);
+  if (!(tm > -INFINITY && w != 0.f)) {
+    no_loss<NT>(a, row, gx);
     return;
   }
-  float ts = 0.f;
-  for (int k = t; k < K; k += NT) {
-    const float e = s_idx[k] >= 0 ? __builtin_amdgcn_exp2f((s_p[k] - tm) * c) : 0.f;
-    ts += e;
+  float m = xt;
+  float f[8];
+#pragma unroll 1
+  for (int j = 0; j < CL; ++j) {
+    unpack8(s_w[j * NT + t], f);
+    m = fmaxf(m, max8(f));
+  }
+#pragma unroll
+  for (int j = 0; j < CR; ++j) {
+    unpack8(v[j], f);
+    m = fmaxf(m, max8(f));
   }
   __syncthreads();
-  ts = block_sum<NT / 64>(ts, red);
-  const float tl2 = __log2f(ts);  // log2 of the teacher's sum
-  // student: running maximum and sum
-  const int V8 = VEC ? V >> 3 : 0;
-  const u32x4* xv = reinterpret_cast<const u32x4*>(x);
-  float m = -INFINITY, s = 0.f;
-  for (int i = t; i < V8; i += NT) {
-    float f[8];
-    unpack8(xv[i], f);
-    const float cm = fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
-    const float nm = fmaxf(m, cm);
+  m = block_max<NT / 64>(m, s_t.red);
+  const bool some = m > -INFINITY;  // false: every logit is -inf, q = 0
+  const float nb = some ? -m * c : 0.f;
+  repack<CR>(v);
+  float s = __builtin_amdgcn_exp2f(fmaf(xt, c, nb));
+#pragma unroll 1
+  for (int j = 0; j < CL; ++j) {
+    unpack8(s_w[j * NT + t], f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += __builtin_amdgcn_exp2f(fmaf(f[e], c, nb));
+  }
+#pragma unroll
+  for (int j = 0; j < CR; ++j) {
+    unpack8(v[j], f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += __builtin_amdgcn_exp2f(fmaf(f[e], c, nb));
+  }
+  __syncthreads();
+  s = block_sum<NT / 64>(s, s_t.red);
+  const float lse2 = some ? fmaf(m, c, __log2f(s)) : INFINITY;  // log2 of the student's sum of exp(logit / t)
+  const float part = s_t.finish(a.K, tm, c, lse2, some);
+  if (t == 0) a.loss[row] = part * kLn2 * a.temp * a.temp * w;
+  const float gw = a.temp * w;
+  repack<CR>(v);
+  auto put = [&](u32x4 q, uint32_t i) {
+    unpack8(q, f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = gw * __builtin_amdgcn_exp2f(fmaf(f[e], c, -lse2));
+    if (i < V8) store8(gx, i, f);
+  };
+#pragma unroll
+  for (int j = 0; j < CR; ++j) put(v[j], (j * NT + t) * 8);
+#pragma unroll 1
+  for (int j = 0; j < CL; ++j) put(s_w[j * NT + t], ((CR + j) * NT + t) * 8);
+  if (tail) gx[V8 + t] = f2bf(gw * __builtin_amdgcn_exp2f(fmaf(xt, c, -lse2)));
+  s_t.patch(a.K, c, lse2, gw, gx);
+}
+
+// Rows longer than that: two passes, running (maximum, sum) in the log2 domain, then the gradient
+template <int NT>
+__global__ void __launch_bounds__(NT) distill_long_kernel(Args a) {
+  __shared__ Teacher<NT> s_t;
+  const int t = threadIdx.x;
+  const int64_t row = blockIdx.x;
+  const bf16_t* x = a.logits + row * a.ld;
+  bf16_t* gx = a.grad + row * a.gld;
+  const float w = a.weight ? a.weight[row] : 1.f;
+  const float c = kL2E / a.temp;
+  const uint32_t V8 = a.V & ~7u;
+  const bool tail = V8 + t < (uint32_t)a.V;
+  const float xt = tail ? bf2f(x[V8 + t]) : -INFINITY;
+  const float tm = s_t.load(x, a.V, a.index + row * a.K, a.teacher + row * a.K, a.K);
+  if (!(tm > -INFINITY && w != 0.f)) {
+    no_loss<NT>(a, row, gx);
+    return;
+  }
+  float m = xt, s = xt > -INFINITY ? 1.f : 0.f, f[8];
+  for (uint32_t i = t * 8; i < V8; i += NT * 8) {
+    unpack8(load8(x, i), f);
+    const float nm = fmaxf(m, max8(f));
     if (nm == -INFINITY) continue;
     const float nb = -nm * c;
     float add = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) add += __builtin_amdgcn_exp2f(fmaf(f[e], c, nb));
-    s = (m == -INFINITY ? 0.f : s * __builtin_amdgcn_exp2f((m - nm) * c)) + add;
-    m = nm;
-  }
-  for (int i = V8 * 8 + t; i < V; i += NT) {
-    const float f = bf2f(x[i]);
-    const float nm = fmaxf(m, f);
-    if (nm == -INFINITY) continue;
-    s = (m == -INFINITY ? 0.f : s * __builtin_amdgcn_exp2f((m - nm) * c)) + __builtin_amdgcn_exp2f((f - nm) * c);
+    s = s * __builtin_amdgcn_exp2f((m - nm) * c) + add;  // m = -inf: times 0
     m = nm;
   }
   __syncthreads();
-  const float M = block_max<NT / 64>(m, red);
+  const float M = block_max<NT / 64>(m, s_t.red);
   __syncthreads();
-  s = block_sum<NT / 64>(m == -INFINITY ? 0.f : s * __builtin_amdgcn_exp2f((m - M) * c), red);
-  const bool some = M > -INFINITY;                              // false: every logit is -inf, q = 0
-  const float lse2 = some ? fmaf(M, c, __log2f(s)) : INFINITY;  // log2 of the student's sum of exp(logit / t)
-  // loss: p_k (log2 p_k - log2 q_k) summed, in nats at the end
-  float part = 0.f;
-  for (int k = t; k < K; k += NT) {
-    if (s_idx[k] < 0) {
-      s_p[k] = 0.f;
-      continue;
-    }
-    const float lp = (s_p[k] - tm) * c - tl2;
-    const float p = __builtin_amdgcn_exp2f(lp);
-    s_p[k] = p;
-    const float lq = some ? fmaf(s_x[k], c, -lse2) : -INFINITY;
-    if (p > 0.f) part += p * (lp - lq);
-  }
-  __syncthreads();
-  part = block_sum<NT / 64>(part, red);
-  if (t == 0) loss[row] = part * kLn2 * temp * temp * w;
-  // gradient: t w q for every logit, then the listed tokens' own elements
-  const float gw = temp * w;
-  u32x4* gv = reinterpret_cast<u32x4*>(gx);
-  for (int i = t; i < V8; i += NT) {
-    float f[8];
-    unpack8(xv[i], f);
+  s = block_sum<NT / 64>(m == -INFINITY ? 0.f : s * __builtin_amdgcn_exp2f((m - M) * c), s_t.red);
+  const bool some = M > -INFINITY;
+  const float lse2 = some ? fmaf(M, c, __log2f(s)) : INFINITY;
+  const float part = s_t.finish(a.K, tm, c, lse2, some);
+  if (t == 0) a.loss[row] = part * kLn2 * a.temp * a.temp * w;
+  const float gw = a.temp * w;
+  for (uint32_t i = t * 8; i < V8; i += NT * 8) {
+    unpack8(load8(x, i), f);
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] = gw * __builtin_amdgcn_exp2f(fmaf(f[e], c, -lse2));
-    gv[i] = pack8(f);
+    store8(gx, i, f);
   }
-  for (int i = V8 * 8 + t; i < V; i += NT) gx[i] = f2bf(gw * __builtin_amdgcn_exp2f(fmaf(bf2f(x[i]), c, -lse2)));
-  __syncthreads();  // every element has been written (and the LDS probabilities are complete)
-  for (int k = t; k < K; k += NT) {
-    const int i = s_idx[k];
-    if (i < 0) continue;
-    float p = 0.f;  // a token listed more than once: its entries' sum, written by the first of them
-    bool first = true;
-    for (int j = 0; j < K; ++j) {
-      const bool same = s_idx[j] == i;
-      p += same ? s_p[j] : 0.f;
-      first = first && !(same && j < k);
-    }
-    if (first) gx[i] = f2bf(gw * (__builtin_amdgcn_exp2f(fmaf(s_x[k], c, -lse2)) - p));
-  }
+  if (tail) gx[V8 + t] = f2bf(gw * __builtin_amdgcn_exp2f(fmaf(xt, c, -lse2)));
+  s_t.patch(a.K, c, lse2, gw, gx);
 }
+}  // namespace
 
 int distill_topk(const bf16_t* logits, int64_t ld, int64_t N, int V, const int* index, const float* teacher, int K,
                  const float* weight, float temp, float* loss, bf16_t* grad, int64_t gld, hipStream_t stream) {
-  if (K < 1 || K > kDistillMaxK || V < 1 || N < 0 || N > 0x7fffffff) return -1;
+  if (K < 1 || K > kDistillMaxK || V < 1 || V > 0x3fffffff || N < 0 || N > 0x7fffffff) return -1;
   if (N == 0) return 0;
-  const bool vec = ld % 8 == 0 && gld % 8 == 0 && reinterpret_cast<uintptr_t>(logits) % 16 == 0 &&
-                   reinterpret_cast<uintptr_t>(grad) % 16 == 0;
-  if (vec)
-    distill_kernel<512, true><<<(unsigned)N, 512, 0, stream>>>(logits, ld, V, index, teacher, K, weight, temp, loss, grad,
-                                                              gld);
-  else
-    distill_kernel<512, false><<<(unsigned)N, 512, 0, stream>>>(logits, ld, V, index, teacher, K, weight, temp, loss,
-                                                               grad, gld);
+  const Args a = {logits, ld, V, K, index, teacher, weight, temp, loss, grad, gld};
+  const unsigned n = (unsigned)N;
+  if (V < 256 * 8 * 4 + 8) distill_row_kernel<256, 4, 0><<<n, 256, 0, stream>>>(a);
+  else if (V < 512 * 8 * 16 + 8) distill_row_kernel<512, 16, 0><<<n, 512, 0, stream>>>(a);
+  else if (V < 512 * 8 * 32 + 8) distill_row_kernel<512, 23, 9><<<n, 512, 0, stream>>>(a);
+  else distill_long_kernel<512><<<n, 512, 0, stream>>>(a);
   return hipGetLastError() == hipSuccess ? 0 : -9;
 }
 

@@ -61,7 +61,7 @@ int verify_draft(const void* target, int64_t ts_b, int64_t ts_t, const void* dra
 // x [M, K], y / out [M, N] rows, a [n, r, K], b [n, N, r] contiguous, index [M] int32, scale [n] fp32.
 // workspace: lora_workspace() bytes. K, N, r multiples of 8, r <= kLoraMaxRank
 constexpr int kLoraMaxRank = 128;
-int64_t lora_workspace(int64_t M, int K, int r);
+int64_t lora_workspace(int64_t M, int K, int N, int n, int r);
 int lora_add(const bf16_t* y, int64_t ys, const bf16_t* x, int64_t xs, const bf16_t* a, const bf16_t* b,
              const int* index, const float* scale, bf16_t* out, int64_t os, int64_t M, int K, int N, int n, int r,
              void* workspace, hipStream_t stream);

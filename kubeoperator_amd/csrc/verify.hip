@@ -11,10 +11,10 @@
 // would move a noticeable share of those borders past it. A logit of -inf or NaN has probability 0; +inf counts as the
 // largest finite value. A row without any probability accepts nothing and yields -1.
 //
-// Three launches: per-chunk maximum and sum of every row (the only pass over all logits); acceptance and the chunk sums of
-// r (the two rows of each sequence's refusal, again); the pick inside the one chunk that u_T falls into. Every
-// workgroup that needs the acceptance re-derives it from the chunk statistics (a few hundred numbers): no atomics, no
-// order-dependent sums.
+// Three launches (greedy: two): maximum and sum of every 8192-logit chunk (the only pass over all logits, each held in
+// registers between its maximum and its sum); acceptance and the sums of r over 1024-logit pieces (the two rows of each
+// sequence's refusal, again); the pick inside the one piece that u_T falls into. A workgroup that needs the acceptance
+// re-derives it from the chunk statistics (a few hundred numbers): no atomics, no order-dependent sums.
 #include <float.h>
 
 #include "common.h"
@@ -24,6 +24,8 @@ namespace kop {
 
 namespace {
 constexpr int kT = 256;       // threads of a workgroup
+constexpr int kChunk = 8192;  // logits per workgroup of the first pass: 32 per thread
+constexpr int kPiece = 1024;  // logits per wave of the second pass, per workgroup of the third
 constexpr int kMaxRows = 2 * kVerifyMaxDraft + 1;
 
 template <typename E>
@@ -33,17 +35,60 @@ __device__ __forceinline__ float ld1<float>(const float* p) { return *p; }
 template <>
 __device__ __forceinline__ float ld1<bf16_t>(const bf16_t* p) { return bf2f(*p); }
 
-// NaN -> -inf (no probability), +inf -> the largest finite value
-__device__ __forceinline__ float clean(float z) { return z != z ? -INFINITY : fminf(z, FLT_MAX); }
+// 16 bytes of a row; rows of odd length start off the 16-byte grid (global loads take any element's alignment)
+template <typename E>
+struct Vec {
+  static constexpr int N = 16 / sizeof(E);
+  struct __attribute__((packed, aligned(sizeof(E)))) U {
+    u32x4 v;
+  };
+  u32x4 w;
+  // logits [i, i + N) of x, -inf at and past `end`
+  __device__ __forceinline__ void load(const E* x, int i, int end) {
+    if (i + N <= end) {
+      w = reinterpret_cast<const U*>(x + i)->v;
+      return;
+    }
+    constexpr uint32_t pad = sizeof(E) == 4 ? 0xff800000u : 0xff80ff80u;
+    w = u32x4{pad, pad, pad, pad};
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (i + k < end) {
+        if constexpr (sizeof(E) == 4) w[k] = __float_as_uint(x[i + k]);
+        else w[k >> 1] = (k & 1) ? (w[k >> 1] & 0xffffu) | ((uint32_t)x[i + k] << 16) : (w[k >> 1] & 0xffff0000u) | x[i + k];
+      }
+  }
+  __device__ __forceinline__ float get(int k) const {
+    if constexpr (sizeof(E) == 4) return __uint_as_float(w[k]);
+    else return __uint_as_float((k & 1) ? w[k >> 1] & 0xffff0000u : w[k >> 1] << 16);
+  }
+};
+
+// 2^x for x <= 0 in 64 bits: 2^n times a degree-9 polynomial of the fraction (Chebyshev interpolation of 2^f on
+// [-1/2, 1/2], 2e-14 relative). NaN and everything below -1100 give 0, everything above 0 gives 1 -- which is what logits of
+// NaN, -inf and +inf are to weigh.
+__device__ __forceinline__ double exp2_neg(double x) {
+  x = fmin(fmax(x, -1100.0), 0.0);
+  const double n = rint(x), f = x - n;
+  double y = 0x1.b6557c7da8ca4p-24;
+  y = fma(y, f, 0x1.63efd536dcb25p-20);
+  y = fma(y, f, 0x1.ffcb7a04d3b13p-17);
+  y = fma(y, f, 0x1.43088df6dd4a7p-13);
+  y = fma(y, f, 0x1.5d87fe8e6c4b1p-10);
+  y = fma(y, f, 0x1.3b2ab72b2b245p-7);
+  y = fma(y, f, 0x1.c6b08d7045e60p-5);
+  y = fma(y, f, 0x1.ebfbdff814945p-3);
+  y = fma(y, f, 0x1.62e42fefa39e9p-1);
+  y = fma(y, f, 0x1.000000000003dp+0);
+  return __builtin_amdgcn_ldexp(y, (int)n);
+}
+// e^((z - m) / temp): c = log2 e / temp. The difference of two fp32 values is exact in 64 bits (or far below 2^-1100)
+__device__ __forceinline__ double weight(float z, float m, double c) { return exp2_neg(((double)z - (double)m) * c); }
 
 __device__ __forceinline__ double wave_sum_d(double v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
   return v;
-}
-// e^((z - m) / temp) in 64 bits; 0 for z = -inf
-__device__ __forceinline__ double weight(float z, float m, double inv_temp) {
-  return z == -INFINITY ? 0.0 : exp(((double)z - (double)m) * inv_temp);
 }
 
 struct Args {
@@ -53,13 +98,13 @@ struct Args {
   const int64_t* tokens;
   const float* u;
   const int* n_draft;  // null: T
-  int B, T, V, nch, chunk;
-  double inv_temp;  // 0: greedy
-  float* pm;        // [B, 2T+1, nch] chunk maximum (rows 0..T target, T+1..2T draft)
-  double* ps;       // [B, 2T+1, nch] sum of weights relative to the chunk maximum; greedy: the argmax's index
-  double* pr;       // [B, nch] chunk sums of r
-  int64_t* out;     // [B, T+1]
-  int* accepted;    // [B]
+  int B, T, V, nch, npc;  // chunks and pieces of a row
+  double c;               // log2 e / temp
+  double* ps;             // [B, 2T+1, nch] sums relative to the chunk's maximum; greedy: the argmax's index
+  double* pr;             // [B, npc] sums of r
+  float* pm;              // [B, 2T+1, nch] maxima (rows 0..T target, T+1..2T draft); -inf: an empty chunk
+  int64_t* out;           // [B, T+1]
+  int* accepted;          // [B]
 };
 __device__ __forceinline__ int drafts(const Args& a, int b) {
   return a.n_draft ? min(max(a.n_draft[b], 0), a.T) : a.T;
@@ -71,116 +116,119 @@ __device__ __forceinline__ const E* row_ptr(const Args& a, int b, int r) {
 }
 
 // ---- pass 1: grid (chunks, rows, B); greedy needs the target's T+1 rows only
-template <typename E>
+template <typename E, bool GREEDY>
 __global__ void __launch_bounds__(kT) verify_stats_kernel(Args a) {
+  constexpr int N = Vec<E>::N, NV = kChunk / (kT * N);
   __shared__ float s_m[kT / 64];
-  __shared__ int s_i[kT / 64];
   __shared__ double s_s[kT / 64];
   const int c = blockIdx.x, r = blockIdx.y, b = blockIdx.z, t = threadIdx.x;
   const int nd = drafts(a, b);
   if (r <= a.T ? r > nd : r - a.T - 1 >= nd) return;  // a row that no drafted token of this sequence needs
   const E* x = row_ptr<E>(a, b, r);
-  const int lo = c * a.chunk, hi = min(a.V, lo + a.chunk);
+  const int lo = c * kChunk, hi = min(a.V, lo + kChunk);
+  Vec<E> v[NV];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) v[k].load(x, lo + (k * kT + t) * N, hi);
   float m = -INFINITY;
-  int at = 0x7fffffff;
-  for (int i = lo + t; i < hi; i += kT) {
-    const float z = clean(ld1(x + i));
-    if (z > m) {
-      m = z;
-      at = i;
-    }
-  }
-  // the workgroup's maximum, at its lowest index
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const float om = __shfl_xor(m, o, 64);
-    const int oi = __shfl_xor(at, o, 64);
-    if (om > m || (om == m && oi < at)) {
-      m = om;
-      at = oi;
-    }
-  }
-  if ((t & 63) == 0) {
-    s_m[t >> 6] = m;
-    s_i[t >> 6] = at;
-  }
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int e = 0; e < N; ++e) m = fmaxf(m, v[k].get(e));  // a NaN is passed over
+  const float mine = m;
+  m = wave_max(m);
+  if ((t & 63) == 0) s_m[t >> 6] = m;
   __syncthreads();
-  m = s_m[0];
-  at = s_i[0];
-#pragma unroll
-  for (int w = 1; w < kT / 64; ++w)
-    if (s_m[w] > m || (s_m[w] == m && s_i[w] < at)) {
-      m = s_m[w];
-      at = s_i[w];
-    }
+  m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
   const int64_t o = ((int64_t)b * (2 * a.T + 1) + r) * a.nch + c;
-  if (a.inv_temp == 0.0) {
+  if constexpr (GREEDY) {
+    int at = 0x7fffffff;  // the lowest index that holds the maximum
+    if (mine == m && m > -INFINITY) {
+#pragma unroll
+      for (int k = NV - 1; k >= 0; --k)
+#pragma unroll
+        for (int e = N - 1; e >= 0; --e)
+          if (v[k].get(e) == m) at = lo + (k * kT + t) * N + e;
+    }
+#pragma unroll
+    for (int k = 32; k > 0; k >>= 1) at = min(at, __shfl_xor(at, k, 64));
+    if ((t & 63) == 0) s_s[t >> 6] = (double)at;
+    __syncthreads();
+    if (t == 0) {
+      a.pm[o] = fminf(m, FLT_MAX);
+      a.ps[o] = fmin(fmin(s_s[0], s_s[1]), fmin(s_s[2], s_s[3]));
+    }
+  } else {
+    m = fminf(m, FLT_MAX);
+    double s = 0.0;
+    if (m > -INFINITY) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int e = 0; e < N; ++e) s += weight(v[k].get(e), m, a.c);
+    }
+    s = wave_sum_d(s);
+    if ((t & 63) == 0) s_s[t >> 6] = s;
+    __syncthreads();
     if (t == 0) {
       a.pm[o] = m;
-      a.ps[o] = m == -INFINITY ? -1.0 : (double)at;
+      a.ps[o] = (s_s[0] + s_s[1]) + (s_s[2] + s_s[3]);
     }
-    return;
-  }
-  double s = 0.0;
-  if (m > -INFINITY)
-    for (int i = lo + t; i < hi; i += kT) s += weight(clean(ld1(x + i)), m, a.inv_temp);
-  s = wave_sum_d(s);
-  if ((t & 63) == 0) s_s[t >> 6] = s;
-  __syncthreads();
-  if (t == 0) {
-#pragma unroll
-    for (int w = 1; w < kT / 64; ++w) s += s_s[w];
-    a.pm[o] = m;
-    a.ps[o] = s;
   }
 }
 
-// The chunk statistics of sequence b's rows folded to one (maximum, sum) per row -- greedy: (maximum, argmax) -- and the
-// number of accepted tokens, in every thread. Called by whole workgroups.
-template <typename E>
-__device__ int decide(const Args& a, int b, float* s_m, double* s_s) {
-  const int t = threadIdx.x, wv = t >> 6, lane = t & 63;
+// Called by whole workgroups: the chunk statistics of sequence b's rows folded to one (maximum, sum) per row -- greedy:
+// (maximum, argmax or -1) -- by 16 lanes a row; returns the number of accepted tokens (one lane a token) in every thread.
+template <typename E, bool GREEDY>
+__device__ int decide(const Args& a, int b, float* s_m, double* s_s, int* s_j) {
+  const int t = threadIdx.x, sub = t & 15;
   const int nd = drafts(a, b), rows = 2 * a.T + 1;
-  for (int r = wv; r < (a.inv_temp == 0.0 ? a.T + 1 : rows); r += kT / 64) {
+  for (int r = t >> 4; r < (GREEDY ? a.T + 1 : rows); r += kT / 16) {
     if (r <= a.T ? r > nd : r - a.T - 1 >= nd) continue;
     const int64_t o = ((int64_t)b * rows + r) * a.nch;
     float m = -INFINITY;
-    for (int c = lane; c < a.nch; c += 64) m = fmaxf(m, a.pm[o + c]);
-    m = wave_max(m);
-    double s = 0.0;
-    if (a.inv_temp == 0.0) {
-      double at = 2147483647.0;  // the lowest index among the chunks that hold the maximum
-      for (int c = lane; c < a.nch; c += 64)
-        if (m > -INFINITY && a.pm[o + c] == m) at = fmin(at, a.ps[o + c]);
+    for (int c = sub; c < a.nch; c += 16) m = fmaxf(m, a.pm[o + c]);
 #pragma unroll
-      for (int k = 32; k > 0; k >>= 1) at = fmin(at, __shfl_xor(at, k, 64));
-      s = m > -INFINITY ? at : -1.0;
-    } else {
-      for (int c = lane; c < a.nch; c += 64)
-        if (a.pm[o + c] > -INFINITY) s += a.ps[o + c] * weight(a.pm[o + c], m, a.inv_temp);
-      s = wave_sum_d(s);
+    for (int k = 8; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor(m, k, 16));
+    double s = GREEDY ? 2147483647.0 : 0.0;
+    for (int c = sub; c < a.nch; c += 16) {
+      const float cm = a.pm[o + c];
+      const double cs = a.ps[o + c];
+      if (cm == -INFINITY) continue;
+      if constexpr (GREEDY) s = cm == m ? fmin(s, cs) : s;
+      else s += cs * weight(cm, m, a.c);
     }
-    if (lane == 0) {
+#pragma unroll
+    for (int k = 8; k > 0; k >>= 1) {
+      const double v = __shfl_xor(s, k, 16);
+      s = GREEDY ? fmin(s, v) : s + v;
+    }
+    if (sub == 0) {
       s_m[r] = m;
-      s_s[r] = s;
+      s_s[r] = GREEDY && m == -INFINITY ? -1.0 : s;
     }
   }
   __syncthreads();
-  int j = 0;
-  for (; j < nd; ++j) {
-    const int64_t x = a.tokens[(int64_t)b * a.T + j];
-    if (x < 0 || x >= a.V) break;
-    if (a.inv_temp == 0.0) {
-      if (s_s[j] != (double)x) break;
-      continue;
+  if (t < 64) {
+    bool ok = false;
+    if (t < nd) {
+      const int64_t x = a.tokens[(int64_t)b * a.T + t];
+      if (x >= 0 && x < a.V) {
+        if constexpr (GREEDY) {
+          ok = s_s[t] == (double)x;
+        } else {
+          const double zp = s_s[t], zq = s_s[a.T + 1 + t];
+          const float lp = ld1(row_ptr<E>(a, b, t) + x), lq = ld1(row_ptr<E>(a, b, a.T + 1 + t) + x);
+          const double p = zp > 0.0 ? weight(lp, s_m[t], a.c) / zp : 0.0;
+          const double q = zq > 0.0 ? weight(lq, s_m[a.T + 1 + t], a.c) / zq : 0.0;
+          ok = (double)a.u[(int64_t)b * (a.T + 1) + t] * q < p;
+        }
+      }
     }
-    const double zp = s_s[j], zq = s_s[a.T + 1 + j];
-    const double p = zp > 0.0 ? weight(clean(ld1(row_ptr<E>(a, b, j) + x)), s_m[j], a.inv_temp) / zp : 0.0;
-    const double q =
-        zq > 0.0 ? weight(clean(ld1(row_ptr<E>(a, b, a.T + 1 + j) + x)), s_m[a.T + 1 + j], a.inv_temp) / zq : 0.0;
-    if (!((double)a.u[(int64_t)b * (a.T + 1) + j] * q < p)) break;
+    const uint64_t no = ~__ballot(ok);  // lanes past the drafts refuse
+    if (t == 0) s_j[0] = __builtin_ctzll(no);
   }
-  return j;
+  __syncthreads();
+  return s_j[0];
 }
 
 // r_i at the refused (or last) position: both rows' normalisers from decide()
@@ -188,11 +236,11 @@ template <typename E>
 struct Rest {
   const E *x, *y;  // y null: r = p
   float mp, mq;
-  double ip, iq, inv_temp;  // 1 / sum, 0 where the row has no probability
-  __device__ __forceinline__ double p(int i) const { return weight(clean(ld1(x + i)), mp, inv_temp) * ip; }
-  __device__ __forceinline__ double r(int i) const {
-    const double v = p(i);
-    return y ? fmax(v - weight(clean(ld1(y + i)), mq, inv_temp) * iq, 0.0) : v;
+  double ip, iq, c;  // 1 / sum, 0 where the row has no probability
+  __device__ __forceinline__ double p(float z) const { return weight(z, mp, c) * ip; }
+  __device__ __forceinline__ double r(float z, float d) const {
+    const double v = p(z);
+    return y ? fmax(v - weight(d, mq, c) * iq, 0.0) : v;
   }
 };
 template <typename E>
@@ -201,109 +249,159 @@ __device__ Rest<E> rest_of(const Args& a, int b, int j, int nd, const float* s_m
   f.x = row_ptr<E>(a, b, j);
   f.mp = s_m[j];
   f.ip = s_s[j] > 0.0 ? 1.0 / s_s[j] : 0.0;
-  f.inv_temp = a.inv_temp;
+  f.c = a.c;
   const int k = a.T + 1 + j;
-  f.y = j < nd && s_s[k] > 0.0 ? row_ptr<E>(a, b, k) : nullptr;
-  f.mq = f.y ? s_m[k] : 0.f;
-  f.iq = f.y ? 1.0 / s_s[k] : 0.0;
+  const bool two = j < nd && s_s[k] > 0.0;
+  f.y = two ? row_ptr<E>(a, b, k) : nullptr;
+  f.mq = two ? s_m[k] : 0.f;
+  f.iq = two ? 1.0 / s_s[k] : 0.0;
   return f;
 }
 
-// ---- pass 2 (not greedy): grid (chunks, B), chunk sums of r
+// ---- pass 2 (not greedy): grid (pieces / 4, B), a wave per piece
 template <typename E>
 __global__ void __launch_bounds__(kT) verify_rest_kernel(Args a) {
+  constexpr int N = Vec<E>::N, NV = kPiece / (64 * N);
   __shared__ float s_m[kMaxRows];
-  __shared__ double s_s[kMaxRows], s_w[kT / 64];
-  const int c = blockIdx.x, b = blockIdx.y, t = threadIdx.x;
-  const int j = decide<E>(a, b, s_m, s_s);
+  __shared__ double s_s[kMaxRows];
+  __shared__ int s_j[1];
+  const int b = blockIdx.y, lane = threadIdx.x & 63;
+  const int pc = blockIdx.x * (kT / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int j = decide<E, false>(a, b, s_m, s_s, s_j);
   const Rest<E> f = rest_of<E>(a, b, j, drafts(a, b), s_m, s_s);
-  const int lo = c * a.chunk, hi = min(a.V, lo + a.chunk);
-  double s = 0.0;
-  for (int i = lo + t; i < hi; i += kT) s += f.r(i);
-  s = wave_sum_d(s);
-  if ((t & 63) == 0) s_w[t >> 6] = s;
-  __syncthreads();
-  if (t == 0) {
+  if (pc >= a.npc) return;
+  const int lo = pc * kPiece, hi = min(a.V, lo + kPiece);
+  Vec<E> v[NV], d[NV];
 #pragma unroll
-    for (int w = 1; w < kT / 64; ++w) s += s_w[w];
-    a.pr[(int64_t)b * a.nch + c] = s;
+  for (int k = 0; k < NV; ++k) v[k].load(f.x, lo + (k * 64 + lane) * N, hi);
+  if (f.y) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) d[k].load(f.y, lo + (k * 64 + lane) * N, hi);
+  } else {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) d[k].w = u32x4{0u, 0u, 0u, 0u};
   }
+  double s = 0.0;
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int e = 0; e < N; ++e) s += f.r(v[k].get(e), d[k].get(e));
+  s = wave_sum_d(s);
+  if (lane == 0) a.pr[(int64_t)b * a.npc + pc] = s;
 }
 
-// the first index of [lo, hi) whose running sum (from `before`) passes `want`, else the last one with r > 0, else -1;
-// in every thread. Thread t owns a run of consecutive indexes, so the order is that of the indexes.
-template <typename F>
-__device__ int pick(F r, int lo, int hi, double before, double want, double* s_w, int* s_i) {
+// inclusive sum over the workgroup's threads in order; every thread also gets the total
+__device__ __forceinline__ double block_scan(double v, double* s_w, double& total) {
   const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
-  const int per = (hi - lo + kT - 1) / kT, i0 = lo + t * per, i1 = min(hi, i0 + per);
-  double mine = 0.0;
-  for (int i = i0; i < i1; ++i) mine += r(i);
-  double inc = mine;  // inclusive sum over the wave's lanes
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const double v = __shfl_up(inc, o, 64);
-    if (lane >= o) inc += v;
+    const double w = __shfl_up(v, o, 64);
+    if (lane >= o) v += w;
   }
-  if (lane == 63) s_w[wv] = inc;
-  if (t == 0) {
-    s_i[0] = 0x7fffffff;
-    s_i[1] = -1;
-  }
+  __syncthreads();  // s_w may still be read
+  if (lane == 63) s_w[wv] = v;
   __syncthreads();
-  double run = before;
-  for (int w = 0; w < wv; ++w) run += s_w[w];
-  run += inc - mine;
-  int hit = 0x7fffffff, last = -1;
-  for (int i = i0; i < i1; ++i) {
-    const double v = r(i);
-    run += v;
-    if (v > 0.0) {
-      last = i;
-      if (hit == 0x7fffffff && run > want) hit = i;
-    }
+  total = 0.0;
+#pragma unroll
+  for (int w = 0; w < kT / 64; ++w) {
+    v += w < wv ? s_w[w] : 0.0;
+    total += s_w[w];
   }
-  atomicMin(&s_i[0], hit);  // minimum / maximum: no order
-  atomicMax(&s_i[1], last);
+  return v;
+}
+// the lowest `i` of any thread (0x7fffffff: none), in every thread
+__device__ __forceinline__ int block_min(int i, int* s_w) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) i = min(i, __shfl_xor(i, o, 64));
   __syncthreads();
-  return s_i[0] != 0x7fffffff ? s_i[0] : s_i[1];
+  if ((threadIdx.x & 63) == 0) s_w[threadIdx.x >> 6] = i;
+  __syncthreads();
+  return min(min(s_w[0], s_w[1]), min(s_w[2], s_w[3]));
 }
 
 // ---- pass 3: grid B
-template <typename E>
+template <typename E, bool GREEDY>
 __global__ void __launch_bounds__(kT) verify_pick_kernel(Args a) {
   __shared__ float s_m[kMaxRows];
   __shared__ double s_s[kMaxRows], s_w[kT / 64];
-  __shared__ int s_i[2];
+  __shared__ int s_j[1], s_i[kT / 64];
   const int b = blockIdx.x, t = threadIdx.x;
-  const int j = decide<E>(a, b, s_m, s_s);
+  const int j = decide<E, GREEDY>(a, b, s_m, s_s, s_j);
   int64_t next = -1;
-  if (a.inv_temp == 0.0) {
+  if constexpr (GREEDY) {
     next = (int64_t)s_s[j];
   } else {
-    const Rest<E> f = rest_of<E>(a, b, j, drafts(a, b), s_m, s_s);
-    const double* pr = a.pr + (int64_t)b * a.nch;
-    double total = 0.0;
-    for (int c = 0; c < a.nch; ++c) total += pr[c];
-    const bool none = !(total > 0.0);  // r = 0 everywhere: the target's own distribution
-    if (none) total = f.ip > 0.0 ? 1.0 : 0.0;
+    constexpr int PER = kPiece / kT;  // consecutive logits of a thread
+    Rest<E> f = rest_of<E>(a, b, j, drafts(a, b), s_m, s_s);
+    const double* pr = a.pr + (int64_t)b * a.npc;
+    // runs over groups of kT pieces, the last run one past the pieces that hold the answer
+    double total = 0.0, part;
+    for (int g = 0; g < a.npc; g += kT) {
+      block_scan(g + t < a.npc ? pr[g + t] : 0.0, s_w, part);
+      total += part;
+    }
+    const bool none = !(total > 0.0);  // r = 0 everywhere: the target's own distribution, by its chunks
+    if (none) {
+      f.y = nullptr;
+      total = f.ip > 0.0 ? 1.0 : 0.0;
+    }
     if (total > 0.0) {
-      const double want = (double)a.u[(int64_t)b * (a.T + 1) + a.T] * total;
-      // the chunk that `want` falls into; past the last sum (u >= 1, rounding): the last chunk with anything in it
       const int64_t o = ((int64_t)b * (2 * a.T + 1) + j) * a.nch;
+      const int n = none ? a.nch : a.npc, size = none ? kChunk : kPiece;
+      const double want = (double)a.u[(int64_t)b * (a.T + 1) + a.T] * total;
+      // the piece that `want` falls into; past the last sum (u >= 1, rounding): the last piece with anything in it
       double run = 0.0, before = 0.0;
-      int at = -1;
-      for (int c = 0; c < a.nch; ++c) {
-        const double v = none ? a.ps[o + c] * weight(a.pm[o + c], f.mp, a.inv_temp) * f.ip : pr[c];
-        if (v > 0.0) {
-          at = c;
-          before = run;
-          run += v;
-          if (run > want) break;
+      int at = 0x7fffffff, last = -1;
+      double last_before = 0.0;
+      for (int g = 0; g < n && at == 0x7fffffff; g += kT) {
+        const int i = g + t;
+        double v = 0.0;
+        if (i < n) v = none ? a.ps[o + i] * weight(a.pm[o + i], f.mp, f.c) * f.ip : pr[i];
+        if (none && i < n && a.pm[o + i] == -INFINITY) v = 0.0;
+        const double inc = run + block_scan(v, s_w, part);
+        at = block_min(i < n && v > 0.0 && inc > want ? i : 0x7fffffff, s_i);
+        const int nz = block_min(v > 0.0 ? -i : 0x7fffffff, s_i);  // minus the group's last piece with anything in it
+        const int pick = at != 0x7fffffff ? at : nz != 0x7fffffff ? -nz : -1;
+        if (pick >= 0) {
+          __syncthreads();
+          if (i == pick) s_w[0] = inc - v;
+          __syncthreads();
+          last = pick;
+          last_before = s_w[0];
+          __syncthreads();
         }
+        run += part;
       }
-      const int lo = at * a.chunk, hi = min(a.V, lo + a.chunk);
-      next = none ? pick([&](int i) { return f.p(i); }, lo, hi, before, want, s_w, s_i)
-                  : pick([&](int i) { return f.r(i); }, lo, hi, before, want, s_w, s_i);
+      before = last_before;
+      // inside it: PER consecutive logits a thread, so that the order is that of the indexes
+      int hit = 0x7fffffff, tail = -1;
+      const int lo = last * size, hi = min(a.V, lo + size);
+      for (int base = lo; base < hi && hit == 0x7fffffff; base += kPiece) {
+        double v[PER], mine = 0.0;
+        const int i0 = base + t * PER;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+          const bool in = i0 + e < hi;
+          v[e] = in ? f.r(ld1(f.x + i0 + e), f.y ? ld1(f.y + i0 + e) : 0.f) : 0.0;
+          mine += v[e];
+        }
+        const double inc = block_scan(mine, s_w, part);
+        double at_e = before + (inc - mine);
+        int h = 0x7fffffff, l = 0x7fffffff;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+          at_e += v[e];
+          if (v[e] > 0.0) {
+            l = -(i0 + e);
+            if (h == 0x7fffffff && at_e > want) h = i0 + e;
+          }
+        }
+        hit = block_min(h, s_i);
+        l = block_min(l, s_i);
+        if (l != 0x7fffffff) tail = -l;
+        before += part;
+      }
+      next = hit != 0x7fffffff ? hit : tail;
     }
   }
   for (int i = t; i <= a.T; i += kT)
@@ -312,38 +410,44 @@ __global__ void __launch_bounds__(kT) verify_pick_kernel(Args a) {
 }
 
 template <typename E>
-int launch(const Args& a, hipStream_t stream) {
-  verify_stats_kernel<E><<<dim3(a.nch, a.inv_temp == 0.0 ? a.T + 1 : 2 * a.T + 1, a.B), kT, 0, stream>>>(a);
-  if (a.inv_temp != 0.0) verify_rest_kernel<E><<<dim3(a.nch, a.B), kT, 0, stream>>>(a);
-  verify_pick_kernel<E><<<a.B, kT, 0, stream>>>(a);
+int launch(const Args& a, bool greedy, hipStream_t stream) {
+  const dim3 rows(a.nch, greedy ? a.T + 1 : 2 * a.T + 1, a.B);
+  if (greedy) {
+    verify_stats_kernel<E, true><<<rows, kT, 0, stream>>>(a);
+    verify_pick_kernel<E, true><<<a.B, kT, 0, stream>>>(a);
+  } else {
+    verify_stats_kernel<E, false><<<rows, kT, 0, stream>>>(a);
+    verify_rest_kernel<E><<<dim3((a.npc + kT / 64 - 1) / (kT / 64), a.B), kT, 0, stream>>>(a);
+    verify_pick_kernel<E, false><<<a.B, kT, 0, stream>>>(a);
+  }
   return hipGetLastError() == hipSuccess ? 0 : -9;
 }
+inline int64_t chunks(int V) { return (V + kChunk - 1) / kChunk; }
+inline int64_t pieces(int V) { return (V + kPiece - 1) / kPiece; }
 }  // namespace
 
-static constexpr int kChunk = 8192;
 int64_t verify_draft_workspace(int B, int T, int V) {
-  const int64_t nch = (V + kChunk - 1) / kChunk, rows = (int64_t)B * (2 * T + 1);
-  return rows * nch * (8 + 4) + (int64_t)B * nch * 8;
+  return (int64_t)B * (2 * T + 1) * chunks(V) * (8 + 4) + (int64_t)B * pieces(V) * 8;
 }
 
 int verify_draft(const void* target, int64_t ts_b, int64_t ts_t, const void* draft, int64_t ds_b, int64_t ds_t, bool f32,
                  const int64_t* tokens, const float* u, const int* n_draft, int B, int T, int V, double temp,
                  void* workspace, int64_t* out, int* accepted, hipStream_t stream) {
-  if (B < 0 || B > 65535 || T < 0 || T > kVerifyMaxDraft || V < 1 || !(temp >= 0.0)) return -1;
+  if (B < 0 || B > 65535 || T < 0 || T > kVerifyMaxDraft || V < 1 || V > 0x3fffffff || !(temp >= 0.0)) return -1;
   if (B == 0) return 0;
   Args a;
   a.target = target, a.draft = draft;
   a.ts_b = ts_b, a.ts_t = ts_t, a.ds_b = ds_b, a.ds_t = ds_t;
   a.tokens = tokens, a.u = u, a.n_draft = n_draft;
   a.B = B, a.T = T, a.V = V;
-  a.chunk = kChunk, a.nch = (V + kChunk - 1) / kChunk;
-  a.inv_temp = temp > 0.0 ? 1.0 / temp : 0.0;
+  a.nch = (int)chunks(V), a.npc = (int)pieces(V);
+  a.c = temp > 0.0 ? 1.4426950408889634 / temp : 0.0;
   const int64_t n = (int64_t)B * (2 * T + 1) * a.nch;
   a.ps = reinterpret_cast<double*>(workspace);
   a.pr = a.ps + n;
-  a.pm = reinterpret_cast<float*>(a.pr + (int64_t)B * a.nch);
+  a.pm = reinterpret_cast<float*>(a.pr + (int64_t)B * a.npc);
   a.out = out, a.accepted = accepted;
-  return f32 ? launch<float>(a, stream) : launch<bf16_t>(a, stream);
+  return f32 ? launch<float>(a, temp == 0.0, stream) : launch<bf16_t>(a, temp == 0.0, stream);
 }
 
 }  // namespace kop
