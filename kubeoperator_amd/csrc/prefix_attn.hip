@@ -21,6 +21,7 @@
 // never read (loads are clamped to it), and in the blocks where some rows see a key and others do not, values that are
 // not finite are kept from the rows that do not.
 #include <algorithm>
+#include <cmath>
 
 #include "attn_common.h"
 #include "kernels.h"
@@ -31,6 +32,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegBig = -3.402823466e38f;
+constexpr int kLds = 65536;
+constexpr int kByRows = 4;
 
 __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -80,84 +83,126 @@ struct Args {
   const int* lens;
   int64_t qs, kph, kps, vph, vps;
   int B, T, G, Hkv, P, Smax, max_len;
+  bool flip;            // scale < 0
   int pchunk, np, rtp;  // prefix: keys per range, ranges, row tiles of all sequences
   int ochunk, ns, rto;  // own keys: keys per range, ranges, row tiles of one sequence
-  float scale_log2;
+  float sl2;            // |scale| log2 e
   float *po, *pml;  // partials [Hkv][B T G][np + ns][D] and [..][2] (max, sum)
 };
 }  // namespace
 
-template <int D, int NT>  // NT: 16-row tiles per workgroup
-__global__ void __launch_bounds__(kThreads) prefix_attn_kernel(Args p) {
-  static_assert(D == 64 || D == 128, "head dim");
+namespace {
+// one workgroup's rows and keys
+struct Work {
+  int kvh, row0, nrow;   // rows [row0, row0 + nrow) of this KV head
+  int slot;              // where its partial goes
+  int k0, kend, nkeys;   // keys [k0, kend); no key at or past nkeys is read
+  int lim0;              // own keys: what token 0 of the sequence sees; prefix: nkeys
+  bool own;
+  const bf16_t *k, *v;
+  int64_t ks, vs;
+};
+__device__ __forceinline__ int seen_by(const Args& p, const Work& w, int bt) { return w.own ? w.lim0 + bt % p.T : w.nkeys; }
+
+// a row's Q^T operand: dims 32 s + 8 g .. + 7 (a negative scale is taken into Q's signs, so that maxima can be taken
+// before scaling)
+template <int D>
+__device__ __forceinline__ void load_q(const Args& p, const Work& w, int r, int g, bf16x8* qf) {
+  const int bt = r / p.G, h = w.kvh * p.G + r % p.G;
+  const bf16_t* qr = p.q + (int64_t)bt * p.qs + (int64_t)h * D + 8 * g;
+#pragma unroll
+  for (int s = 0; s < D / 32; ++s) {
+    u32x4 v = *reinterpret_cast<const u32x4*>(qr + 32 * s);
+    if (p.flip) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] ^= 0x80008000u;
+    }
+    qf[s] = __builtin_bit_cast(bf16x8, v);
+  }
+}
+
+// One 16-row tile's running softmax over NB blocks of 32 keys: sc[b] = scores of products 2 b, 2 b + 1 (the lane's keys
+// 32 (b / 2) + 8 g + 4 (b % 2) + e); leaves P^T in pf. `left`: the lane's keys of block 0 with a number below it are seen (block b:
+// left - 32 b); only looked at on an edge.
+template <int NB, int NC>
+__device__ __forceinline__ void softmax_step(const f32x4* sc, bool edge, int left, float sl2, float& m, float& l, f32x4* acc,
+                                             bf16x8* pf) {
+  float v[8 * NB];
+#pragma unroll
+  for (int j = 0; j < 8 * NB; ++j) v[j] = sc[j >> 2][j & 3];
+  if (edge) {
+#pragma unroll
+    for (int j = 0; j < 8 * NB; ++j) v[j] = 32 * (j >> 3) + (j & 7) < left ? v[j] : kNegBig;
+  }
+  float mx = v[0];
+#pragma unroll
+  for (int j = 1; j < 8 * NB; ++j) mx = fmaxf(mx, v[j]);
+  mx = xor32_max(xor16_max(mx)) * sl2;
+  if (__any(mx > m)) {
+    const float nm = fmaxf(m, mx);
+    const float al = __builtin_amdgcn_exp2f(m - nm);
+    m = nm;
+    l *= al;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[c][e] *= al;
+  }
+#pragma unroll
+  for (int j = 0; j < 8 * NB; ++j) v[j] = __builtin_amdgcn_exp2f(fmaf(v[j], sl2, -m));
+  if (edge) {
+#pragma unroll
+    for (int j = 0; j < 8 * NB; ++j) v[j] = 32 * (j >> 3) + (j & 7) < left ? v[j] : 0.f;
+  }
+  float s = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8 * NB; ++j) s += v[j];
+  l += s;  // the lane's own keys; the four groups' sums meet at the end
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const float* q = v + 8 * b;
+    pf[b] = __builtin_bit_cast(bf16x8, u32x4{pack2(q[0], q[1]), pack2(q[2], q[3]), pack2(q[4], q[5]), pack2(q[6], q[7])});
+  }
+}
+
+// acc += V^T . P^T where some rows see a key and others do not: values that are not finite reach only the rows that see them
+// (as NaN). True if there were any; `left` as in softmax_step, of this block.
+template <int NT>
+__device__ __forceinline__ bool edge_pv(bf16x8 vf, const bf16x8* pf, const int* left, f32x4* acc) {
+  bf16x8 fin, bad;
+  if (!__any(split_finite(vf, fin, bad))) return false;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    bf16x8 ones;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ones[j] = j < left[n] ? (short)0x3f80 : (short)0;
+    const f32x4 nb = mfma16(bad, ones, f32x4{0.f, 0.f, 0.f, 0.f});
+    acc[n] = mfma16(fin, pf[n], acc[n]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[n][e] = nb[e] > 0.f ? __builtin_nanf("") : acc[n][e];
+  }
+  return true;
+}
+
+// ---- few rows: all 4 waves take the same 16 NT rows, and every fourth 32-key block
+template <int D, int NT>
+__device__ __forceinline__ void by_keys(const Args& p, const Work& w, char* smem) {
   constexpr int ROWB = D * 2, NS = D / 32, NC = D / 16, KW = 32, NWV = kThreads / 64, KSTEP = KW * NWV;
   constexpr int IMG = KW * ROWB, VPW = IMG / 1024, SLOTS = ROWB / 16, RPP = 1024 / ROWB;
   // two V images per wave; afterwards the waves' O^T (two of them at a time)
-  __shared__ __attribute__((aligned(16))) char s_v[NWV * 2 * IMG > 2 * NT * 16 * D * 4 ? NWV * 2 * IMG : 2 * NT * 16 * D * 4];
+  static_assert(NWV * 2 * IMG <= kLds && 2 * NT * 16 * D * 4 <= kLds, "LDS");
   __shared__ float s_ml[NWV][NT * 16][2];
   const int t = threadIdx.x, lane = t & 63, col = lane & 15, g = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int RR = p.B * p.T * p.G, nslot = p.np + p.ns;
-  // ---- which rows and keys
-  int kvh, row0, nrow, slot, k0, kend, nkeys, lim0 = 0;  // rows [row0, row0 + nrow) of this KV head; own keys: lim0 = len - T
-  bool own_keys;
-  const bf16_t *kb_ptr, *vb_ptr;
-  int64_t ks, vs;
-  int id = blockIdx.x;
-  const int nprefix = p.Hkv * p.rtp * p.np;
-  if (id < nprefix) {
-    own_keys = false;
-    const int split = id / (p.Hkv * p.rtp);
-    id -= split * p.Hkv * p.rtp;
-    kvh = id % p.Hkv;
-    row0 = (id / p.Hkv) * NT * 16;
-    nrow = min(NT * 16, RR - row0);
-    slot = split;
-    k0 = split * p.pchunk;
-    nkeys = p.P;
-    kend = min(p.P, k0 + p.pchunk);
-    kb_ptr = p.kp + kvh * p.kph;
-    vb_ptr = p.vp + kvh * p.vph;
-    ks = p.kps;
-    vs = p.vps;
-  } else {
-    own_keys = true;
-    id -= nprefix;
-    const int split = id % p.ns;
-    id /= p.ns;
-    kvh = id % p.Hkv;
-    id /= p.Hkv;
-    const int rt = id % p.rto, b = id / p.rto;
-    const int first = rt * NT * 16;
-    nrow = min(NT * 16, p.T * p.G - first);
-    row0 = b * p.T * p.G + first;
-    slot = p.np + split;
-    k0 = split * p.ochunk;
-    nkeys = min(max(p.lens[b], 0), p.max_len);
-    lim0 = nkeys - p.T + 1;
-    const int most = lim0 + (first + nrow - 1) / p.G;  // keys that the tile's last token sees
-    kend = min(most, k0 + p.ochunk);
-    kb_ptr = p.kc + ((int64_t)b * p.Hkv + kvh) * p.Smax * D;
-    vb_ptr = p.vc + ((int64_t)b * p.Hkv + kvh) * p.Smax * D;
-    ks = vs = D;
-  }
-  if (k0 >= kend) return;  // nothing to see: pass 2 does not read this range's partials
-  // ---- Q^T operands and each lane's rows
   bf16x8 qf[NT][NS];
-  int lim[NT];  // keys that the lane's row sees
+  int lim[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const bool in = 16 * n + col < nrow;
-    const int r = row0 + (in ? 16 * n + col : 0);
-    const int bt = r / p.G, h = kvh * p.G + r % p.G;
-    const bf16_t* qr = p.q + (int64_t)bt * p.qs + (int64_t)h * D + 8 * g;
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      qf[n][s] = *reinterpret_cast<const bf16x8*>(qr + 32 * s);
-    }
-    lim[n] = own_keys ? lim0 + bt % p.T : nkeys;
+    const int r = w.row0 + (16 * n + col < w.nrow ? 16 * n + col : 0);
+    load_q<D>(p, w, r, g, qf[n]);
+    lim[n] = seen_by(p, w, r / p.G);
   }
-  char* const vimg = s_v + wv * (2 * IMG);
+  char* const vimg = smem + wv * (2 * IMG);
   const int tq = (lane >> 2) & 3, tp = lane & 3;
   const int x = vx<ROWB>(8 * g + tq) >> 1;
   uint32_t va[NC];
@@ -176,8 +221,8 @@ __global__ void __launch_bounds__(kThreads) prefix_attn_kernel(Args p) {
   auto load_k = [&](int kb, bf16x8 (*kf)[NS]) {
 #pragma unroll
     for (int bb = 0; bb < 2; ++bb) {
-      const int key = min(kb + 8 * (col >> 2) + 4 * bb + (col & 3), nkeys - 1);
-      const bf16_t* kr = kb_ptr + key * ks + 8 * g;
+      const int key = min(kb + 8 * (col >> 2) + 4 * bb + (col & 3), w.nkeys - 1);
+      const bf16_t* kr = w.k + key * w.ks + 8 * g;
 #pragma unroll
       for (int s = 0; s < NS; ++s) kf[bb][s] = *reinterpret_cast<const bf16x8*>(kr + 32 * s);
     }
@@ -185,54 +230,40 @@ __global__ void __launch_bounds__(kThreads) prefix_attn_kernel(Args p) {
   auto load_v = [&](int kb, char* img) {
 #pragma unroll
     for (int i = 0; i < VPW; ++i) {
-      const int r = RPP * i + lane / SLOTS, slot_ = lane % SLOTS;
-      const int key = min(kb + r, nkeys - 1);
-      glds16(vb_ptr + key * vs + 8 * (slot_ ^ vx<ROWB>(r)), img + 1024 * i);
+      const int r = RPP * i + lane / SLOTS, slot = lane % SLOTS;
+      const int key = min(kb + r, w.nkeys - 1);
+      glds16(w.v + key * w.vs + 8 * (slot ^ vx<ROWB>(r)), img + 1024 * i);
     }
   };
-  auto step = [&](int kb, const bf16x8 (*kf)[NS], int buf) {
-    const bool edge = own_keys && kb + KW > lim0;  // some rows see some of these keys and others do not
-    bf16x8 pf[NT], pm[NT];
+  // the wave's blocks. In flight during a block's softmax and second product: the next one's K (registers, free after the
+  // first product) and V (LDS-DMA into the other image, issued before it)
+  int kb = w.k0 + KW * wv, buf = 0;
+  bf16x8 kf[2][NS];
+  if (kb < w.kend) {
+    load_k(kb, kf);
+    load_v(kb, vimg);
+  }
+  for (; kb < w.kend; kb += KSTEP, buf ^= 1) {
+    const bool more = kb + KSTEP < w.kend;
+    const bool edge = kb + KW > w.lim0;  // some rows see some of these keys and others do not
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (more) load_v(kb + KSTEP, vimg + (buf ^ 1) * IMG);
+    f32x4 sc[NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      f32x4 sc[2];
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int bb = 0; bb < 2; ++bb) {
-        sc[bb] = f32x4{0.f, 0.f, 0.f, 0.f};
+        sc[n][bb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int s = 0; s < NS; ++s) sc[bb] = mfma16(kf[bb][s], qf[n][s], sc[bb]);
+        for (int s = 0; s < NS; ++s) sc[n][bb] = mfma16(kf[bb][s], qf[n][s], sc[n][bb]);
       }
-      float pv[8], mx = kNegBig;
-      const int left = lim[n] - kb - 8 * g;  // the lane's keys 0 .. left - 1 are seen
+    if (more) load_k(kb + KSTEP, kf);
+    bf16x8 pf[NT];
+    int left[NT];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        pv[j] = j < left ? sc[j >> 2][j & 3] * p.scale_log2 : kNegBig;
-        mx = fmaxf(mx, pv[j]);
-      }
-      mx = xor32_max(xor16_max(mx));
-      if (__any(mx > m[n])) {
-        const float nm = fmaxf(m[n], mx);
-        const float al = __builtin_amdgcn_exp2f(m[n] - nm);
-        m[n] = nm;
-        l[n] *= al;
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[n][c][e] *= al;
-      }
-      float ls = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        pv[j] = j < left ? __builtin_amdgcn_exp2f(pv[j] - m[n]) : 0.f;
-        ls += pv[j];
-      }
-      l[n] += ls;  // the lane's own keys; the four groups' sums meet at the end
-      const u32x4 pw = {pack2(pv[0], pv[1]), pack2(pv[2], pv[3]), pack2(pv[4], pv[5]), pack2(pv[6], pv[7])};
-      pf[n] = __builtin_bit_cast(bf16x8, pw);
-      if (edge) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) pm[n][j] = j < left ? (short)0x3f80 : (short)0;
-      }
+    for (int n = 0; n < NT; ++n) {
+      left[n] = lim[n] - kb - 8 * g;
+      softmax_step<1, NC>(sc[n], edge, left[n], p.sl2, m[n], l[n], acc[n], &pf[n]);
     }
 #pragma unroll
     for (int c0 = 0; c0 < NC; c0 += 4) {
@@ -244,15 +275,12 @@ __global__ void __launch_bounds__(kThreads) prefix_attn_kernel(Args p) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         if (edge) {
-          bf16x8 fin, bad;
-          if (__any(split_finite(vf[c], fin, bad))) {
+          f32x4 an[NT];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              const f32x4 nb = mfma16(bad, pm[n], f32x4{0.f, 0.f, 0.f, 0.f});
-              acc[n][c0 + c] = mfma16(fin, pf[n], acc[n][c0 + c]);
+          for (int n = 0; n < NT; ++n) an[n] = acc[n][c0 + c];
+          if (edge_pv<NT>(vf[c], pf, left, an)) {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) acc[n][c0 + c][e] = nb[e] > 0.f ? __builtin_nanf("") : acc[n][c0 + c][e];
-            }
+            for (int n = 0; n < NT; ++n) acc[n][c0 + c] = an[n];
             continue;
           }
         }
@@ -260,32 +288,8 @@ __global__ void __launch_bounds__(kThreads) prefix_attn_kernel(Args p) {
         for (int n = 0; n < NT; ++n) acc[n][c0 + c] = mfma16(vf[c], pf[n], acc[n][c0 + c]);
       }
     }
-  };
-  // ---- the wave's blocks: the next one's K and V in flight during a block's products
-  int kb = k0 + KW * wv;
-  bf16x8 ka[2][NS], kn[2][NS];
-  if (kb < kend) {
-    load_k(kb, ka);
-    load_v(kb, vimg);
   }
-  while (kb < kend) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (kb + KSTEP < kend) {
-      load_k(kb + KSTEP, kn);
-      load_v(kb + KSTEP, vimg + IMG);
-    }
-    step(kb, ka, 0);
-    kb += KSTEP;
-    if (kb >= kend) break;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (kb + KSTEP < kend) {
-      load_k(kb + KSTEP, ka);
-      load_v(kb + KSTEP, vimg);
-    }
-    step(kb, kn, 1);
-    kb += KSTEP;
-  }
-  // ---- the 4 waves' (m, l, O^T) -> one partial: waves 2, 3 into 0, 1, then 1 into 0
+  // the 4 waves' (m, l, O^T) -> one partial: waves 2, 3 into 0, 1, then 1 into 0
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     l[n] = xor32_sum(xor16_sum(l[n]));
@@ -295,7 +299,7 @@ __global__ void __launch_bounds__(kThreads) prefix_attn_kernel(Args p) {
     }
   }
   __syncthreads();  // every wave is done with its V images
-  f32x4* so = reinterpret_cast<f32x4*>(s_v);  // [2][NT][NC][64]
+  f32x4* so = reinterpret_cast<f32x4*>(smem);  // [2][NT][NC][64]
 #pragma unroll
   for (int half = 2; half >= 1; half >>= 1) {
     if (wv >= half && wv < 2 * half) {
@@ -310,8 +314,8 @@ __global__ void __launch_bounds__(kThreads) prefix_attn_kernel(Args p) {
       for (int n = 0; n < NT; ++n) {
         const float om = s_ml[wv + half][16 * n + col][0], ol = s_ml[wv + half][16 * n + col][1];
         const float nm = fmaxf(m[n], om);
-        const float wa = l[n] > 0.f ? __builtin_amdgcn_exp2f(m[n] - nm) : l[n] != l[n] ? 1.f : 0.f;
-        const float wb = ol > 0.f ? __builtin_amdgcn_exp2f(om - nm) : ol != ol ? 1.f : 0.f;
+        const float wa = l[n] == 0.f ? 0.f : __builtin_amdgcn_exp2f(m[n] - nm);
+        const float wb = ol == 0.f ? 0.f : __builtin_amdgcn_exp2f(om - nm);
         m[n] = nm;
         l[n] = l[n] * wa + ol * wb;
 #pragma unroll
@@ -333,10 +337,11 @@ __global__ void __launch_bounds__(kThreads) prefix_attn_kernel(Args p) {
     __syncthreads();
   }
   if (wv != 0) return;
+  const int RR = p.B * p.T * p.G;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    if (16 * n + col >= nrow) continue;
-    const int64_t at = ((int64_t)kvh * RR + row0 + 16 * n + col) * nslot + slot;
+    if (16 * n + col >= w.nrow) continue;
+    const int64_t at = ((int64_t)w.kvh * RR + w.row0 + 16 * n + col) * (p.np + p.ns) + w.slot;
 #pragma unroll
     for (int c = 0; c < NC; ++c) *reinterpret_cast<f32x4*>(p.po + at * D + 16 * c + 4 * g) = acc[n][c];
     if (g == 0) {
@@ -344,6 +349,180 @@ __global__ void __launch_bounds__(kThreads) prefix_attn_kernel(Args p) {
       p.pml[2 * at + 1] = l[n];
     }
   }
+}
+
+// ---- many rows: each wave takes 32 rows of its own, all 4 take every 64-key tile from LDS (K and V images, two of each:
+// the next tile travels through registers while one is computed)
+template <int D>
+__device__ __forceinline__ void by_rows(const Args& p, const Work& w, char* smem) {
+  constexpr int ROWB = D * 2, NS = D / 32, NC = D / 16, TK = 64, IMG = TK * ROWB, SLOTS = ROWB / 16, NT = 2;
+  constexpr int PER = TK * SLOTS / kThreads;  // 16-byte pieces per thread and image
+  static_assert(4 * IMG <= kLds, "LDS");
+  const int t = threadIdx.x, lane = t & 63, col = lane & 15, g = lane >> 4;
+  const int wv = __builtin_amdgcn_readfirstlane(t >> 6);
+  const bool live = 32 * wv < w.nrow;
+  bf16x8 qf[NT][NS];
+  int lim[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int i = 32 * wv + 16 * n + col, r = w.row0 + (i < w.nrow ? i : 0);
+    load_q<D>(p, w, r, g, qf[n]);
+    lim[n] = seen_by(p, w, r / p.G);
+  }
+  // K image: chunk slots XORed with the row's number in a 16-row operand (8 a + 4 b + q -> 4 a + q), so that its 16 rows'
+  // reads of one chunk fall on different banks; V image as in by_keys
+  auto kx = [](int r) { return ROWB == 256 ? (((r >> 3) & 3) << 2) | (r & 3) : (((r >> 3) & 3) << 1) | ((r >> 1) & 1); };
+  int ka[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    const int r = 8 * (col >> 2) + (col & 3);
+    ka[s] = r * ROWB + 16 * ((4 * s + g) ^ kx(r));
+  }
+  const int tq = (lane >> 2) & 3, tp = lane & 3;
+  const int x = vx<ROWB>(8 * g + tq) >> 1;
+  int va[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) va[c] = (8 * g + tq) * ROWB + 8 * (tp & 1) + 16 * ((2 * c + (tp >> 1)) ^ (2 * x));
+  float m[NT], l[NT];
+  f32x4 acc[NT][NC];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    m[n] = kNegBig;
+    l[n] = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) acc[n][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  u32x4 kr[PER], vr[PER];
+  auto fetch = [&](int kb) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int id = i * kThreads + t, r = id / SLOTS, ch = id % SLOTS;
+      const int key = min(kb + r, w.nkeys - 1);
+      kr[i] = *reinterpret_cast<const u32x4*>(w.k + key * w.ks + 8 * ch);
+      vr[i] = *reinterpret_cast<const u32x4*>(w.v + key * w.vs + 8 * ch);
+    }
+  };
+  fetch(w.k0);
+  int buf = 0;
+  for (int kb = w.k0; kb < w.kend; kb += TK, buf ^= 1) {
+    char* const kimg = smem + buf * (2 * IMG);
+    char* const vimg = kimg + IMG;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int id = i * kThreads + t, r = id / SLOTS, ch = id % SLOTS;
+      *reinterpret_cast<u32x4*>(kimg + r * ROWB + 16 * (ch ^ kx(r))) = kr[i];
+      *reinterpret_cast<u32x4*>(vimg + r * ROWB + 16 * (ch ^ vx<ROWB>(r & 31))) = vr[i];
+    }
+    // the tile is there, and every wave is done with the tile before (whose images the next one takes)
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (kb + TK < w.kend) fetch(kb + TK);
+    if (!live) continue;
+    const bool edge = kb + TK > w.lim0;
+    f32x4 sc[NT][4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) sc[n][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        const bf16x8 kf = lds_read8(kimg + ka[s] + (32 * (b >> 1) + 4 * (b & 1)) * ROWB);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) sc[n][b] = mfma16(kf, qf[n][s], sc[n][b]);
+      }
+    }
+    bf16x8 pf[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) softmax_step<2, NC>(sc[n], edge, lim[n] - kb - 8 * g, p.sl2, m[n], l[n], acc[n], pf[n]);
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const bf16x8 vf = cat44(lds_tr_read(vimg + va[c] + 32 * b * ROWB), lds_tr_read(vimg + va[c] + (32 * b + 4) * ROWB));
+        if (edge && w.own) {
+          bf16x8 pfn[NT];
+          f32x4 an[NT];
+          int left[NT];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) pfn[n] = pf[n][b], an[n] = acc[n][c], left[n] = lim[n] - kb - 8 * g - 32 * b;
+          if (edge_pv<NT>(vf, pfn, left, an)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[n][c] = an[n];
+            continue;
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[n][c] = mfma16(vf, pf[n][b], acc[n][c]);
+      }
+  }
+  if (!live) return;
+  const int RR = p.B * p.T * p.G;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    l[n] = xor32_sum(xor16_sum(l[n]));
+    const int i = 32 * wv + 16 * n + col;
+    if (i >= w.nrow) continue;
+    const int64_t at = ((int64_t)w.kvh * RR + w.row0 + i) * (p.np + p.ns) + w.slot;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) *reinterpret_cast<f32x4*>(p.po + at * D + 16 * c + 4 * g) = acc[n][c];
+    if (g == 0) {
+      p.pml[2 * at] = m[n];
+      p.pml[2 * at + 1] = l[n];
+    }
+  }
+}
+
+constexpr int tile_rows(int mode) { return mode == kByRows ? 128 : 16 * mode; }
+template <int D, int MODE>
+__device__ __forceinline__ void run_part(const Args& p, const Work& w, char* smem) {
+  if constexpr (MODE == kByRows) by_rows<D>(p, w, smem);
+  else by_keys<D, MODE>(p, w, smem);
+}
+}  // namespace
+
+// PM / OM: how the prefix's / the own keys' workgroups work (1, 2: by keys, that many 16-row tiles; kByRows)
+// Two workgroups per CU (256 registers); by rows over own keys at D = 128 takes about 30 more, and one.
+template <int D, int PM, int OM>
+__global__ void __launch_bounds__(kThreads, OM == kByRows && D == 128 ? 1 : 2) prefix_attn_kernel(Args p) {
+  __shared__ __attribute__((aligned(16))) char smem[kLds];
+  Work w;
+  int id = blockIdx.x;
+  const int nprefix = p.Hkv * p.rtp * p.np;
+  if (id < nprefix) {
+    w.own = false;
+    w.slot = id / (p.Hkv * p.rtp);
+    id -= w.slot * p.Hkv * p.rtp;
+    w.kvh = id % p.Hkv;
+    w.row0 = (id / p.Hkv) * tile_rows(PM);
+    w.nrow = min(tile_rows(PM), p.B * p.T * p.G - w.row0);
+    w.k0 = w.slot * p.pchunk;
+    w.nkeys = w.lim0 = p.P;
+    w.kend = min(p.P, w.k0 + p.pchunk);
+    w.k = p.kp + w.kvh * p.kph;
+    w.v = p.vp + w.kvh * p.vph;
+    w.ks = p.kps;
+    w.vs = p.vps;
+  } else {
+    w.own = true;
+    id -= nprefix;
+    const int split = id % p.ns;
+    id /= p.ns;
+    w.kvh = id % p.Hkv;
+    id /= p.Hkv;
+    const int b = id / p.rto, first = (id % p.rto) * tile_rows(OM);
+    w.nrow = min(tile_rows(OM), p.T * p.G - first);
+    w.row0 = b * p.T * p.G + first;
+    w.slot = p.np + split;
+    w.k0 = split * p.ochunk;
+    w.nkeys = min(max(p.lens[b], 0), p.max_len);
+    w.lim0 = w.nkeys - p.T + 1;
+    w.kend = min(w.lim0 + (first + w.nrow - 1) / p.G, w.k0 + p.ochunk);  // up to what the tile's last token sees
+    w.k = p.kc + ((int64_t)b * p.Hkv + w.kvh) * p.Smax * D;
+    w.v = p.vc + ((int64_t)b * p.Hkv + w.kvh) * p.Smax * D;
+    w.ks = w.vs = D;
+  }
+  if (w.k0 >= w.kend) return;  // nothing to see: pass 2 does not read this range's partials
+  if (PM == OM || !w.own) run_part<D, PM>(p, w, smem);
+  else run_part<D, OM>(p, w, smem);
 }
 
 // one wave per (row, KV head): the ranges that its row sees, then o = sum O 2^(m - M) / sum l 2^(m - M)
@@ -383,28 +562,29 @@ __global__ void __launch_bounds__(kThreads) prefix_attn_combine_kernel(Args p, b
 }
 
 namespace {
-// row tiles of 16 or 32; ranges of whole 128-key steps, as many as fill the chip
 struct Plan {
-  int nt, rtp, rto, np, pchunk, ns, ochunk;
+  int pm, om;               // how each part's workgroups work
+  int rtp, rto, np, pchunk, ns, ochunk;
 };
 inline int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+inline int mode_of(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : kByRows; }
 Plan make_plan(int B, int T, int G, int Hkv, int P, int max_len) {
   Plan q;
   const int64_t rows = (int64_t)B * T * G;
-  q.nt = (P > 0 ? rows : (int64_t)T * G) <= 16 ? 1 : 2;
-  q.rtp = P > 0 ? cdiv(rows, 16 * q.nt) : 0;
-  q.rto = cdiv((int64_t)T * G, 16 * q.nt);
-  auto ranges = [](int keys, int64_t groups, int& chunk) {
-    if (keys == 0) {
-      chunk = 128;
-      return 0;
-    }
-    int n = (int)std::min<int64_t>(cdiv(keys, 128), std::max<int64_t>(1, cdiv(1024, groups)));
+  q.om = mode_of((int64_t)T * G);
+  q.pm = P > 0 ? mode_of(rows) : q.om;
+  q.rtp = P > 0 ? cdiv(rows, tile_rows(q.pm)) : 0;
+  q.rto = cdiv((int64_t)T * G, tile_rows(q.om));
+  // key ranges of at least `least` keys, as many as make `want` workgroups
+  auto ranges = [](int keys, int64_t groups, int want, int least, int& chunk) {
+    chunk = least;
+    if (keys == 0) return 0;
+    const int n = (int)std::min<int64_t>(cdiv(keys, least), std::max<int64_t>(1, want / std::max<int64_t>(1, groups)));
     chunk = cdiv(cdiv(keys, n), 128) * 128;
     return cdiv(keys, chunk);
   };
-  q.np = ranges(P, (int64_t)Hkv * std::max(q.rtp, 1), q.pchunk);
-  q.ns = ranges(max_len, (int64_t)B * Hkv * q.rto, q.ochunk);
+  q.np = ranges(P, (int64_t)Hkv * q.rtp, 256, q.pm == kByRows ? 256 : 128, q.pchunk);
+  q.ns = ranges(max_len, (int64_t)B * Hkv * q.rto, 512, q.om == kByRows ? 256 : 128, q.ochunk);
   return q;
 }
 }  // namespace
@@ -429,19 +609,18 @@ int prefix_attn(const bf16_t* q, int64_t qs, const bf16_t* kp, int64_t kph, int6
   a.B = B, a.T = T, a.G = G, a.Hkv = Hkv, a.P = P, a.Smax = Smax, a.max_len = max_len;
   a.pchunk = pl.pchunk, a.np = pl.np, a.rtp = pl.rtp;
   a.ochunk = pl.ochunk, a.ns = pl.ns, a.rto = pl.rto;
-  a.scale_log2 = scale * kLog2e;
+  a.sl2 = std::abs(scale) * kLog2e;
+  a.flip = scale < 0.f;
   const int64_t parts = (int64_t)B * T * Hq * (pl.np + pl.ns);
   a.po = reinterpret_cast<float*>(workspace);
   a.pml = a.po + parts * D;
   const int64_t grid = (int64_t)Hkv * pl.rtp * pl.np + (int64_t)B * Hkv * pl.rto * pl.ns;
   if (grid > 0x7fffffff) return -1;
-#define KOP_PA(DV, NT)                                                                                        \
-  if (D == DV && pl.nt == NT && grid > 0)                                                                     \
-    prefix_attn_kernel<DV, NT><<<(unsigned)grid, kThreads, 0, stream>>>(a);
-  KOP_PA(128, 1)
-  KOP_PA(128, 2)
-  KOP_PA(64, 1)
-  KOP_PA(64, 2)
+#define KOP_PA(DV, PM, OM)                                   \
+  if (D == DV && pl.pm == PM && pl.om == OM && grid > 0)     \
+    prefix_attn_kernel<DV, PM, OM><<<(unsigned)grid, kThreads, 0, stream>>>(a);
+  KOP_PA(128, 1, 1) KOP_PA(128, 2, 1) KOP_PA(128, 2, 2) KOP_PA(128, 4, 1) KOP_PA(128, 4, 2) KOP_PA(128, 4, 4)
+  KOP_PA(64, 1, 1) KOP_PA(64, 2, 1) KOP_PA(64, 2, 2) KOP_PA(64, 4, 1) KOP_PA(64, 4, 2) KOP_PA(64, 4, 4)
 #undef KOP_PA
   const unsigned cg = (unsigned)(((int64_t)B * T * Hq + 3) / 4);
   if (D == 128)
