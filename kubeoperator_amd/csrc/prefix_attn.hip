@@ -22,6 +22,7 @@
 // not finite are kept from the rows that do not.
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 
 #include "attn_common.h"
 #include "kernels.h"
@@ -124,13 +125,13 @@ __device__ __forceinline__ void load_q(const Args& p, const Work& w, int r, int 
 // One 16-row tile's running softmax over NB blocks of 32 keys: sc[b] = scores of products 2 b, 2 b + 1 (the lane's keys
 // 32 (b / 2) + 8 g + 4 (b % 2) + e); leaves P^T in pf. `left`: the lane's keys of block 0 with a number below it are seen (block b:
 // left - 32 b); only looked at on an edge.
-template <int NB, int NC>
-__device__ __forceinline__ void softmax_step(const f32x4* sc, bool edge, int left, float sl2, float& m, float& l, f32x4* acc,
+template <bool EDGE, int NB, int NC>
+__device__ __forceinline__ void softmax_step(const f32x4* sc, int left, float sl2, float& m, float& l, f32x4* acc,
                                              bf16x8* pf) {
   float v[8 * NB];
 #pragma unroll
   for (int j = 0; j < 8 * NB; ++j) v[j] = sc[j >> 2][j & 3];
-  if (edge) {
+  if constexpr (EDGE) {
 #pragma unroll
     for (int j = 0; j < 8 * NB; ++j) v[j] = 32 * (j >> 3) + (j & 7) < left ? v[j] : kNegBig;
   }
@@ -150,7 +151,7 @@ __device__ __forceinline__ void softmax_step(const f32x4* sc, bool edge, int lef
   }
 #pragma unroll
   for (int j = 0; j < 8 * NB; ++j) v[j] = __builtin_amdgcn_exp2f(fmaf(v[j], sl2, -m));
-  if (edge) {
+  if constexpr (EDGE) {
 #pragma unroll
     for (int j = 0; j < 8 * NB; ++j) v[j] = 32 * (j >> 3) + (j & 7) < left ? v[j] : 0.f;
   }
@@ -243,9 +244,9 @@ __device__ __forceinline__ void by_keys(const Args& p, const Work& w, char* smem
     load_k(kb, kf);
     load_v(kb, vimg);
   }
-  for (; kb < w.kend; kb += KSTEP, buf ^= 1) {
+  auto block = [&](auto edge_) {
+    constexpr bool EDGE = decltype(edge_)::value;
     const bool more = kb + KSTEP < w.kend;
-    const bool edge = kb + KW > w.lim0;  // some rows see some of these keys and others do not
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     if (more) load_v(kb + KSTEP, vimg + (buf ^ 1) * IMG);
     f32x4 sc[NT][2];
@@ -263,7 +264,7 @@ __device__ __forceinline__ void by_keys(const Args& p, const Work& w, char* smem
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       left[n] = lim[n] - kb - 8 * g;
-      softmax_step<1, NC>(sc[n], edge, left[n], p.sl2, m[n], l[n], acc[n], &pf[n]);
+      softmax_step<EDGE, 1, NC>(sc[n], left[n], p.sl2, m[n], l[n], acc[n], &pf[n]);
     }
 #pragma unroll
     for (int c0 = 0; c0 < NC; c0 += 4) {
@@ -274,21 +275,26 @@ __device__ __forceinline__ void by_keys(const Args& p, const Work& w, char* smem
       read_v4<ROWB>(a, vf);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        if (edge) {
+        if constexpr (EDGE) {
           f32x4 an[NT];
 #pragma unroll
           for (int n = 0; n < NT; ++n) an[n] = acc[n][c0 + c];
-          if (edge_pv<NT>(vf[c], pf, left, an)) {
+          if (!edge_pv<NT>(vf[c], pf, left, an)) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n) acc[n][c0 + c] = an[n];
-            continue;
+            for (int n = 0; n < NT; ++n) an[n] = mfma16(vf[c], pf[n], an[n]);
           }
-        }
 #pragma unroll
-        for (int n = 0; n < NT; ++n) acc[n][c0 + c] = mfma16(vf[c], pf[n], acc[n][c0 + c]);
+          for (int n = 0; n < NT; ++n) acc[n][c0 + c] = an[n];
+          __builtin_amdgcn_sched_barrier(0);
+        } else {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) acc[n][c0 + c] = mfma16(vf[c], pf[n], acc[n][c0 + c]);
+        }
       }
     }
-  }
+  };
+  for (; kb < w.kend && kb + KW <= w.lim0; kb += KSTEP, buf ^= 1) block(std::false_type{});
+  for (; kb < w.kend; kb += KSTEP, buf ^= 1) block(std::true_type{});  // edges: some rows see some of the keys, others do not
   // the 4 waves' (m, l, O^T) -> one partial: waves 2, 3 into 0, 1, then 1 into 0
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -353,7 +359,7 @@ __device__ __forceinline__ void by_keys(const Args& p, const Work& w, char* smem
 
 // ---- many rows: each wave takes 32 rows of its own, all 4 take every 64-key tile from LDS (K and V images, two of each:
 // the next tile travels through registers while one is computed)
-template <int D>
+template <int D, bool OWN>  // OWN: the keys may be a sequence's own (rows see different numbers of them)
 __device__ __forceinline__ void by_rows(const Args& p, const Work& w, char* smem) {
   constexpr int ROWB = D * 2, NS = D / 32, NC = D / 16, TK = 64, IMG = TK * ROWB, SLOTS = ROWB / 16, NT = 2;
   constexpr int PER = TK * SLOTS / kThreads;  // 16-byte pieces per thread and image
@@ -402,58 +408,87 @@ __device__ __forceinline__ void by_rows(const Args& p, const Work& w, char* smem
       vr[i] = *reinterpret_cast<const u32x4*>(w.v + key * w.vs + 8 * ch);
     }
   };
-  fetch(w.k0);
-  int buf = 0;
-  for (int kb = w.k0; kb < w.kend; kb += TK, buf ^= 1) {
-    char* const kimg = smem + buf * (2 * IMG);
-    char* const vimg = kimg + IMG;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int id = i * kThreads + t, r = id / SLOTS, ch = id % SLOTS;
-      *reinterpret_cast<u32x4*>(kimg + r * ROWB + 16 * (ch ^ kx(r))) = kr[i];
-      *reinterpret_cast<u32x4*>(vimg + r * ROWB + 16 * (ch ^ vx<ROWB>(r & 31))) = vr[i];
-    }
-    // the tile is there, and every wave is done with the tile before (whose images the next one takes)
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (kb + TK < w.kend) fetch(kb + TK);
-    if (!live) continue;
-    const bool edge = kb + TK > w.lim0;
+  auto tile = [&](auto edge_, int kb, const char* kimg) {
+    constexpr bool EDGE = decltype(edge_)::value;
+    const char* const vimg = kimg + IMG;
     f32x4 sc[NT][4];
+    // operands one product ahead of the matrix cores (the fences keep the compiler from reading further ahead, for registers)
+    bf16x8 kf[2][NS];
+    auto read_k = [&](int b, bf16x8* f) {
+#pragma unroll
+      for (int s = 0; s < NS; ++s) f[s] = lds_read8(kimg + ka[s] + (32 * (b >> 1) + 4 * (b & 1)) * ROWB);
+    };
+    read_k(0, kf[0]);
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
+      if (b < 3) read_k(b + 1, kf[(b + 1) & 1]);
 #pragma unroll
       for (int n = 0; n < NT; ++n) sc[n][b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        const bf16x8 kf = lds_read8(kimg + ka[s] + (32 * (b >> 1) + 4 * (b & 1)) * ROWB);
+      for (int s = 0; s < NS; ++s)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) sc[n][b] = mfma16(kf, qf[n][s], sc[n][b]);
-      }
+        for (int n = 0; n < NT; ++n) sc[n][b] = mfma16(kf[b & 1][s], qf[n][s], sc[n][b]);
+      __builtin_amdgcn_sched_barrier(0);
     }
     bf16x8 pf[NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) softmax_step<2, NC>(sc[n], edge, lim[n] - kb - 8 * g, p.sl2, m[n], l[n], acc[n], pf[n]);
+    for (int n = 0; n < NT; ++n)
+      softmax_step<EDGE, 2, NC>(sc[n], lim[n] - kb - 8 * g, p.sl2, m[n], l[n], acc[n], pf[n]);
+    __builtin_amdgcn_sched_barrier(0);
+    constexpr bool SIFT = EDGE && OWN;
+    constexpr int VG = SIFT ? 1 : 4;  // 16-dim blocks read together
+    bf16x8 vf[2][VG];
+    auto read_v = [&](int i, bf16x8* f) {  // blocks VG * i .. of the 2 NC (32-key block, 16-dim block) pairs
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+      for (int k = 0; k < VG; ++k) {
+        const int b = (VG * i + k) / NC, c = (VG * i + k) % NC;
+        f[k] = cat44(lds_tr_read(vimg + va[c] + 32 * b * ROWB), lds_tr_read(vimg + va[c] + (32 * b + 4) * ROWB));
+      }
+    };
+    read_v(0, vf[0]);
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const bf16x8 vf = cat44(lds_tr_read(vimg + va[c] + 32 * b * ROWB), lds_tr_read(vimg + va[c] + (32 * b + 4) * ROWB));
-        if (edge && w.own) {
+    for (int i = 0; i < 2 * NC / VG; ++i) {
+      if (i + 1 < 2 * NC / VG) read_v(i + 1, vf[(i + 1) & 1]);
+#pragma unroll
+      for (int k = 0; k < VG; ++k) {
+        const int b = (VG * i + k) / NC, c = (VG * i + k) % NC;
+        if constexpr (SIFT) {
           bf16x8 pfn[NT];
           f32x4 an[NT];
           int left[NT];
 #pragma unroll
           for (int n = 0; n < NT; ++n) pfn[n] = pf[n][b], an[n] = acc[n][c], left[n] = lim[n] - kb - 8 * g - 32 * b;
-          if (edge_pv<NT>(vf, pfn, left, an)) {
+          if (!edge_pv<NT>(vf[i & 1][k], pfn, left, an)) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n) acc[n][c] = an[n];
-            continue;
+            for (int n = 0; n < NT; ++n) an[n] = mfma16(vf[i & 1][k], pfn[n], an[n]);
           }
-        }
 #pragma unroll
-        for (int n = 0; n < NT; ++n) acc[n][c] = mfma16(vf, pf[n][b], acc[n][c]);
+          for (int n = 0; n < NT; ++n) acc[n][c] = an[n];
+        } else {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) acc[n][c] = mfma16(vf[i & 1][k], pf[n][b], acc[n][c]);
+        }
       }
-  }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  fetch(w.k0);
+  int buf = 0, kb = w.k0;
+  auto stage = [&](auto edge_) {
+    char* const kimg = smem + buf * (2 * IMG);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int id = i * kThreads + t, r = id / SLOTS, ch = id % SLOTS;
+      *reinterpret_cast<u32x4*>(kimg + r * ROWB + 16 * (ch ^ kx(r))) = kr[i];
+      *reinterpret_cast<u32x4*>(kimg + IMG + r * ROWB + 16 * (ch ^ vx<ROWB>(r & 31))) = vr[i];
+    }
+    // the tile is there, and every wave is done with the tile before (whose images the next one takes)
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (kb + TK < w.kend) fetch(kb + TK);
+    if (live) tile(edge_, kb, kimg);
+  };
+  for (; kb < w.kend && kb + TK <= w.lim0; kb += TK, buf ^= 1) stage(std::false_type{});
+  for (; kb < w.kend; kb += TK, buf ^= 1) stage(std::true_type{});
   if (!live) return;
   const int RR = p.B * p.T * p.G;
 #pragma unroll
@@ -472,9 +507,9 @@ __device__ __forceinline__ void by_rows(const Args& p, const Work& w, char* smem
 }
 
 constexpr int tile_rows(int mode) { return mode == kByRows ? 128 : 16 * mode; }
-template <int D, int MODE>
+template <int D, int MODE, bool OWN>
 __device__ __forceinline__ void run_part(const Args& p, const Work& w, char* smem) {
-  if constexpr (MODE == kByRows) by_rows<D>(p, w, smem);
+  if constexpr (MODE == kByRows) by_rows<D, OWN>(p, w, smem);
   else by_keys<D, MODE>(p, w, smem);
 }
 }  // namespace
@@ -521,8 +556,8 @@ __global__ void __launch_bounds__(kThreads, OM == kByRows && D == 128 ? 1 : 2) p
     w.ks = w.vs = D;
   }
   if (w.k0 >= w.kend) return;  // nothing to see: pass 2 does not read this range's partials
-  if (PM == OM || !w.own) run_part<D, PM>(p, w, smem);
-  else run_part<D, OM>(p, w, smem);
+  if (PM == OM || !w.own) run_part<D, PM, PM == OM>(p, w, smem);
+  else run_part<D, OM, true>(p, w, smem);
 }
 
 // one wave per (row, KV head): the ranges that its row sees, then o = sum O 2^(m - M) / sum l 2^(m - M)
@@ -583,8 +618,9 @@ Plan make_plan(int B, int T, int G, int Hkv, int P, int max_len) {
     chunk = cdiv(cdiv(keys, n), 128) * 128;
     return cdiv(keys, chunk);
   };
-  q.np = ranges(P, (int64_t)Hkv * q.rtp, 256, q.pm == kByRows ? 256 : 128, q.pchunk);
-  q.ns = ranges(max_len, (int64_t)B * Hkv * q.rto, 512, q.om == kByRows ? 256 : 128, q.ochunk);
+  auto ev = [](const char* n, int d) { const char* e = getenv(n); return e ? atoi(e) : d; };
+  q.np = ranges(P, (int64_t)Hkv * q.rtp, ev("PA_PW", 256), q.pm == kByRows ? ev("PA_PL", 256) : 128, q.pchunk);
+  q.ns = ranges(max_len, (int64_t)B * Hkv * q.rto, ev("PA_OW", 512), q.om == kByRows ? 256 : 128, q.ochunk);
   return q;
 }
 }  // namespace
