@@ -608,6 +608,7 @@ Tensor prefix_attn(const Tensor& q, const Tensor& k_prefix, const Tensor& v_pref
                 "prefix must be [Hkv, P, D] with the cache's heads and head dim, K and V alike");
     TORCH_CHECK(t->numel() == 0 || (t->stride(2) == 1 && t->stride(0) % 8 == 0 && t->stride(1) % 8 == 0),
                 "prefix keys must be contiguous rows with strides that are multiples of 8");
+    TORCH_CHECK(t->numel() == 0 || (t->stride(1) >= 0 && t->stride(1) <= 1 << 23), "prefix key stride too large");
     check_aligned(*t, "prefix");
   }
   const int64_t P = k_prefix.size(1);

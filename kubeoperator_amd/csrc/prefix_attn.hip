@@ -22,7 +22,6 @@
 // not finite are kept from the rows that do not.
 #include <algorithm>
 #include <cmath>
-#include <cstdlib>
 
 #include "attn_common.h"
 #include "kernels.h"
@@ -122,12 +121,14 @@ __device__ __forceinline__ void load_q(const Args& p, const Work& w, int r, int 
   }
 }
 
+// maximum that passes a NaN on: no quieting of each operand first, two values per instruction
+__device__ __forceinline__ float vmax(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
 // One 16-row tile's running softmax over NB blocks of 32 keys: sc[b] = scores of products 2 b, 2 b + 1 (the lane's keys
 // 32 (b / 2) + 8 g + 4 (b % 2) + e); leaves P^T in pf. `left`: the lane's keys of block 0 with a number below it are seen (block b:
-// left - 32 b); only looked at on an edge.
+// left - 32 b); only looked at on an edge. acc holds NC blocks of O^T and, last, the row's sum (see sum_p).
 template <bool EDGE, int NB, int NC>
-__device__ __forceinline__ void softmax_step(const f32x4* sc, int left, float sl2, float& m, float& l, f32x4* acc,
-                                             bf16x8* pf) {
+__device__ __forceinline__ void softmax_step(const f32x4* sc, int left, float sl2, float& m, f32x4* acc, bf16x8* pf) {
   float v[8 * NB];
 #pragma unroll
   for (int j = 0; j < 8 * NB; ++j) v[j] = sc[j >> 2][j & 3];
@@ -135,17 +136,17 @@ __device__ __forceinline__ void softmax_step(const f32x4* sc, int left, float sl
 #pragma unroll
     for (int j = 0; j < 8 * NB; ++j) v[j] = 32 * (j >> 3) + (j & 7) < left ? v[j] : kNegBig;
   }
-  float mx = v[0];
+  float mx = vmax(vmax(v[0], v[1]), v[2]);
 #pragma unroll
-  for (int j = 1; j < 8 * NB; ++j) mx = fmaxf(mx, v[j]);
+  for (int j = 3; j + 1 < 8 * NB; j += 2) mx = vmax(vmax(mx, v[j]), v[j + 1]);
+  mx = vmax(mx, v[8 * NB - 1]);
   mx = xor32_max(xor16_max(mx)) * sl2;
   if (__any(mx > m)) {
     const float nm = fmaxf(m, mx);
     const float al = __builtin_amdgcn_exp2f(m - nm);
     m = nm;
-    l *= al;
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
+    for (int c = 0; c <= NC; ++c)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[c][e] *= al;
   }
@@ -155,15 +156,16 @@ __device__ __forceinline__ void softmax_step(const f32x4* sc, int left, float sl
 #pragma unroll
     for (int j = 0; j < 8 * NB; ++j) v[j] = 32 * (j >> 3) + (j & 7) < left ? v[j] : 0.f;
   }
-  float s = 0.f;
-#pragma unroll
-  for (int j = 0; j < 8 * NB; ++j) s += v[j];
-  l += s;  // the lane's own keys; the four groups' sums meet at the end
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     const float* q = v + 8 * b;
     pf[b] = __builtin_bit_cast(bf16x8, u32x4{pack2(q[0], q[1]), pack2(q[2], q[3]), pack2(q[4], q[5]), pack2(q[6], q[7])});
   }
+}
+// the row's sum of the rounded P on the matrix cores: every lane of the row gets it whole
+__device__ __forceinline__ f32x4 sum_p(bf16x8 pf, f32x4 acc) {
+  constexpr short one = 0x3f80;
+  return mfma16(bf16x8{one, one, one, one, one, one, one, one}, pf, acc);
 }
 
 // acc += V^T . P^T where some rows see a key and others do not: values that are not finite reach only the rows that see them
@@ -211,44 +213,65 @@ __device__ __forceinline__ void by_keys(const Args& p, const Work& w, char* smem
   for (int c = 0; c < NC; ++c)
     va[c] = lds_addr(vimg) + (8 * g + tq) * ROWB + 8 * (tp & 1) + 16 * ((2 * c + (tp >> 1)) ^ (2 * x));
   float m[NT], l[NT];
-  f32x4 acc[NT][NC];
+  f32x4 acc[NT][NC + 1];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     m[n] = kNegBig;
-    l[n] = 0.f;
 #pragma unroll
-    for (int c = 0; c < NC; ++c) acc[n][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c <= NC; ++c) acc[n][c] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  auto load_k = [&](int kb, bf16x8 (*kf)[NS]) {
+  // 32-bit lane offsets from the block's first key; `LAST`: the block may reach past the last key, whose row is read instead
+  const uint32_t ko = (uint32_t)((8 * (col >> 2) + (col & 3)) * (int)w.ks + 8 * g) * 2;
+  uint32_t vo[2];  // V pieces i: the swizzle has two forms, of i's bit 1 (D = 128) or 0 (D = 64)
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    vo[h] = (uint32_t)((lane / SLOTS) * (int)w.vs + 8 * ((lane % SLOTS) ^ vx<ROWB>(8 * h + lane / SLOTS))) * 2;
+  static_assert(ROWB == 256 || ROWB == 128, "piece -> swizzle form");
+  auto load_k = [&](auto last_, int kb, bf16x8 (*kf)[NS]) {
+    const char* base = reinterpret_cast<const char*>(w.k + kb * w.ks);
 #pragma unroll
     for (int bb = 0; bb < 2; ++bb) {
-      const int key = min(kb + 8 * (col >> 2) + 4 * bb + (col & 3), w.nkeys - 1);
-      const bf16_t* kr = w.k + key * w.ks + 8 * g;
+      uint32_t o = ko;
+      if constexpr (decltype(last_)::value)
+        o = (uint32_t)(min(8 * (col >> 2) + 4 * bb + (col & 3), w.nkeys - 1 - kb) * (int)w.ks + 8 * g) * 2;
+      else base += bb * 8 * w.ks;
 #pragma unroll
-      for (int s = 0; s < NS; ++s) kf[bb][s] = *reinterpret_cast<const bf16x8*>(kr + 32 * s);
+      for (int s = 0; s < NS; ++s) kf[bb][s] = *reinterpret_cast<const bf16x8*>(base + o + 64 * s);
     }
   };
-  auto load_v = [&](int kb, char* img) {
+  auto load_v = [&](auto last_, int kb, char* img) {
+    const char* base = reinterpret_cast<const char*>(w.v + kb * w.vs);
 #pragma unroll
     for (int i = 0; i < VPW; ++i) {
-      const int r = RPP * i + lane / SLOTS, slot = lane % SLOTS;
-      const int key = min(kb + r, w.nkeys - 1);
-      glds16(w.v + key * w.vs + 8 * (slot ^ vx<ROWB>(r)), img + 1024 * i);
+      uint32_t o = vo[(ROWB == 256 ? i >> 1 : i) & 1];
+      if constexpr (decltype(last_)::value) {
+        const int r = RPP * i + lane / SLOTS;
+        o = (uint32_t)(min(r, w.nkeys - 1 - kb) * (int)w.vs + 8 * ((lane % SLOTS) ^ vx<ROWB>(r))) * 2;
+        glds16(base + o, img + 1024 * i);
+      } else {
+        glds16(base + 2 * RPP * i * w.vs + o, img + 1024 * i);
+      }
     }
+  };
+  auto load = [&](int kb, auto&& f) {
+    if (kb + KW <= w.nkeys) f(std::false_type{});
+    else f(std::true_type{});
   };
   // the wave's blocks. In flight during a block's softmax and second product: the next one's K (registers, free after the
   // first product) and V (LDS-DMA into the other image, issued before it)
   int kb = w.k0 + KW * wv, buf = 0;
   bf16x8 kf[2][NS];
   if (kb < w.kend) {
-    load_k(kb, kf);
-    load_v(kb, vimg);
+    load(kb, [&](auto last) {
+      load_k(last, kb, kf);
+      load_v(last, kb, vimg);
+    });
   }
   auto block = [&](auto edge_) {
     constexpr bool EDGE = decltype(edge_)::value;
     const bool more = kb + KSTEP < w.kend;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (more) load_v(kb + KSTEP, vimg + (buf ^ 1) * IMG);
+    if (more) load(kb + KSTEP, [&](auto last) { load_v(last, kb + KSTEP, vimg + (buf ^ 1) * IMG); });
     f32x4 sc[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -258,13 +281,14 @@ __device__ __forceinline__ void by_keys(const Args& p, const Work& w, char* smem
 #pragma unroll
         for (int s = 0; s < NS; ++s) sc[n][bb] = mfma16(kf[bb][s], qf[n][s], sc[n][bb]);
       }
-    if (more) load_k(kb + KSTEP, kf);
+    if (more) load(kb + KSTEP, [&](auto last) { load_k(last, kb + KSTEP, kf); });
     bf16x8 pf[NT];
     int left[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       left[n] = lim[n] - kb - 8 * g;
-      softmax_step<EDGE, 1, NC>(sc[n], left[n], p.sl2, m[n], l[n], acc[n], &pf[n]);
+      softmax_step<EDGE, 1, NC>(sc[n], left[n], p.sl2, m[n], acc[n], &pf[n]);
+      acc[n][NC] = sum_p(pf[n], acc[n][NC]);
     }
 #pragma unroll
     for (int c0 = 0; c0 < NC; c0 += 4) {
@@ -298,7 +322,7 @@ __device__ __forceinline__ void by_keys(const Args& p, const Work& w, char* smem
   // the 4 waves' (m, l, O^T) -> one partial: waves 2, 3 into 0, 1, then 1 into 0
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    l[n] = xor32_sum(xor16_sum(l[n]));
+    l[n] = acc[n][NC][0];
     if (g == 0) {
       s_ml[wv][16 * n + col][0] = m[n];
       s_ml[wv][16 * n + col][1] = l[n];
@@ -389,25 +413,44 @@ __device__ __forceinline__ void by_rows(const Args& p, const Work& w, char* smem
   int va[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) va[c] = (8 * g + tq) * ROWB + 8 * (tp & 1) + 16 * ((2 * c + (tp >> 1)) ^ (2 * x));
-  float m[NT], l[NT];
-  f32x4 acc[NT][NC];
+  float m[NT];
+  f32x4 acc[NT][NC + 1];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     m[n] = kNegBig;
-    l[n] = 0.f;
 #pragma unroll
-    for (int c = 0; c < NC; ++c) acc[n][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c <= NC; ++c) acc[n][c] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
+  // a thread's pieces are rows t / SLOTS + i * RSTEP of the tile, all at chunk t % SLOTS
+  constexpr int RSTEP = kThreads / SLOTS;
+  const int tr = t / SLOTS, ch = t % SLOTS;
   u32x4 kr[PER], vr[PER];
+  const uint32_t ko = (uint32_t)(tr * (int)w.ks + 8 * ch) * 2, vo = (uint32_t)(tr * (int)w.vs + 8 * ch) * 2;
   auto fetch = [&](int kb) {
+    const char* kp = reinterpret_cast<const char*>(w.k + kb * w.ks);
+    const char* vp = reinterpret_cast<const char*>(w.v + kb * w.vs);
+    if (kb + TK <= w.nkeys) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int id = i * kThreads + t, r = id / SLOTS, ch = id % SLOTS;
-      const int key = min(kb + r, w.nkeys - 1);
-      kr[i] = *reinterpret_cast<const u32x4*>(w.k + key * w.ks + 8 * ch);
-      vr[i] = *reinterpret_cast<const u32x4*>(w.v + key * w.vs + 8 * ch);
+      for (int i = 0; i < PER; ++i) {
+        kr[i] = *reinterpret_cast<const u32x4*>(kp + 2 * RSTEP * i * w.ks + ko);
+        vr[i] = *reinterpret_cast<const u32x4*>(vp + 2 * RSTEP * i * w.vs + vo);
+      }
+    } else {  // rows past the last key: the last key's
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int r = min(tr + RSTEP * i, w.nkeys - 1 - kb);
+        kr[i] = *reinterpret_cast<const u32x4*>(kp + (uint32_t)(r * (int)w.ks + 8 * ch) * 2);
+        vr[i] = *reinterpret_cast<const u32x4*>(vp + (uint32_t)(r * (int)w.vs + 8 * ch) * 2);
+      }
     }
   };
+  int kw[PER], vw[PER];  // where they go in the images
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int r = tr + RSTEP * i;
+    kw[i] = r * ROWB + 16 * (ch ^ kx(r));
+    vw[i] = IMG + r * ROWB + 16 * (ch ^ vx<ROWB>(r & 31));
+  }
   auto tile = [&](auto edge_, int kb, const char* kimg) {
     constexpr bool EDGE = decltype(edge_)::value;
     const char* const vimg = kimg + IMG;
@@ -432,8 +475,10 @@ __device__ __forceinline__ void by_rows(const Args& p, const Work& w, char* smem
     }
     bf16x8 pf[NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-      softmax_step<EDGE, 2, NC>(sc[n], lim[n] - kb - 8 * g, p.sl2, m[n], l[n], acc[n], pf[n]);
+    for (int n = 0; n < NT; ++n) {
+      softmax_step<EDGE, 2, NC>(sc[n], lim[n] - kb - 8 * g, p.sl2, m[n], acc[n], pf[n]);
+      acc[n][NC] = sum_p(pf[n][1], sum_p(pf[n][0], acc[n][NC]));
+    }
     __builtin_amdgcn_sched_barrier(0);
     constexpr bool SIFT = EDGE && OWN;
     constexpr int VG = SIFT ? 1 : 4;  // 16-dim blocks read together
@@ -478,9 +523,8 @@ __device__ __forceinline__ void by_rows(const Args& p, const Work& w, char* smem
     char* const kimg = smem + buf * (2 * IMG);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int id = i * kThreads + t, r = id / SLOTS, ch = id % SLOTS;
-      *reinterpret_cast<u32x4*>(kimg + r * ROWB + 16 * (ch ^ kx(r))) = kr[i];
-      *reinterpret_cast<u32x4*>(kimg + IMG + r * ROWB + 16 * (ch ^ vx<ROWB>(r & 31))) = vr[i];
+      *reinterpret_cast<u32x4*>(kimg + kw[i]) = kr[i];
+      *reinterpret_cast<u32x4*>(kimg + vw[i]) = vr[i];
     }
     // the tile is there, and every wave is done with the tile before (whose images the next one takes)
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -493,7 +537,6 @@ __device__ __forceinline__ void by_rows(const Args& p, const Work& w, char* smem
   const int RR = p.B * p.T * p.G;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    l[n] = xor32_sum(xor16_sum(l[n]));
     const int i = 32 * wv + 16 * n + col;
     if (i >= w.nrow) continue;
     const int64_t at = ((int64_t)w.kvh * RR + w.row0 + i) * (p.np + p.ns) + w.slot;
@@ -501,7 +544,7 @@ __device__ __forceinline__ void by_rows(const Args& p, const Work& w, char* smem
     for (int c = 0; c < NC; ++c) *reinterpret_cast<f32x4*>(p.po + at * D + 16 * c + 4 * g) = acc[n][c];
     if (g == 0) {
       p.pml[2 * at] = m[n];
-      p.pml[2 * at + 1] = l[n];
+      p.pml[2 * at + 1] = acc[n][NC][0];
     }
   }
 }
@@ -618,9 +661,8 @@ Plan make_plan(int B, int T, int G, int Hkv, int P, int max_len) {
     chunk = cdiv(cdiv(keys, n), 128) * 128;
     return cdiv(keys, chunk);
   };
-  auto ev = [](const char* n, int d) { const char* e = getenv(n); return e ? atoi(e) : d; };
-  q.np = ranges(P, (int64_t)Hkv * q.rtp, ev("PA_PW", 256), q.pm == kByRows ? ev("PA_PL", 256) : 128, q.pchunk);
-  q.ns = ranges(max_len, (int64_t)B * Hkv * q.rto, ev("PA_OW", 512), q.om == kByRows ? 256 : 128, q.ochunk);
+  q.np = ranges(P, (int64_t)Hkv * q.rtp, 256, q.pm == kByRows ? 256 : 128, q.pchunk);
+  q.ns = ranges(max_len, (int64_t)B * Hkv * q.rto, 512, q.om == kByRows ? 256 : 128, q.ochunk);
   return q;
 }
 }  // namespace

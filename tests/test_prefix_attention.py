@@ -2,8 +2,9 @@
 prefix and own keys: head layouts, one to many tokens, lengths on and around the 32-key blocks and 128-key steps,
 empty prefixes and sequences, stale and non-finite cache rows behind each length, strides, refusals, captured calls.
 
-Tolerance per output, with A = sum_j p_j |v_j|: P is rounded to bf16 before its product with V (2^-8 A), the output once more
-(2^-8 |o|); a score is an fp32 sum of D products, scaled (D + 4 roundings of sum |q||k| scale), and the exponential's
+Tolerance per output, with A = sum_j p_j |v_j|: P is rounded to bf16 (d_j, at most 2^-8 relative) before its product with V
+and before its sum, so the quotient is off by sum_j p_j d_j (v_j - o), at most 2^-8 (A + |o|), and the output is rounded once
+more (2^-8 |o|); a score is an fp32 sum of D products, scaled (D + 4 roundings of sum |q||k| scale), and the exponential's
 argument carries two more roundings of its size, so p is off by e = ((D + 4) max_j sum |q k_j| scale + 4 max |s|) 2^-24 + 2^-22
 relative, in the numerator and in the denominator; sums over n keys in fp32 add n 2^-24 to each."""
 import math
@@ -45,7 +46,7 @@ def oracle(q, kp, vp, kc, vc, lens, max_len, T, scale):
             o, A = (p @ v).squeeze(1), (p @ v.abs()).squeeze(1)
             e = ((D + 4) * (k.abs() @ row.abs()).squeeze(-1).amax(-1) * scale + 4 * s.abs().amax(-1)) * U + 2.0 ** -22 + k.shape[1] * U
             out[b * T + t] = o
-            tol[b * T + t] = (2.0 ** -8 + 2 * e.unsqueeze(-1)) * A * (1 + 2.0 ** -7) + 2.0 ** -8 * o.abs()
+            tol[b * T + t] = (2.0 ** -8 + 2 * e.unsqueeze(-1)) * (A + o.abs()) * (1 + 2.0 ** -7) + 2.0 ** -8 * o.abs()
     return out.view(B * T, Hq * D).cpu(), tol.view(B * T, Hq * D).cpu()
 
 
