@@ -149,13 +149,14 @@ class Llama(nn.Module):
         return (x.is_cuda and torch.is_grad_enabled() and not self.tp.enabled and kf.norm_t_enabled()
                 and getattr(self.layers[0].wqkv, "w8", None) is None and kf._t_ok(x))
 
-    def forward(self, ids: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
+    def _trunk(self, ids: torch.Tensor):
+        """(final hidden rows, this rank's slice of the token rows or None: all of them)."""
         B, S = ids.shape
         cos, sin = self.rope_tables(S, ids.device)
-        ids, targets = ids.reshape(-1), targets.reshape(-1)
+        ids, rows = ids.reshape(-1), None
         if self.tp.seq_parallel:  # this rank's token rows: embedding, norms, LM head and loss on 1/tp of them
             rows = sp_rows(ids.numel(), self.tp)
-            ids, targets = ids[rows], targets[rows]
+            ids = ids[rows]
         x = kf.embedding(ids, self.tok_emb)
         pending = None
         # transposed companions of the norms (see LlamaBlock._forward_t): one box per block for its MLP output
@@ -169,5 +170,24 @@ class Llama(nn.Module):
                 x, pending = blk(x, pending, cos, sin, B, S, box_in, box)
             box_in = box
         y, _ = kf.rms_norm(x, self.final_norm, self.cfg.norm_eps, residual=pending, box=box_in)
-        head = self.tok_emb if self.cfg.tie_embeddings else self.lm_head
-        return kf.cross_entropy_lmhead(y, head, targets)
+        return y, rows
+
+    def _head(self):
+        return self.tok_emb if self.cfg.tie_embeddings else self.lm_head
+
+    def forward(self, ids: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
+        y, rows = self._trunk(ids)
+        targets = targets.reshape(-1)
+        return kf.cross_entropy_lmhead(y, self._head(), targets if rows is None else targets[rows])
+
+    def distill(self, ids: torch.Tensor, index: torch.Tensor, teacher: torch.Tensor, temperature: float = 1.0,
+                weight: torch.Tensor | None = None) -> torch.Tensor:
+        """Distillation loss of this model's next-token distributions [B, S] against a teacher's top logits: index / teacher
+        [B, S, K] (or [B * S, K]) name the tokens and hold their logits, weight [B, S] (default: the mean) the rows' shares
+        (``ops.distill_topk_lmhead``). How a draft model for ``LlamaGenerator.speculate`` is trained."""
+        if self.tp.enabled:
+            raise ValueError("distillation runs without tensor parallelism")
+        y, _ = self._trunk(ids)
+        k = index.shape[-1]
+        return kf.distill_topk_lmhead(y, self._head(), index.reshape(-1, k), teacher.reshape(-1, k), temperature,
+                                      None if weight is None else weight.reshape(-1))

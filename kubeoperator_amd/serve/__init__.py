@@ -1,4 +1,4 @@
 """Serving path of the bundled models: KV-cache generation (``generate.LlamaGenerator``)."""
-from .generate import KVCache, LlamaGenerator
+from .generate import KVCache, LlamaGenerator, LoraAdapters
 
-__all__ = ["KVCache", "LlamaGenerator"]
+__all__ = ["KVCache", "LlamaGenerator", "LoraAdapters"]

@@ -8,6 +8,13 @@ cache. MI355X-first sizing: the cache is one contiguous [B, Hkv, Smax, D] bf16 t
 V (each (sequence, KV head) a contiguous slab the decode kernel streams) (Llama-3-8B: 128 KiB per token across its 32 layers, so 288 GB of HBM minus 16 GB of weights holds ~2M
 cached tokens, e.g. 256 sequences x 8k context), allocated once, never reshaped or copied between steps.
 
+Many requests on one model. A prompt that every request starts with is prefilled once (``set_prefix``): its K / V are held
+once, every step reads them once for the whole batch, and the sequences' own caches start behind it
+(``kf.prefix_attention``). Requests can bring low-rank adapters (``set_adapters``, one index per cache slot): each
+projection adds its rows' own (``kf.lora_add``). ``extend`` pushes several tokens per sequence through one step, and
+``speculate`` uses it to check the tokens that a small draft model proposes (``kf.verify_draft``): the outputs are the
+large model's own samples, several per step of it.
+
 Weights are the model's own parameters (views into a trainer's flat store, or any loaded Llama module); the
 generator adds no autograd state (``torch.no_grad``). On CPU every op falls back to its PyTorch reference.
 """
@@ -42,8 +49,69 @@ class KVCache:
         self.host_lens[slot] = 0
         self.lens[slot] = 0
 
+    def truncate(self, lens: list) -> None:
+        """Forget what rows [0, len(lens)) hold past the given lengths (drafted tokens that were refused)."""
+        if len(lens) > self.batch or any(not 0 <= n <= h for n, h in zip(lens, self.host_lens)):
+            raise ValueError("truncate can only shorten the cached sequences")
+        self.host_lens[: len(lens)] = [int(n) for n in lens]
+        self.lens[: len(lens)] = torch.tensor(lens, dtype=torch.int32).to(self.lens.device)
+
     def bytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in self.k + self.v)
+
+
+class LoraAdapters:
+    """Low-rank adapters of many requests for the block projections, stacked so that one launch serves a mixed batch: per
+    layer and projection a [n, rank, in] and b [n, out, rank] in bf16 (``ops.lora_add``), and one scale per adapter.
+    ``rank``: a multiple of 8 (pad smaller adapters with zeros). New adapters are zero: ``set`` fills one in."""
+
+    TARGETS = ("wqkv", "wo", "w_gate_up", "w_down")
+
+    def __init__(self, cfg, n: int, rank: int, device, targets=TARGETS):
+        if n < 1 or rank < 8 or rank % 8 or rank > 128 or not targets or any(t not in self.TARGETS for t in targets):
+            raise ValueError("n >= 1 adapters, a rank that is a multiple of 8 up to 128, targets among " + ", ".join(self.TARGETS))
+        D, H, F = cfg.head_dim, cfg.hidden, cfg.ffn_hidden
+        shape = {"wqkv": ((cfg.n_heads + 2 * cfg.n_kv_heads) * D, H), "wo": (H, cfg.n_heads * D), "w_gate_up": (2 * F, H),
+                 "w_down": (H, F)}
+        self.n, self.rank, self.targets = n, rank, tuple(targets)
+        self.scale = torch.ones(n, dtype=torch.float32, device=device)
+        self.layers = [{t: (torch.zeros(n, rank, shape[t][1], dtype=torch.bfloat16, device=device),
+                            torch.zeros(n, shape[t][0], rank, dtype=torch.bfloat16, device=device)) for t in targets}
+                       for _ in range(cfg.n_layers)]
+
+    def set(self, i: int, layer: int, target: str, a: torch.Tensor, b: torch.Tensor) -> None:
+        """Adapter ``i`` of one projection: a [r, in], b [out, r] with r <= rank (the rest is zero)."""
+        A, B = self.layers[layer][target]
+        if not 0 <= i < self.n or a.shape[0] > self.rank or b.shape[1] != a.shape[0] or a.shape[1] != A.shape[2] \
+                or b.shape[0] != B.shape[1]:
+            raise ValueError("adapter index or shape")
+        A[i].zero_()
+        B[i].zero_()
+        A[i, : a.shape[0]] = a.to(A)
+        B[i, :, : a.shape[0]] = b.to(B)
+
+    def state_dict(self) -> dict:
+        out = {"scale": self.scale}
+        for li, layer in enumerate(self.layers):
+            for t, (a, b) in layer.items():
+                out[f"layers.{li}.{t}.a"], out[f"layers.{li}.{t}.b"] = a, b
+        return out
+
+    @classmethod
+    def load(cls, cfg, path: str, device) -> "LoraAdapters":
+        """From a file of ``torch.save(adapters.state_dict(), path)`` (read with ``weights_only=True``)."""
+        sd = torch.load(path, map_location=device, weights_only=True)
+        targets = [t for t in cls.TARGETS if f"layers.0.{t}.a" in sd]
+        if not targets or "scale" not in sd:
+            raise ValueError(f"{path} holds no adapters")
+        n, rank, _ = sd[f"layers.0.{targets[0]}.a"].shape
+        self = cls(cfg, n, rank, device, targets)
+        mine = self.state_dict()
+        if mine.keys() != sd.keys() or any(mine[k].shape != sd[k].shape for k in mine):
+            raise ValueError(f"{path}: adapters of another model")
+        for k in mine:
+            mine[k].copy_(sd[k])
+        return self
 
 
 class LlamaGenerator:
@@ -71,6 +139,10 @@ class LlamaGenerator:
         self.cache = KVCache(c.n_layers, max_batch, max_seq, c.n_kv_heads, c.head_dim, self.device)
         self.cos, self.sin = ref.rope_cache(max_seq, c.head_dim, c.rope_theta, device=self.device)
         self.scale = 1.0 / math.sqrt(c.head_dim)
+        self.prefix_len = 0
+        self.prefix: list = []  # per layer (K, V) [Hkv, P, D] of the prompt that every sequence starts with
+        self.adapters: LoraAdapters | None = None
+        self.slot_adapter = torch.full((max_batch,), -1, dtype=torch.int32, device=self.device)  # -1: none
         self.graph = graph and self.device.type == "cuda"
         self._graphs: dict = {}  # batch -> (graph, static token input, static logits output)
         # decode projections of <= GEMV_ROWS token rows through the HIP GEMV (csrc/gemv.hip); KOP_DECODE_GEMV=0: GEMMs
@@ -104,32 +176,96 @@ class LlamaGenerator:
             return load().gemv(x, w)
         return kf.linear(x, w)
 
-    def _mlp(self, blk, y2):
+    def _proj(self, x, i: int, name: str, rows):
+        """Projection ``name`` of layer i, with the rows' adapters added (``rows``: each row's adapter, or None)."""
+        y = self._lin(x, getattr(self.model.layers[i], name))
+        if rows is not None and name in self.adapters.targets:
+            a, b = self.adapters.layers[i][name]
+            y = kf.lora_add(y, x, a, b, rows, self.adapters.scale, out=y)
+        return y
+
+    def _adapter_rows(self, slots: torch.Tensor, tokens: int):
+        """Adapter index of every row of a batch of ``tokens`` rows per slot (None: no adapters are set)."""
+        if self.adapters is None:
+            return None
+        idx = self.slot_adapter[slots]
+        return idx.repeat_interleave(tokens) if tokens > 1 else idx
+
+    def _mlp(self, blk, y2, i: int = 0, rows=None):
+        if rows is not None:
+            return self._proj(kf.swiglu(self._proj(y2, i, "w_gate_up", rows)), i, "w_down", rows)
         if self._gemv_ok(y2, blk.w_gate_up) and self._gemv_ok(y2, blk.w_down):
             return self._lin(kf.swiglu(self._lin(y2, blk.w_gate_up)), blk.w_down)
         return kf.swiglu_mlp(y2, blk.w_gate_up, blk.w_down)
 
+    def set_adapters(self, adapters: LoraAdapters | None) -> None:
+        """Serve with these adapters (``prefill(adapters=)`` chooses each sequence's); None: without."""
+        self.adapters = adapters
+        self.slot_adapter.fill_(-1)
+        self._graphs.clear()  # captured steps hold the launches of the old set
+
+    @torch.no_grad()
+    def set_prefix(self, ids: torch.Tensor | None) -> None:
+        """The tokens [P] that every sequence starts with (a system prompt), prefilled here once and for all: prompts given
+        to ``prefill`` from now on are what follows it, and ``max_seq`` bounds that part alone. None: no prefix. Empties the
+        cache. The prefix is the base model's: adapters apply to what follows."""
+        c = self.cfg
+        P = 0 if ids is None else int(ids.numel())
+        if P and self.device.type == "cuda" and c.head_dim not in (64, 128):
+            raise ValueError("a shared prefix needs a head dim of 64 or 128")
+        self._graphs.clear()
+        self.prefix_len, self.prefix = 0, []
+        self.cache.host_lens = [0] * self.cache.batch
+        self.cache.lens.zero_()
+        if P:
+            # through a cache of its own, as long as the prefill pads to
+            tmp = LlamaGenerator(self.model, 1, -(-P // 128) * 128)
+            tmp.prefill(ids.reshape(1, P).to(self.device))
+            self.prefix = [(k[0, :, :P].contiguous(), v[0, :, :P].contiguous()) for k, v in zip(tmp.cache.k, tmp.cache.v)]
+            self.prefix_len = P
+        cos, sin = ref.rope_cache(P + self.cache.max_seq, c.head_dim, c.rope_theta, device=self.device)
+        self.cos, self.sin = cos[P:].contiguous(), sin[P:].contiguous()  # own positions start behind the prefix
+
+    def _attend(self, i: int, q, k, v, lens, max_len: int, tokens: int):
+        """Attention of ``tokens`` new rows per sequence over its cached keys, and the prefix if there is one."""
+        if not self.prefix_len and tokens == 1:
+            return kf.decode_attention(q, k, v, lens, max_len, self.scale)
+        pk, pv = self.prefix[i] if self.prefix_len else (k[0, :, :0], v[0, :, :0])
+        return kf.prefix_attention(q, pk, pv, k, v, lens, max_len, tokens, self.scale)
+
     @torch.no_grad()
     def prefill(self, ids: torch.Tensor, slot: int = 0, lengths: list | None = None,
-                slots: list | None = None) -> torch.Tensor:
+                slots: list | None = None, adapters: list | None = None) -> torch.Tensor:
         """Prompts ``ids`` [B, S] into cache rows [slot, slot + B) (or the listed ``slots``) -> logits of each
         prompt's last position [B, vocab] (fp32). ``lengths``: real lengths of right-padded rows (default S):
-        causal attention keeps every real position independent of the padding after it."""
+        causal attention keeps every real position independent of the padding after it. ``adapters``: each sequence's
+        adapter index (-1: none; default none)."""
         c, m = self.cfg, self.model
         B, S = ids.shape
         slots = list(range(slot, slot + B)) if slots is None else list(slots)
         lengths = [S] * B if lengths is None else list(lengths)
         if len(slots) != B or len(lengths) != B or max(slots) >= self.cache.batch or S > self.cache.max_seq:
             raise ValueError("prompt batch / length exceeds the cache")
+        if adapters is not None and (self.adapters is None or len(adapters) != B
+                                     or any(not -1 <= int(x) < self.adapters.n for x in adapters)):
+            raise ValueError("adapters: one index in [-1, n) per prompt, with adapters set")
         contiguous = slots == list(range(slots[0], slots[0] + B))
         rows = slice(slots[0], slots[0] + B) if contiguous else torch.tensor(slots, device=self.device)
-        if ids.is_cuda and S % 128 and S + 128 - S % 128 <= self.cache.max_seq:
+        if ids.is_cuda and S % 128 and not self.prefix_len and S + 128 - S % 128 <= self.cache.max_seq:
             # right-pad to the HIP flash forward's 128-row tiles: causal attention keeps the real positions
             # independent of the padding, whose cache rows lie past lens and are overwritten by decode steps
             ids = torch.cat([ids, ids.new_zeros(B, 128 - S % 128)], dim=1)
             S = ids.shape[1]
         Hq, Hkv, D = c.n_heads, c.n_kv_heads, c.head_dim
         a, kc = Hq * D, (Hq + Hkv) * D
+        ad = full = None
+        if self.adapters is not None:
+            slot_t = torch.tensor(slots, device=self.device)
+            self.slot_adapter[slot_t] = torch.tensor(adapters if adapters is not None else [-1] * B, dtype=torch.int32,
+                                                     device=self.device)
+            ad = self._adapter_rows(slot_t, S) if adapters is not None else None
+        if self.prefix_len:  # every row of a (padded) prompt sees the prefix and the rows before it
+            full = torch.full((B,), S, dtype=torch.int32, device=self.device)
         x = kf.embedding(ids.reshape(-1), m.tok_emb)
         pending = None
         for i, blk in enumerate(m.layers):
@@ -137,7 +273,7 @@ class LlamaGenerator:
                 y, x1 = kf.rms_norm(x, blk.attn_norm, c.norm_eps), x
             else:
                 y, x1 = kf.rms_norm(x, blk.attn_norm, c.norm_eps, residual=pending)
-            qkv = kf.linear(y, blk.wqkv)
+            qkv = kf.linear(y, blk.wqkv) if ad is None else self._proj(y, i, "wqkv", ad)
             if qkv.is_cuda:
                 from ..ops import load
 
@@ -152,12 +288,14 @@ class LlamaGenerator:
             else:  # index tensor: advanced indexing returns a COPY, so write through index_put_ (assignment)
                 self.cache.k[i][rows, :, :S] = kh
                 self.cache.v[i][rows, :, :S] = vh
-            if q.is_cuda and S % 128 == 0:  # the HIP flash forward's tile constraint
+            if self.prefix_len:
+                o = self._attend(i, q, kh.contiguous(), vh.contiguous(), full, S, S)
+            elif q.is_cuda and S % 128 == 0:  # the HIP flash forward's tile constraint
                 o, _ = kf.flash_attention(q, k, v, B, S, Hq, Hkv, D, causal=True, scale=self.scale)
             else:
                 o, _ = ref.attention_ref(q, k, v, B, S, Hq, Hkv, D, True, self.scale)
-            y2, x = kf.rms_norm(x1, blk.mlp_norm, c.norm_eps, residual=self._lin(o, blk.wo))
-            pending = self._mlp(blk, y2)
+            y2, x = kf.rms_norm(x1, blk.mlp_norm, c.norm_eps, residual=self._proj(o, i, "wo", ad))
+            pending = self._mlp(blk, y2, i, ad)
         y, _ = kf.rms_norm(x, m.final_norm, c.norm_eps, residual=pending)
         lt = torch.tensor(lengths, dtype=torch.int32)
         self.cache.lens[rows] = lt.to(self.device)
@@ -192,6 +330,19 @@ class LlamaGenerator:
             self.cache.host_lens[r] += 1
         return out
 
+    @torch.no_grad()
+    def extend(self, tok: torch.Tensor) -> torch.Tensor:
+        """Several new tokens per sequence ``tok`` [B, T] (cache rows [0, B)) at positions lens[b] .. lens[b] + T - 1 ->
+        the logits after each of them [B, T, vocab] (fp32): T decode steps in one pass over the weights and the caches.
+        ``cache.truncate`` takes tokens back."""
+        B, T = tok.shape
+        if B < 1 or T < 1 or B > self.cache.batch or max(self.cache.host_lens[:B]) + T > self.cache.max_seq:
+            raise ValueError("KV cache is full")
+        out = self._decode(tok, max(self.cache.host_lens[:B]) + T)
+        for r in range(B):
+            self.cache.host_lens[r] += T
+        return out.view(B, T, -1)
+
     def _capture(self, B: int, tok: torch.Tensor) -> None:
         static_tok = tok.clone()
         lens0 = self.cache.lens.clone()
@@ -208,15 +359,18 @@ class LlamaGenerator:
         self._graphs[B] = (g, static_tok, static_out)
 
     def _decode(self, tok: torch.Tensor, max_len: int, active: torch.Tensor | None = None) -> torch.Tensor:
-        """Device-side body of a decode step (no host reads: capturable); ``max_len`` sizes the split grid."""
+        """Device-side body of a decode step (no host reads: capturable); ``max_len`` sizes the split grid. ``tok`` [B], or
+        [B, T] for T tokens per sequence (rows b * T + t)."""
         c, m = self.cfg, self.model
         B = tok.shape[0]
+        T = tok.shape[1] if tok.dim() == 2 else 1
         Hq, Hkv, D = c.n_heads, c.n_kv_heads, c.head_dim
         a, kc = Hq * D, (Hq + Hkv) * D
         pos = self.cache.lens[:B].clone()
         rows = self._rows(B)
-        pl = pos.long()
-        lens = pos + 1
+        pls = [(pos + t) for t in range(T)] if T > 1 else [pos]
+        lens = pos + T
+        ad = self._adapter_rows(rows, T)
         x = kf.embedding(tok.reshape(-1), m.tok_emb)
         pending = None
         for i, blk in enumerate(m.layers):
@@ -224,18 +378,21 @@ class LlamaGenerator:
                 y, x1 = kf.rms_norm(x, blk.attn_norm, c.norm_eps), x
             else:
                 y, x1 = kf.rms_norm(x, blk.attn_norm, c.norm_eps, residual=pending)
-            qkv = self._lin(y, blk.wqkv)
-            if qkv.is_cuda:  # one kernel: RoPE at pos on Q / K + K / V rows appended to the cache
-                from ..ops import load
+            qkv = self._proj(y, i, "wqkv", ad)
+            by_tok = qkv.view(B, T, -1)
+            for t, pt in enumerate(pls):
+                row = by_tok[:, t]
+                if qkv.is_cuda:  # one kernel: RoPE at pos on Q / K + K / V rows appended to the cache
+                    from ..ops import load
 
-                load().decode_rope_append_(qkv, self.cos, self.sin, pos, self.cache.k[i], self.cache.v[i], Hq)
-            else:
-                kf.rope_positions_(qkv, self.cos, self.sin, pos, Hq + Hkv, D)
-                self.cache.k[i][rows, :, pl] = qkv[:, a:kc].reshape(B, Hkv, D)
-                self.cache.v[i][rows, :, pl] = qkv[:, kc:].reshape(B, Hkv, D)
-            o = kf.decode_attention(qkv[:, :a], self.cache.k[i][:B], self.cache.v[i][:B], lens, max_len, self.scale)
-            y2, x = kf.rms_norm(x1, blk.mlp_norm, c.norm_eps, residual=self._lin(o, blk.wo))
-            pending = self._mlp(blk, y2)
+                    load().decode_rope_append_(row, self.cos, self.sin, pt, self.cache.k[i], self.cache.v[i], Hq)
+                else:
+                    row.copy_(ref.rope_ref(row, self.cos, self.sin, 1, Hq + Hkv, D, pos=pt))
+                    self.cache.k[i][rows, :, pt.long()] = row[:, a:kc].reshape(B, Hkv, D)
+                    self.cache.v[i][rows, :, pt.long()] = row[:, kc:].reshape(B, Hkv, D)
+            o = self._attend(i, qkv[:, :a], self.cache.k[i][:B], self.cache.v[i][:B], lens, max_len, T)
+            y2, x = kf.rms_norm(x1, blk.mlp_norm, c.norm_eps, residual=self._proj(o, i, "wo", ad))
+            pending = self._mlp(blk, y2, i, ad)
         y, _ = kf.rms_norm(x, m.final_norm, c.norm_eps, residual=pending)
         self.cache.lens[:B] = lens if active is None else pos + active
         return self._lin(y, self._head()).float() if self._gemv_ok(y, self._head()) else \
@@ -259,3 +416,54 @@ class LlamaGenerator:
                 break
             logits = self.decode(nxt)
         return torch.cat(out, dim=1)
+
+    @torch.no_grad()
+    def speculate(self, draft: "LlamaGenerator", ids: torch.Tensor, max_new_tokens: int, drafts: int = 4,
+                  temperature: float = 0.0, generator: torch.Generator | None = None):
+        """Continuation of ``ids`` [B, S] through a small draft model: it proposes ``drafts`` tokens per round, one ``extend`` of
+        this model scores them all, and ``ops.verify_draft`` keeps the first ones and draws the token after them. With
+        ``temperature`` 0 the result is this model's greedy continuation, otherwise it is distributed as this model's
+        samples (uniform numbers from ``generator``). Returns ([B, S + max_new_tokens] tokens, kept drafts per round)."""
+        B, S = ids.shape
+        if draft.cfg.vocab_size != self.cfg.vocab_size or not 1 <= drafts <= 32 or max_new_tokens < 1:
+            raise ValueError("the draft needs this model's vocabulary; 1 to 32 drafts per round")
+        if draft.prefix_len != self.prefix_len:
+            raise ValueError("give the draft the same prefix")
+        for g in (self, draft):  # the last round may start one token before the end and brings drafts + 1
+            if B > g.cache.batch or S + max_new_tokens + drafts > g.cache.max_seq:
+                raise ValueError("KV cache too small for the continuation and one round of drafts")
+
+        def uniform(*shape):
+            return torch.rand(*shape, device=self.device, generator=generator)
+
+        def sample(logits):  # one token per row, as verify_draft draws it: no drafted tokens to check
+            none = torch.empty(B, 0, dtype=torch.long, device=self.device)
+            return kf.verify_draft(logits.unsqueeze(1), None, none, uniform(B, 1), temperature)[0][:, 0]
+
+        cur = sample(self.prefill(ids))
+        draft.prefill(ids)
+        out = [[int(t)] for t in cur.tolist()]
+        rounds = []
+        while min(len(o) for o in out) < max_new_tokens:
+            start = list(self.cache.host_lens[:B])
+            tok, toks, qs = cur, [], []
+            for _ in range(drafts):
+                q = draft.decode(tok)
+                tok = sample(q)
+                toks.append(tok)
+                qs.append(q)
+            draft.decode(tok)  # the last one's keys: all of them may be kept
+            proposed = torch.stack(toks, 1)
+            p = self.extend(torch.cat([cur.unsqueeze(1), proposed], 1))
+            new, kept = kf.verify_draft(p, torch.stack(qs, 1), proposed, uniform(B, drafts + 1), temperature)
+            cur = new.gather(1, kept.long().unsqueeze(1)).squeeze(1)
+            new, kept = new.tolist(), kept.tolist()
+            rounds.append(kept)
+            for b in range(B):
+                out[b] += new[b][: kept[b] + 1]
+            # a finished sequence stays where this round began: it goes on computing rows that are thrown away
+            lens = [n if len(o) >= max_new_tokens else n + k + 1 for n, k, o in zip(start, kept, out)]
+            for g in (self, draft):
+                g.cache.truncate(lens)
+        res = torch.tensor([o[:max_new_tokens] for o in out], dtype=ids.dtype, device=ids.device)
+        return torch.cat([ids, res], dim=1), rounds

@@ -7,13 +7,16 @@ greedy continuation of every prompt. Continuous batching (``ContinuousBatcher``)
 concurrent request takes a free sequence slot of the KV cache as soon as one is free (its own prefill), and one
 decode step advances all active slots together -- prompts of any length, joining and leaving between steps, so
 the decode GEMMs and the decode-attention kernel see the whole live batch (ragged cache lengths). ``GET /v1/model`` describes the loaded model,
-``GET /healthz`` answers readiness probes. Token ids in, token ids out: the chart ships no tokenizer files.
+``GET /healthz`` answers readiness probes. ``--prefix FILE`` (a JSON list of token ids) is a system prompt that every
+prompt follows: prefilled once, held and read once for the whole batch. ``--adapters FILE`` (``LoraAdapters.state_dict``)
+serves low-rank adapters beside the base model: a request names its own with ``"adapter": index``. Token ids in, token ids out: the chart ships no tokenizer files.
 Weights are random-init unless ``--ckpt`` names a training checkpoint directory (the trainer's flat layout;
 loaded with ``torch.load(weights_only=True)``).
 """
 from __future__ import annotations
 
 import argparse
+import json
 import queue
 import threading
 import time
@@ -22,17 +25,18 @@ import torch
 from pydantic import BaseModel
 
 from ..models import build_model, get_config
-from .generate import LlamaGenerator
+from .generate import LlamaGenerator, LoraAdapters
 
 
 class GenerateRequest(BaseModel):
     tokens: list[list[int]]
     max_new_tokens: int = 16
+    adapter: int = -1
 
 
 class _Seq:
-    def __init__(self, prompt: list[int], max_new: int):
-        self.prompt, self.max_new = prompt, max_new
+    def __init__(self, prompt: list[int], max_new: int, adapter: int = -1):
+        self.prompt, self.max_new, self.adapter = prompt, max_new, adapter
         self.out: list[int] = []
         self.done = threading.Event()
         self.error: Exception | None = None
@@ -52,8 +56,8 @@ class ContinuousBatcher:
         self._thread = threading.Thread(target=self._loop, name="kop-serve-batcher", daemon=True)
         self._thread.start()
 
-    def generate(self, prompts: list[list[int]], max_new: int) -> list[list[int]]:
-        seqs = [_Seq(p, max_new) for p in prompts]
+    def generate(self, prompts: list[list[int]], max_new: int, adapter: int = -1) -> list[list[int]]:
+        seqs = [_Seq(p, max_new, adapter) for p in prompts]
         for sq in seqs:
             self.q.put(sq)
         for sq in seqs:
@@ -89,7 +93,8 @@ class ContinuousBatcher:
                 for r, (_, sq) in enumerate(members):
                     ids[r, :len(sq.prompt)] = torch.tensor(sq.prompt, dtype=torch.long)
                 logits = self.gen.prefill(ids.to(self.gen.device), slots=[sl for sl, _ in members],
-                                          lengths=[len(sq.prompt) for _, sq in members])
+                                          lengths=[len(sq.prompt) for _, sq in members],
+                                          adapters=[sq.adapter for _, sq in members] if self.gen.adapters else None)
                 nxt = logits.argmax(-1).tolist()
             except Exception as e:  # a bad request fails alone
                 for slot, sq in members:
@@ -142,10 +147,17 @@ class ContinuousBatcher:
                     self._finish(i)
 
 
-def create_app(model, max_batch: int, max_seq: int, graph: bool = False, fp8: bool = False):
+def create_app(model, max_batch: int, max_seq: int, graph: bool = False, fp8: bool = False,
+               prefix: list[int] | None = None, adapters: LoraAdapters | None = None):
     from fastapi import FastAPI, HTTPException
 
     gen = LlamaGenerator(model, max_batch=max_batch, max_seq=max_seq, graph=graph, fp8=fp8)
+    if prefix:
+        if any(not 0 <= t < model.cfg.vocab_size for t in prefix):
+            raise ValueError(f"prefix: token ids must be in [0, {model.cfg.vocab_size})")
+        gen.set_prefix(torch.tensor(prefix, dtype=torch.long))
+    if adapters is not None:
+        gen.set_adapters(adapters)
     batcher = ContinuousBatcher(gen)
     app = FastAPI(title="KubeOperator-AMD serving", docs_url="/docs")
     app.state.batcher = batcher
@@ -159,7 +171,8 @@ def create_app(model, max_batch: int, max_seq: int, graph: bool = False, fp8: bo
         c = model.cfg
         return {"model": c.name, "params": c.num_params(), "max_batch": max_batch, "max_seq": max_seq,
                 "active": sum(x is not None for x in batcher.slots), "decode_steps": batcher.steps,
-                "kv_cache_gb": round(gen.cache.bytes() / 1e9, 3), "hip_graph": gen.graph, "fp8_weights": fp8}
+                "kv_cache_gb": round(gen.cache.bytes() / 1e9, 3), "hip_graph": gen.graph, "fp8_weights": fp8,
+                "prefix_tokens": gen.prefix_len, "adapters": gen.adapters.n if gen.adapters else 0}
 
     @app.post("/v1/generate")
     def generate(req: GenerateRequest):
@@ -171,8 +184,11 @@ def create_app(model, max_batch: int, max_seq: int, graph: bool = False, fp8: bo
         vocab = model.cfg.vocab_size
         if any(t < 0 or t >= vocab for row in req.tokens for t in row):
             raise HTTPException(400, f"token ids must be in [0, {vocab})")
+        n = gen.adapters.n if gen.adapters else 0
+        if not -1 <= req.adapter < n:
+            raise HTTPException(400, f"adapter must be -1 (none) or one of the {n} loaded ones")
         t0 = time.perf_counter()
-        new = batcher.generate(req.tokens, req.max_new_tokens)
+        new = batcher.generate(req.tokens, req.max_new_tokens, req.adapter)
         return {"tokens": new, "ms": round((time.perf_counter() - t0) * 1e3, 3)}
 
     return app
@@ -226,6 +242,8 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--graph", type=int, default=0, choices=[0, 1])
     ap.add_argument("--fp8", type=int, default=0, choices=[0, 1])
     ap.add_argument("--ckpt", default="")
+    ap.add_argument("--prefix", default="", help="JSON file: token ids that every prompt follows")
+    ap.add_argument("--adapters", default="", help="low-rank adapters (torch.save of LoraAdapters.state_dict())")
     ap.add_argument("--host", default="0.0.0.0")
     ap.add_argument("--port", type=int, default=8000)
     return ap
@@ -236,7 +254,12 @@ def main(argv=None) -> int:
     import uvicorn
 
     dev = "cuda" if torch.cuda.is_available() else "cpu"
-    app = create_app(load_model(a.model, dev, a.ckpt), a.max_batch, a.max_seq, bool(a.graph), bool(a.fp8))
+    prefix = None
+    if a.prefix:
+        with open(a.prefix) as f:
+            prefix = [int(t) for t in json.load(f)]
+    adapters = LoraAdapters.load(get_config(a.model), a.adapters, dev) if a.adapters else None
+    app = create_app(load_model(a.model, dev, a.ckpt), a.max_batch, a.max_seq, bool(a.graph), bool(a.fp8), prefix, adapters)
     uvicorn.run(app, host=a.host, port=a.port, log_level="warning")
     return 0
 
