@@ -34,6 +34,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegBig = -3.402823466e38f;
 constexpr int kLds = 65536;
 constexpr int kByRows = 4;
+constexpr int kMfma = 0x8, kDsRead = 0x100;  // instruction classes of sched_group_barrier
 
 __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -455,24 +456,26 @@ __device__ __forceinline__ void by_rows(const Args& p, const Work& w, char* smem
     constexpr bool EDGE = decltype(edge_)::value;
     const char* const vimg = kimg + IMG;
     f32x4 sc[NT][4];
-    // operands one product ahead of the matrix cores (the fences keep the compiler from reading further ahead, for registers)
-    bf16x8 kf[2][NS];
-    auto read_k = [&](int b, bf16x8* f) {
-#pragma unroll
-      for (int s = 0; s < NS; ++s) f[s] = lds_read8(kimg + ka[s] + (32 * (b >> 1) + 4 * (b & 1)) * ROWB);
-    };
-    read_k(0, kf[0]);
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      if (b < 3) read_k(b + 1, kf[(b + 1) & 1]);
 #pragma unroll
       for (int n = 0; n < NT; ++n) sc[n][b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int s = 0; s < NS; ++s)
+      for (int s = 0; s < NS; ++s) {
+        const bf16x8 kf = lds_read8(kimg + ka[s] + (32 * (b >> 1) + 4 * (b & 1)) * ROWB);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) sc[n][b] = mfma16(kf[b & 1][s], qf[n][s], sc[n][b]);
-      __builtin_amdgcn_sched_barrier(0);
+        for (int n = 0; n < NT; ++n) sc[n][b] = mfma16(kf, qf[n][s], sc[n][b]);
+      }
     }
+    // issue order: the operands of one 16-key product ahead of the matrix cores
+    __builtin_amdgcn_sched_group_barrier(kDsRead, NS, 0);
+#pragma unroll
+    for (int b = 0; b < 3; ++b) {
+      __builtin_amdgcn_sched_group_barrier(kDsRead, NS, 0);
+      __builtin_amdgcn_sched_group_barrier(kMfma, NS * NT, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(kMfma, NS * NT, 0);
+    __builtin_amdgcn_sched_barrier(0);
     bf16x8 pf[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -481,41 +484,40 @@ __device__ __forceinline__ void by_rows(const Args& p, const Work& w, char* smem
     }
     __builtin_amdgcn_sched_barrier(0);
     constexpr bool SIFT = EDGE && OWN;
-    constexpr int VG = SIFT ? 1 : 4;  // 16-dim blocks read together
-    bf16x8 vf[2][VG];
-    auto read_v = [&](int i, bf16x8* f) {  // blocks VG * i .. of the 2 NC (32-key block, 16-dim block) pairs
 #pragma unroll
-      for (int k = 0; k < VG; ++k) {
-        const int b = (VG * i + k) / NC, c = (VG * i + k) % NC;
-        f[k] = cat44(lds_tr_read(vimg + va[c] + 32 * b * ROWB), lds_tr_read(vimg + va[c] + (32 * b + 4) * ROWB));
-      }
-    };
-    read_v(0, vf[0]);
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
-    for (int i = 0; i < 2 * NC / VG; ++i) {
-      if (i + 1 < 2 * NC / VG) read_v(i + 1, vf[(i + 1) & 1]);
-#pragma unroll
-      for (int k = 0; k < VG; ++k) {
-        const int b = (VG * i + k) / NC, c = (VG * i + k) % NC;
+      for (int c = 0; c < NC; ++c) {
+        const bf16x8 vf = cat44(lds_tr_read(vimg + va[c] + 32 * b * ROWB), lds_tr_read(vimg + va[c] + (32 * b + 4) * ROWB));
         if constexpr (SIFT) {
           bf16x8 pfn[NT];
           f32x4 an[NT];
           int left[NT];
 #pragma unroll
           for (int n = 0; n < NT; ++n) pfn[n] = pf[n][b], an[n] = acc[n][c], left[n] = lim[n] - kb - 8 * g - 32 * b;
-          if (!edge_pv<NT>(vf[i & 1][k], pfn, left, an)) {
+          if (!edge_pv<NT>(vf, pfn, left, an)) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n) an[n] = mfma16(vf[i & 1][k], pfn[n], an[n]);
+            for (int n = 0; n < NT; ++n) an[n] = mfma16(vf, pfn[n], an[n]);
           }
 #pragma unroll
           for (int n = 0; n < NT; ++n) acc[n][c] = an[n];
+          __builtin_amdgcn_sched_barrier(0);
         } else {
 #pragma unroll
-          for (int n = 0; n < NT; ++n) acc[n][c] = mfma16(vf[i & 1][k], pf[n][b], acc[n][c]);
+          for (int n = 0; n < NT; ++n) acc[n][c] = mfma16(vf, pf[n][b], acc[n][c]);
         }
       }
-      __builtin_amdgcn_sched_barrier(0);
+    if constexpr (!SIFT) {  // issue order: four 16-dim blocks' operands ahead
+      constexpr int VG = 4;
+      __builtin_amdgcn_sched_group_barrier(kDsRead, 2 * VG, 0);
+#pragma unroll
+      for (int i = 0; i + 1 < 2 * NC / VG; ++i) {
+        __builtin_amdgcn_sched_group_barrier(kDsRead, 2 * VG, 0);
+        __builtin_amdgcn_sched_group_barrier(kMfma, VG * NT, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(kMfma, VG * NT, 0);
     }
+    __builtin_amdgcn_sched_barrier(0);
   };
   fetch(w.k0);
   int buf = 0, kb = w.k0;
