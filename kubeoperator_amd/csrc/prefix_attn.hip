@@ -34,7 +34,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegBig = -3.402823466e38f;
 constexpr int kLds = 65536;
 constexpr int kByRows = 4;
-constexpr int kMfma = 0x8, kDsRead = 0x100;  // instruction classes of sched_group_barrier
+constexpr int kTrans = 0x400, kMfma = 0x8, kDsRead = 0x100;  // instruction classes of sched_group_barrier
 
 __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -126,21 +126,19 @@ __device__ __forceinline__ void load_q(const Args& p, const Work& w, int r, int 
 __device__ __forceinline__ float vmax(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 // One 16-row tile's running softmax over NB blocks of 32 keys: sc[b] = scores of products 2 b, 2 b + 1 (the lane's keys
-// 32 (b / 2) + 8 g + 4 (b % 2) + e); leaves P^T in pf. `left`: the lane's keys of block 0 with a number below it are seen (block b:
-// left - 32 b); only looked at on an edge. acc holds NC blocks of O^T and, last, the row's sum (see sum_p).
+// 32 (b / 2) + 8 g + 4 (b % 2) + e). `left`: the lane's keys of block 0 with a number below it are seen (block b:
+// left - 32 b); only looked at on an edge. First the maximum: masked scores leave sc, and where a row's maximum rises, acc (NC
+// blocks of O^T and, last, the row's sum: see sum_p) is scaled down.
 template <bool EDGE, int NB, int NC>
-__device__ __forceinline__ void softmax_step(const f32x4* sc, int left, float sl2, float& m, f32x4* acc, bf16x8* pf) {
-  float v[8 * NB];
-#pragma unroll
-  for (int j = 0; j < 8 * NB; ++j) v[j] = sc[j >> 2][j & 3];
+__device__ __forceinline__ void raise_max(f32x4* sc, int left, float sl2, float& m, f32x4* acc) {
   if constexpr (EDGE) {
 #pragma unroll
-    for (int j = 0; j < 8 * NB; ++j) v[j] = 32 * (j >> 3) + (j & 7) < left ? v[j] : kNegBig;
+    for (int j = 0; j < 8 * NB; ++j) sc[j >> 2][j & 3] = 32 * (j >> 3) + (j & 7) < left ? sc[j >> 2][j & 3] : kNegBig;
   }
-  float mx = vmax(vmax(v[0], v[1]), v[2]);
+  float mx = sc[0][0];
 #pragma unroll
-  for (int j = 3; j + 1 < 8 * NB; j += 2) mx = vmax(vmax(mx, v[j]), v[j + 1]);
-  mx = vmax(mx, v[8 * NB - 1]);
+  for (int j = 1; j + 1 < 8 * NB; j += 2) mx = vmax(vmax(mx, sc[j >> 2][j & 3]), sc[(j + 1) >> 2][(j + 1) & 3]);
+  mx = vmax(mx, sc[2 * NB - 1][3]);
   mx = xor32_max(xor16_max(mx)) * sl2;
   if (__any(mx > m)) {
     const float nm = fmaxf(m, mx);
@@ -151,8 +149,13 @@ __device__ __forceinline__ void softmax_step(const f32x4* sc, int left, float sl
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[c][e] *= al;
   }
+}
+// Then the weights, P^T, rounded to bf16.
+template <bool EDGE, int NB>
+__device__ __forceinline__ void weights(const f32x4* sc, int left, float sl2, float m, bf16x8* pf) {
+  float v[8 * NB];
 #pragma unroll
-  for (int j = 0; j < 8 * NB; ++j) v[j] = __builtin_amdgcn_exp2f(fmaf(v[j], sl2, -m));
+  for (int j = 0; j < 8 * NB; ++j) v[j] = __builtin_amdgcn_exp2f(fmaf(sc[j >> 2][j & 3], sl2, -m));
   if constexpr (EDGE) {
 #pragma unroll
     for (int j = 0; j < 8 * NB; ++j) v[j] = 32 * (j >> 3) + (j & 7) < left ? v[j] : 0.f;
@@ -288,7 +291,8 @@ __device__ __forceinline__ void by_keys(const Args& p, const Work& w, char* smem
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       left[n] = lim[n] - kb - 8 * g;
-      softmax_step<EDGE, 1, NC>(sc[n], left[n], p.sl2, m[n], acc[n], &pf[n]);
+      raise_max<EDGE, 1, NC>(sc[n], left[n], p.sl2, m[n], acc[n]);
+      weights<EDGE, 1>(sc[n], left[n], p.sl2, m[n], &pf[n]);
       acc[n][NC] = sum_p(pf[n], acc[n][NC]);
     }
 #pragma unroll
@@ -403,17 +407,10 @@ __device__ __forceinline__ void by_rows(const Args& p, const Work& w, char* smem
   // K image: chunk slots XORed with the row's number in a 16-row operand (8 a + 4 b + q -> 4 a + q), so that its 16 rows'
   // reads of one chunk fall on different banks; V image as in by_keys
   auto kx = [](int r) { return ROWB == 256 ? (((r >> 3) & 3) << 2) | (r & 3) : (((r >> 3) & 3) << 1) | ((r >> 1) & 1); };
-  int ka[NS];
-#pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    const int r = 8 * (col >> 2) + (col & 3);
-    ka[s] = r * ROWB + 16 * ((4 * s + g) ^ kx(r));
-  }
-  const int tq = (lane >> 2) & 3, tp = lane & 3;
-  const int x = vx<ROWB>(8 * g + tq) >> 1;
-  int va[NC];
-#pragma unroll
-  for (int c = 0; c < NC; ++c) va[c] = (8 * g + tq) * ROWB + 8 * (tp & 1) + 16 * ((2 * c + (tp >> 1)) ^ (2 * x));
+  // chunk 4 s + g of a K row is at ka ^ 64 s, 16-dim block c of V^T at va ^ 32 c
+  const int krow = 8 * (col >> 2) + (col & 3), vrow = 8 * g + ((lane >> 2) & 3), tp = lane & 3;
+  const int ka = krow * ROWB + 16 * (g ^ kx(krow));
+  const int va = vrow * ROWB + 8 * (tp & 1) + 16 * ((tp >> 1) ^ vx<ROWB>(vrow));
   float m[NT];
   f32x4 acc[NT][NC + 1];
 #pragma unroll
@@ -425,70 +422,101 @@ __device__ __forceinline__ void by_rows(const Args& p, const Work& w, char* smem
   // a thread's pieces are rows t / SLOTS + i * RSTEP of the tile, all at chunk t % SLOTS
   constexpr int RSTEP = kThreads / SLOTS;
   const int tr = t / SLOTS, ch = t % SLOTS;
-  u32x4 kr[PER], vr[PER];
   const uint32_t ko = (uint32_t)(tr * (int)w.ks + 8 * ch) * 2, vo = (uint32_t)(tr * (int)w.vs + 8 * ch) * 2;
-  auto fetch = [&](int kb) {
-    const char* kp = reinterpret_cast<const char*>(w.k + kb * w.ks);
-    const char* vp = reinterpret_cast<const char*>(w.v + kb * w.vs);
+  auto fetch = [&](const bf16_t* src, int64_t stride, uint32_t off, int kb, u32x4* to) {
+    const char* base = reinterpret_cast<const char*>(src + kb * stride);
     if (kb + TK <= w.nkeys) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        kr[i] = *reinterpret_cast<const u32x4*>(kp + 2 * RSTEP * i * w.ks + ko);
-        vr[i] = *reinterpret_cast<const u32x4*>(vp + 2 * RSTEP * i * w.vs + vo);
-      }
+      for (int i = 0; i < PER; ++i) to[i] = *reinterpret_cast<const u32x4*>(base + 2 * RSTEP * i * stride + off);
     } else {  // rows past the last key: the last key's
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int r = min(tr + RSTEP * i, w.nkeys - 1 - kb);
-        kr[i] = *reinterpret_cast<const u32x4*>(kp + (uint32_t)(r * (int)w.ks + 8 * ch) * 2);
-        vr[i] = *reinterpret_cast<const u32x4*>(vp + (uint32_t)(r * (int)w.vs + 8 * ch) * 2);
-      }
+      for (int i = 0; i < PER; ++i)
+        to[i] = *reinterpret_cast<const u32x4*>(
+            base + (uint32_t)(min(tr + RSTEP * i, w.nkeys - 1 - kb) * (int)stride + 8 * ch) * 2);
     }
   };
-  int kw[PER], vw[PER];  // where they go in the images
+  // where they go in the images: RSTEP rows on, the K swizzle has one of two forms and the V swizzle stays
+  static_assert(RSTEP == 16 || RSTEP == 32, "rows between a thread's pieces");
+  int kw[2];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int r = tr + RSTEP * i;
-    kw[i] = r * ROWB + 16 * (ch ^ kx(r));
-    vw[i] = IMG + r * ROWB + 16 * (ch ^ vx<ROWB>(r & 31));
-  }
-  auto tile = [&](auto edge_, int kb, const char* kimg) {
-    constexpr bool EDGE = decltype(edge_)::value;
-    const char* const vimg = kimg + IMG;
-    f32x4 sc[NT][4];
+  for (int h = 0; h < 2; ++h) kw[h] = tr * ROWB + 16 * (ch ^ kx(tr + RSTEP * h));
+  const int vw = tr * ROWB + 16 * (ch ^ vx<ROWB>(tr));
+  char* const kimg = smem;            // two K images, two V images
+  char* const vimg = smem + 2 * IMG;
+  auto put_k = [&](const u32x4* from, int buf) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) *reinterpret_cast<u32x4*>(kimg + buf * IMG + kw[i & 1] + i * RSTEP * ROWB) = from[i];
+  };
+  auto put_v = [&](const u32x4* from, int buf) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) *reinterpret_cast<u32x4*>(vimg + buf * IMG + vw + i * RSTEP * ROWB) = from[i];
+  };
+  f32x4 sc[NT][4];
+  // a product's addresses, settled before its stretch of code is put in order (address arithmetic would count as work to place)
+  auto k_at = [&](int buf, uint32_t* at) {
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      at[s] = (uint32_t)((buf * IMG + ka) ^ (64 * s));
+      asm volatile("" : "+v"(at[s]));
+    }
+  };
+  auto v_at = [&](int buf, uint32_t* at) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      at[c] = (uint32_t)((buf * IMG + va) ^ (32 * c));
+      asm volatile("" : "+v"(at[c]));
+    }
+  };
+  auto scores = [&](const uint32_t* at, f32x4 (*s4)[4]) {
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) sc[n][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int n = 0; n < NT; ++n) s4[n][b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
-        const bf16x8 kf = lds_read8(kimg + ka[s] + (32 * (b >> 1) + 4 * (b & 1)) * ROWB);
+        const bf16x8 kf = lds_read8(kimg + at[s] + (32 * (b >> 1) + 4 * (b & 1)) * ROWB);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) sc[n][b] = mfma16(kf, qf[n][s], sc[n][b]);
+        for (int n = 0; n < NT; ++n) s4[n][b] = mfma16(kf, qf[n][s], s4[n][b]);
       }
     }
-    // issue order: the operands of one 16-key product ahead of the matrix cores
-    __builtin_amdgcn_sched_group_barrier(kDsRead, NS, 0);
+  };
+  // One tile: its scores are there. The next tile's scores (matrix cores) are computed beside this one's weights (vector ALUs).
+  auto tile = [&](auto edge_, auto next_, int kb, int buf) {
+    constexpr bool EDGE = decltype(edge_)::value, NEXT = decltype(next_)::value, SIFT = EDGE && OWN;
 #pragma unroll
-    for (int b = 0; b < 3; ++b) {
-      __builtin_amdgcn_sched_group_barrier(kDsRead, NS, 0);
-      __builtin_amdgcn_sched_group_barrier(kMfma, NS * NT, 0);
-    }
-    __builtin_amdgcn_sched_group_barrier(kMfma, NS * NT, 0);
-    __builtin_amdgcn_sched_barrier(0);
+    for (int n = 0; n < NT; ++n) raise_max<EDGE, 2, NC>(sc[n], lim[n] - kb - 8 * g, p.sl2, m[n], acc[n]);
     bf16x8 pf[NT][2];
+    f32x4 nx[NT][4];
+    uint32_t kat[NS], vat[NC];
+    if constexpr (NEXT) k_at(buf ^ 1, kat);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (NEXT) scores(kat, nx);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      softmax_step<EDGE, 2, NC>(sc[n], lim[n] - kb - 8 * g, p.sl2, m[n], acc[n], pf[n]);
-      acc[n][NC] = sum_p(pf[n][1], sum_p(pf[n][0], acc[n][NC]));
+    for (int n = 0; n < NT; ++n) weights<EDGE, 2>(sc[n], lim[n] - kb - 8 * g, p.sl2, m[n], pf[n]);
+    if constexpr (NEXT && !EDGE) {
+      // issue order: operands of one 16-key product ahead, and between two matrix instructions what one of them leaves time for
+      __builtin_amdgcn_sched_group_barrier(kDsRead, NS, 0);
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        if (b < 3) __builtin_amdgcn_sched_group_barrier(kDsRead, NS, 0);
+#pragma unroll
+        for (int i = 0; i < NS * NT; ++i) {
+          __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(kTrans, 8 / (NS * NT), 0);
+        }
+      }
     }
     __builtin_amdgcn_sched_barrier(0);
-    constexpr bool SIFT = EDGE && OWN;
+    v_at(buf, vat);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[n][NC] = sum_p(pf[n][1], sum_p(pf[n][0], acc[n][NC]));
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        const bf16x8 vf = cat44(lds_tr_read(vimg + va[c] + 32 * b * ROWB), lds_tr_read(vimg + va[c] + (32 * b + 4) * ROWB));
+        const char* vp = vimg + vat[c] + 32 * b * ROWB;
+        const bf16x8 vf = cat44(lds_tr_read(vp), lds_tr_read(vp + 4 * ROWB));
         if constexpr (SIFT) {
           bf16x8 pfn[NT];
           f32x4 an[NT];
@@ -507,34 +535,58 @@ __device__ __forceinline__ void by_rows(const Args& p, const Work& w, char* smem
           for (int n = 0; n < NT; ++n) acc[n][c] = mfma16(vf, pf[n][b], acc[n][c]);
         }
       }
-    if constexpr (!SIFT) {  // issue order: four 16-dim blocks' operands ahead
-      constexpr int VG = 4;
-      __builtin_amdgcn_sched_group_barrier(kDsRead, 2 * VG, 0);
+    if constexpr (!SIFT) {  // issue order: three 16-dim blocks' operands ahead
+      __builtin_amdgcn_sched_group_barrier(kDsRead, 6, 0);
 #pragma unroll
-      for (int i = 0; i + 1 < 2 * NC / VG; ++i) {
-        __builtin_amdgcn_sched_group_barrier(kDsRead, 2 * VG, 0);
-        __builtin_amdgcn_sched_group_barrier(kMfma, VG * NT, 0);
+      for (int i = 0; i < 2 * NC - 3; ++i) {
+        __builtin_amdgcn_sched_group_barrier(kMfma, NT, 0);
+        __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 0);
       }
-      __builtin_amdgcn_sched_group_barrier(kMfma, VG * NT, 0);
+      __builtin_amdgcn_sched_group_barrier(kMfma, 3 * NT, 0);
     }
     __builtin_amdgcn_sched_barrier(0);
-  };
-  fetch(w.k0);
-  int buf = 0, kb = w.k0;
-  auto stage = [&](auto edge_) {
-    char* const kimg = smem + buf * (2 * IMG);
+    if constexpr (NEXT) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      *reinterpret_cast<u32x4*>(kimg + kw[i]) = kr[i];
-      *reinterpret_cast<u32x4*>(kimg + vw[i]) = vr[i];
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) sc[n][b] = nx[n][b];
     }
-    // the tile is there, and every wave is done with the tile before (whose images the next one takes)
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (kb + TK < w.kend) fetch(kb + TK);
-    if (live) tile(edge_, kb, kimg);
   };
-  for (; kb < w.kend && kb + TK <= w.lim0; kb += TK, buf ^= 1) stage(std::false_type{});
-  for (; kb < w.kend; kb += TK, buf ^= 1) stage(std::true_type{});
+  // Tile i reads V image i and K image i + 1 (both modulo 2); meanwhile V i + 1 and K i + 2 go from registers into the images
+  // that tile i - 1 has left, and V i + 2 and K i + 3 into the registers.
+  u32x4 kr[PER], vr[PER];
+  int kb = w.k0, buf = 0;
+  auto barrier = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+  fetch(w.k, w.ks, ko, kb, kr);
+  fetch(w.v, w.vs, vo, kb, vr);
+  put_k(kr, 0);
+  put_v(vr, 0);
+  if (kb + TK < w.kend) {
+    fetch(w.k, w.ks, ko, kb + TK, kr);
+    put_k(kr, 1);
+    fetch(w.v, w.vs, vo, kb + TK, vr);
+  }
+  if (kb + 2 * TK < w.kend) fetch(w.k, w.ks, ko, kb + 2 * TK, kr);
+  barrier();
+  uint32_t kat0[NS];
+  k_at(0, kat0);
+  if (live) scores(kat0, sc);
+  auto stage = [&](auto edge_, auto next_) {
+    // every wave is done with the tile before: image `buf` of K (whose scores are taken) and the other one of V are free
+    barrier();
+    if (kb + TK < w.kend) put_v(vr, buf ^ 1);
+    if (kb + 2 * TK < w.kend) {
+      put_k(kr, buf);
+      fetch(w.v, w.vs, vo, kb + 2 * TK, vr);
+    }
+    if (kb + 3 * TK < w.kend) fetch(w.k, w.ks, ko, kb + 3 * TK, kr);
+    if (live) tile(edge_, next_, kb, buf);
+    kb += TK;
+    buf ^= 1;
+  };
+  while (kb + TK < w.kend && kb + TK <= w.lim0) stage(std::false_type{}, std::true_type{});
+  while (kb + TK < w.kend) stage(std::true_type{}, std::true_type{});
+  stage(std::true_type{}, std::false_type{});
   if (!live) return;
   const int RR = p.B * p.T * p.G;
 #pragma unroll
