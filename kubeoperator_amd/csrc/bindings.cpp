@@ -733,7 +733,7 @@ std::vector<Tensor> verify_draft(const Tensor& target, const c10::optional<Tenso
   auto out = at::empty({B, T + 1}, target.options().dtype(at::kLong));
   auto accepted = at::empty({B}, target.options().dtype(at::kInt));
   if (B == 0) return {out, accepted};
-  auto ws = at::empty({kop::verify_draft_workspace((int)B, (int)T, (int)V)}, target.options().dtype(at::kByte));
+  auto ws = at::empty({kop::verify_draft_workspace((int)B, (int)T, (int)V, f32)}, target.options().dtype(at::kByte));
   rc(kop::verify_draft(target.data_ptr(), target.stride(0), target.stride(1), dp, ds_b, ds_t, f32,
                        tokens.data_ptr<int64_t>(), u.data_ptr<float>(), nd, (int)B, (int)T, (int)V, temperature,
                        ws.data_ptr(), out.data_ptr<int64_t>(), accepted.data_ptr<int>(), cur_stream()),

@@ -80,6 +80,7 @@ struct Teacher {
       if (i < 0) continue;
       float sum = 0.f;
       bool first = true;
+#pragma unroll 8
       for (int j = 0; j < K; ++j) {
         const bool same = idx[j] == i;
         sum += same ? p[j] : 0.f;
@@ -121,7 +122,7 @@ __device__ __forceinline__ void repack(u32x4* v) {
 // One workgroup per row that holds the whole row: CR 16-byte pieces per thread in registers, CL more in LDS, so every
 // logit is read once and every gradient element written once. Two plain reductions, no running rescale.
 template <int NT, int CR, int CL>
-__global__ void __launch_bounds__(NT, CL > 0 ? 4 : 1) distill_row_kernel(Args a) {
+__global__ void __launch_bounds__(NT, NT >= 512 && CR + CL > 16 ? 4 : 1) distill_row_kernel(Args a) {
   __shared__ Teacher<NT> s_t;
   __shared__ u32x4 s_w[CL > 0 ? CL * NT : 1];
   const int t = threadIdx.x;
@@ -267,10 +268,28 @@ int distill_topk(const bf16_t* logits, int64_t ld, int64_t N, int V, const int* 
   if (N == 0) return 0;
   const Args a = {logits, ld, V, K, index, teacher, weight, temp, loss, grad, gld};
   const unsigned n = (unsigned)N;
-  if (V < 256 * 8 * 4 + 8) distill_row_kernel<256, 4, 0><<<n, 256, 0, stream>>>(a);
-  else if (V < 512 * 8 * 16 + 8) distill_row_kernel<512, 16, 0><<<n, 512, 0, stream>>>(a);
-  else if (V < 512 * 8 * 32 + 8) distill_row_kernel<512, 23, 9><<<n, 512, 0, stream>>>(a);
-  else distill_long_kernel<512><<<n, 512, 0, stream>>>(a);
+  // The smallest workgroup that holds a row, so that several rows share a CU: a wave up to 4096 logits, 512 threads above (two
+  // rows per CU). With too few rows to fill the chip that way, 1024 threads per row instead: half the time of a row.
+#define KOP_ROW(NT, CR, CL)                                        \
+  if (V < NT * 8 * (CR + CL) + 8) {                                \
+    distill_row_kernel<NT, CR, CL><<<n, NT, 0, stream>>>(a);       \
+    return hipGetLastError() == hipSuccess ? 0 : -9;               \
+  }
+  KOP_ROW(64, 1, 0)
+  KOP_ROW(64, 2, 0)
+  KOP_ROW(64, 4, 0)
+  KOP_ROW(64, 8, 0)
+  KOP_ROW(256, 4, 0)
+  if (N <= 256) {
+    KOP_ROW(1024, 4, 0)
+    KOP_ROW(1024, 8, 0)
+    KOP_ROW(1024, 16, 0)
+  }
+  KOP_ROW(512, 8, 0)
+  KOP_ROW(512, 16, 0)
+  KOP_ROW(512, 23, 9)
+#undef KOP_ROW
+  distill_long_kernel<512><<<n, 512, 0, stream>>>(a);
   return hipGetLastError() == hipSuccess ? 0 : -9;
 }
 

@@ -52,7 +52,7 @@ int distill_topk(const bf16_t* logits, int64_t ld, int64_t N, int V, const int* 
 // verify.hip: accepted prefix of T drafted tokens per sequence and the token after it, from uniform numbers u [B, T+1];
 // temp 0: greedy. Row strides in elements; n_draft [B] or null; workspace: verify_draft_workspace() bytes, 8-byte aligned
 constexpr int kVerifyMaxDraft = 32;
-int64_t verify_draft_workspace(int B, int T, int V);
+int64_t verify_draft_workspace(int B, int T, int V, bool f32);
 int verify_draft(const void* target, int64_t ts_b, int64_t ts_t, const void* draft, int64_t ds_b, int64_t ds_t, bool f32,
                  const int64_t* tokens, const float* u, const int* n_draft, int B, int T, int V, double temp,
                  void* workspace, int64_t* out, int* accepted, hipStream_t stream);

@@ -12,9 +12,10 @@
 // largest finite value. A row without any probability accepts nothing and yields -1.
 //
 // Three launches (greedy: two): maximum and sum of every 8192-logit chunk (the only pass over all logits, each held in
-// registers between its maximum and its sum); acceptance and the sums of r over 1024-logit pieces (the two rows of each
+// registers between its maximum and its sum); acceptance and the sums of r over small pieces (the two rows of each
 // sequence's refusal, again); the pick inside the one piece that u_T falls into. A workgroup that needs the acceptance
-// re-derives it from the chunk statistics (a few hundred numbers): no atomics, no order-dependent sums.
+// re-derives it from the chunk statistics (a few hundred numbers): no atomics, no order-dependent sums. Small problems, whose
+// time is all launches, do the same in one: a workgroup per sequence.
 #include <float.h>
 
 #include "common.h"
@@ -25,7 +26,11 @@ namespace kop {
 namespace {
 constexpr int kT = 256;       // threads of a workgroup
 constexpr int kChunk = 8192;  // logits per workgroup of the first pass: 32 per thread
-constexpr int kPiece = 1024;  // logits per wave of the second pass, per workgroup of the third
+// logits per sum of the second pass: what a wave reads with one access each
+template <typename E>
+constexpr int piece() { return 64 * 16 / (int)sizeof(E); }
+constexpr int kPieces = 4;        // pieces per wave of the second pass
+constexpr int kOneRow = 4096, kOneLaunch = 32768;  // logits per row and sequence up to which one launch does everything
 constexpr int kMaxRows = 2 * kVerifyMaxDraft + 1;
 
 template <typename E>
@@ -86,9 +91,52 @@ __device__ __forceinline__ double exp2_neg(double x) {
 // e^((z - m) / temp) for z <= m, c = log2 e / temp. The difference of two fp32 values is exact in 64 bits, or far below 2^-1100
 __device__ __forceinline__ double weight(float z, float m, double c) { return exp2_neg(((double)z - (double)m) * c); }
 
+// lane exchanges of 64-bit values in registers (a __shfl is two LDS round trips): DPP inside 16-lane rows, swaps across
+template <int CTRL, bool ZERO = false>
+__device__ __forceinline__ double dpp_d(double v) {
+  return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, 0xF, 0xF, ZERO),
+                          __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, 0xF, 0xF, ZERO));
+}
+// the sum over each 16-lane row / over the wave, in every lane
+__device__ __forceinline__ double row_sum_d(double v) {
+  v += dpp_d<0xB1>(v);
+  v += dpp_d<0x4E>(v);
+  v += dpp_d<0x141>(v);
+  return v + dpp_d<0x140>(v);
+}
+__device__ __forceinline__ double row_min_d(double v) {
+  v = fmin(v, dpp_d<0xB1>(v));
+  v = fmin(v, dpp_d<0x4E>(v));
+  v = fmin(v, dpp_d<0x141>(v));
+  return fmin(v, dpp_d<0x140>(v));
+}
+__device__ __forceinline__ float row_max_f(float v) {
+  v = fmaxf(v, dpp_f32<0xB1>(v));
+  v = fmaxf(v, dpp_f32<0x4E>(v));
+  v = fmaxf(v, dpp_f32<0x141>(v));
+  return fmaxf(v, dpp_f32<0x140>(v));
+}
+__device__ __forceinline__ double readlane_d(double v, int lane) {
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), lane),
+                          __builtin_amdgcn_readlane(__double2loint(v), lane));
+}
 __device__ __forceinline__ double wave_sum_d(double v) {
+  v = row_sum_d(v);
+  return (readlane_d(v, 0) + readlane_d(v, 16)) + (readlane_d(v, 32) + readlane_d(v, 48));
+}
+// inclusive sum over the lanes in order
+__device__ __forceinline__ double wave_scan_d(double v) {
+  v += dpp_d<0x111, true>(v);  // row_shr 1, 2, 4, 8; zeros come in
+  v += dpp_d<0x112, true>(v);
+  v += dpp_d<0x114, true>(v);
+  v += dpp_d<0x118, true>(v);
+  const double a = readlane_d(v, 15), b = a + readlane_d(v, 31), c = b + readlane_d(v, 47);
+  const int row = (threadIdx.x >> 4) & 3;
+  return v + (row == 0 ? 0.0 : row == 1 ? a : row == 2 ? b : c);
+}
+__device__ __forceinline__ int wave_min_i(int v) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
   return v;
 }
 
@@ -123,6 +171,9 @@ __device__ __forceinline__ const E* row_ptr(const Args& a, int b, int r) {
                   : reinterpret_cast<const E*>(a.draft) + b * a.ds_b + (int64_t)(r - a.T - 1) * a.ds_t;
 }
 
+// whether sequence b's row r is one that none of its drafted tokens needs
+__device__ __forceinline__ bool idle(const Args& a, int r, int nd) { return r <= a.T ? r > nd : r - a.T - 1 >= nd; }
+
 // ---- pass 1: grid (chunks, rows, B); greedy needs the target's T+1 rows only
 template <typename E, bool GREEDY>
 __global__ void __launch_bounds__(kT) verify_stats_kernel(Args a) {
@@ -130,8 +181,7 @@ __global__ void __launch_bounds__(kT) verify_stats_kernel(Args a) {
   __shared__ float s_m[kT / 64];
   __shared__ double s_s[kT / 64];
   const int c = blockIdx.x, r = blockIdx.y, b = blockIdx.z, t = threadIdx.x;
-  const int nd = drafts(a, b);
-  if (r <= a.T ? r > nd : r - a.T - 1 >= nd) return;  // a row that no drafted token of this sequence needs
+  if (idle(a, r, drafts(a, b))) return;
   const E* x = row_ptr<E>(a, b, r);
   const int lo = c * kChunk, hi = min(a.V, lo + kChunk);
   Vec<E> v[NV];
@@ -157,8 +207,7 @@ __global__ void __launch_bounds__(kT) verify_stats_kernel(Args a) {
         for (int e = N - 1; e >= 0; --e)
           if (v[k].get(e) == m) at = lo + (k * kT + t) * N + e;
     }
-#pragma unroll
-    for (int k = 32; k > 0; k >>= 1) at = min(at, __shfl_xor(at, k, 64));
+    at = wave_min_i(at);
     if ((t & 63) == 0) s_s[t >> 6] = (double)at;
     __syncthreads();
     if (t == 0) {
@@ -184,61 +233,40 @@ __global__ void __launch_bounds__(kT) verify_stats_kernel(Args a) {
   }
 }
 
-// Called by whole workgroups: the chunk statistics of sequence b's rows folded to one (maximum, sum) per row -- greedy:
-// (maximum, argmax or -1) -- by 16 lanes a row; returns the number of accepted tokens (one lane a token) in every thread.
+// one drafted token's own logits, loaded before the rows' statistics are there
+struct Drafted {
+  int64_t x;
+  float lp, lq, u;
+};
 template <typename E, bool GREEDY>
-__device__ int decide(const Args& a, int b, float* s_m, double* s_s, int* s_j) {
-  const int t = threadIdx.x, sub = t & 15;
-  const int nd = drafts(a, b), rows = 2 * a.T + 1;
-  // the drafted tokens' own logits, on their way while the statistics are folded
-  int64_t x = -1;
-  float lp = 0.f, lq = 0.f, u = 0.f;
+__device__ __forceinline__ Drafted drafted(const Args& a, int b, int nd) {
+  const int t = threadIdx.x;
+  Drafted d = {-1, 0.f, 0.f, 0.f};
   if (t < nd) {
-    x = a.tokens[(int64_t)b * a.T + t];
-    if (!GREEDY && x >= 0 && x < a.V) {
-      lp = ld1(row_ptr<E>(a, b, t) + x);
-      lq = ld1(row_ptr<E>(a, b, a.T + 1 + t) + x);
-      u = a.u[(int64_t)b * (a.T + 1) + t];
+    d.x = a.tokens[(int64_t)b * a.T + t];
+    if (!GREEDY && d.x >= 0 && d.x < a.V) {
+      d.lp = ld1(row_ptr<E>(a, b, t) + d.x);
+      d.lq = ld1(row_ptr<E>(a, b, a.T + 1 + t) + d.x);
+      d.u = a.u[(int64_t)b * (a.T + 1) + t];
     }
   }
-  for (int r = t >> 4; r < (GREEDY ? a.T + 1 : rows); r += kT / 16) {
-    if (r <= a.T ? r > nd : r - a.T - 1 >= nd) continue;
-    const int64_t o = ((int64_t)b * rows + r) * a.nch;
-    float m = -INFINITY;
-    for (int c = sub; c < a.nch; c += 16) m = fmaxf(m, a.pm[o + c]);
-#pragma unroll
-    for (int k = 8; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor(m, k, 16));
-    double s = GREEDY ? 2147483647.0 : 0.0;
-    for (int c = sub; c < a.nch; c += 16) {
-      const float cm = a.pm[o + c];
-      const double cs = a.ps[o + c];
-      if (cm == -INFINITY) continue;
-      if constexpr (GREEDY) s = cm == m ? fmin(s, cs) : s;
-      else s += cs * weight(cm, m, a.c);
-    }
-#pragma unroll
-    for (int k = 8; k > 0; k >>= 1) {
-      const double v = __shfl_xor(s, k, 16);
-      s = GREEDY ? fmin(s, v) : s + v;
-    }
-    if (sub == 0) {
-      s_m[r] = m;
-      s_s[r] = GREEDY && m == -INFINITY ? -1.0 : s;
-    }
-  }
-  __syncthreads();
+  return d;
+}
+// The number of accepted tokens, one lane of the first wave a token, in every thread: s_m / s_s hold each row's (maximum, sum)
+// -- greedy: (maximum, argmax or -1).
+template <typename E, bool GREEDY>
+__device__ __forceinline__ int accept(const Args& a, const Drafted& d, int nd, const float* s_m, const double* s_s, int* s_j) {
+  const int t = threadIdx.x;
   if (t < 64) {
     bool ok = false;
-    if (t < nd) {
-      if (x >= 0 && x < a.V) {
-        if constexpr (GREEDY) {
-          ok = s_s[t] == (double)x;
-        } else {
-          const double zp = s_s[t], zq = s_s[a.T + 1 + t];
-          const double p = zp > 0.0 ? weight(lp, s_m[t], a.c) / zp : 0.0;
-          const double q = zq > 0.0 ? weight(lq, s_m[a.T + 1 + t], a.c) / zq : 0.0;
-          ok = (double)u * q < p;
-        }
+    if (t < nd && d.x >= 0 && d.x < a.V) {
+      if constexpr (GREEDY) {
+        ok = s_s[t] == (double)d.x;
+      } else {
+        const double zp = s_s[t], zq = s_s[a.T + 1 + t];
+        const double p = zp > 0.0 ? weight(d.lp, s_m[t], a.c) / zp : 0.0;
+        const double q = zq > 0.0 ? weight(d.lq, s_m[a.T + 1 + t], a.c) / zq : 0.0;
+        ok = (double)d.u * q < p;
       }
     }
     const uint64_t no = ~__ballot(ok);  // lanes past the drafts refuse
@@ -246,6 +274,38 @@ __device__ int decide(const Args& a, int b, float* s_m, double* s_s, int* s_j) {
   }
   __syncthreads();
   return s_j[0];
+}
+// The same from the chunk statistics, folded to one (maximum, sum) per row by 16 lanes each. Called by whole workgroups.
+template <typename E, bool GREEDY>
+__device__ int decide(const Args& a, int b, float* s_m, double* s_s, int* s_j) {
+  const int t = threadIdx.x, sub = t & 15;
+  const int nd = drafts(a, b), rows = 2 * a.T + 1;
+  const Drafted d = drafted<E, GREEDY>(a, b, nd);
+  for (int r = t >> 4; r < (GREEDY ? a.T + 1 : rows); r += kT / 16) {
+    if (idle(a, r, nd)) continue;
+    const int64_t o = ((int64_t)b * rows + r) * a.nch;
+    // the first 16 chunks' numbers in registers: most vocabularies have no more
+    const float c0 = sub < a.nch ? a.pm[o + sub] : -INFINITY;
+    const double s0 = sub < a.nch ? a.ps[o + sub] : 0.0;
+    float m = c0;
+    for (int c = sub + 16; c < a.nch; c += 16) m = fmaxf(m, a.pm[o + c]);
+    m = row_max_f(m);
+    double s = GREEDY ? 2147483647.0 : 0.0;
+    auto fold = [&](float cm, double cs) {
+      if (cm == -INFINITY) return;
+      if constexpr (GREEDY) s = cm == m ? fmin(s, cs) : s;
+      else s += cs * weight(cm, m, a.c);
+    };
+    fold(c0, s0);
+    for (int c = sub + 16; c < a.nch; c += 16) fold(a.pm[o + c], a.ps[o + c]);
+    s = GREEDY ? row_min_d(s) : row_sum_d(s);
+    if (sub == 0) {
+      s_m[r] = m;
+      s_s[r] = GREEDY && m == -INFINITY ? -1.0 : s;
+    }
+  }
+  __syncthreads();
+  return accept<E, GREEDY>(a, d, nd, s_m, s_s, s_j);
 }
 
 // r_i at the refused (or last) position
@@ -257,10 +317,20 @@ struct Rest {
   __device__ __forceinline__ Rest(const Args& a, int b, const Head& h)
       : x(row_ptr<E>(a, b, h.j)), y(h.two ? row_ptr<E>(a, b, a.T + 1 + h.j) : nullptr), mp(h.mp), mq(h.mq), ip(h.ip),
         iq(h.iq), c(a.c) {}
-  __device__ __forceinline__ double p(float z) const { return weight(z, mp, c) * ip; }
   __device__ __forceinline__ double r(float z, float d) const {
-    const double v = p(z);
+    const double v = weight(z, mp, c) * ip;
     return y ? fmax(v - weight(d, mq, c) * iq, 0.0) : v;
+  }
+  // r of the lane's vector of piece pc (0 past the row's end)
+  __device__ __forceinline__ void vec(int pc, int V, double* out) const {
+    constexpr int N = Vec<E>::N;
+    const int i = pc * piece<E>() + (threadIdx.x & 63) * N;
+    Vec<E> v, d;
+    v.load(x, i, V);
+    if (y) d.load(y, i, V);
+    else d.w = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int e = 0; e < N; ++e) out[e] = r(v.get(e), d.get(e));
   }
 };
 __device__ __forceinline__ Head head_of(const Args& a, int b, int j, const float* s_m, const double* s_s) {
@@ -274,183 +344,220 @@ __device__ __forceinline__ Head head_of(const Args& a, int b, int j, const float
   h.iq = h.two ? 1.0 / s_s[k] : 0.0;
   return h;
 }
+// the sums of COUNT pieces from `pc` on into pr, by one wave
+template <int COUNT, typename E>
+__device__ __forceinline__ void piece_sums(const Args& a, const Rest<E>& f, int pc, double* pr) {
+  constexpr int N = Vec<E>::N;
+#pragma unroll
+  for (int k = 0; k < COUNT; ++k) {
+    double v[N], s = 0.0;
+    f.vec(pc + k, a.V, v);  // zeros past the last piece
+#pragma unroll
+    for (int e = 0; e < N; ++e) s += v[e];
+    s = wave_sum_d(s);
+    if ((threadIdx.x & 63) == 0 && pc + k < a.npc) pr[pc + k] = s;
+  }
+}
 
-// ---- pass 2 (not greedy): grid (pieces / 4, B), a wave per piece
+// ---- pass 2 (not greedy): grid (pieces / (4 kPieces), B)
 template <typename E>
 __global__ void __launch_bounds__(kT) verify_rest_kernel(Args a) {
-  constexpr int N = Vec<E>::N, NV = kPiece / (64 * N);
   __shared__ float s_m[kMaxRows];
   __shared__ double s_s[kMaxRows];
   __shared__ int s_j[1];
-  const int b = blockIdx.y, lane = threadIdx.x & 63;
-  const int pc = blockIdx.x * (kT / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b = blockIdx.y, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int j = decide<E, false>(a, b, s_m, s_s, s_j);
   const Head h = head_of(a, b, j, s_m, s_s);
   if (blockIdx.x == 0 && threadIdx.x == 0) a.head[b] = h;
-  if (pc >= a.npc) return;
-  const Rest<E> f(a, b, h);
-  const int lo = pc * kPiece, hi = min(a.V, lo + kPiece);
-  Vec<E> v[NV], d[NV];
-#pragma unroll
-  for (int k = 0; k < NV; ++k) v[k].load(f.x, lo + (k * 64 + lane) * N, hi);
-  if (f.y) {
-#pragma unroll
-    for (int k = 0; k < NV; ++k) d[k].load(f.y, lo + (k * 64 + lane) * N, hi);
-  } else {
-#pragma unroll
-    for (int k = 0; k < NV; ++k) d[k].w = u32x4{0u, 0u, 0u, 0u};
-  }
-  double s = 0.0;
-#pragma unroll
-  for (int k = 0; k < NV; ++k)
-#pragma unroll
-    for (int e = 0; e < N; ++e) s += f.r(v[k].get(e), d[k].get(e));
-  s = wave_sum_d(s);
-  if (lane == 0) a.pr[(int64_t)b * a.npc + pc] = s;
+  piece_sums<kPieces>(a, Rest<E>(a, b, h), (blockIdx.x * (kT / 64) + wv) * kPieces, a.pr + (int64_t)b * a.npc);
 }
 
-// inclusive sum over the workgroup's threads in order; every thread also gets the total
-__device__ __forceinline__ double block_scan(double v, double* s_w, double& total) {
-  const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
+// One wave: the smallest of n items whose running sum, from `before` on, passes `want` -- past the last sum (u >= 1, rounding) the
+// last item that is more than 0, -1 if there is none. Lane l owns items l * per .. and gives their values through `at`.
+// `before` becomes the running sum in front of the item.
+template <int PER, typename F>  // PER: items of a lane, 0: as many as n takes
+__device__ __forceinline__ int search(int n, F at, double want, double& before) {
+  const int lane = threadIdx.x & 63, per = PER > 0 ? PER : (n + 63) / 64;
+  double mine = 0.0;
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double w = __shfl_up(v, o, 64);
-    if (lane >= o) v += w;
+  for (int k = 0; k < per; ++k)
+    if (lane * per + k < n) mine += at(lane * per + k, k);
+  const double inc = before + wave_scan_d(mine);
+  const uint64_t over = __ballot(mine > 0.0 && inc > want), some = __ballot(mine > 0.0);
+  if (!some) {
+    before = readlane_d(inc, 63);
+    return -1;
   }
-  __syncthreads();  // s_w may still be read
-  if (lane == 63) s_w[wv] = v;
-  __syncthreads();
-  total = 0.0;
+  const int l = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
+  double run = inc - mine, front = 0.0;
+  int found = -1;
+  bool hit = false;
 #pragma unroll
-  for (int w = 0; w < kT / 64; ++w) {
-    v += w < wv ? s_w[w] : 0.0;
-    total += s_w[w];
+  for (int k = 0; k < per; ++k) {
+    const double v = lane * per + k < n ? at(lane * per + k, k) : 0.0;
+    const bool take = v > 0.0 && !hit;
+    found = take ? lane * per + k : found;
+    front = take ? run : front;
+    run = take ? run + v : run;
+    hit = hit || (take && run > want);
   }
-  return v;
-}
-// the lowest `i` of any thread (0x7fffffff: none), in every thread
-__device__ __forceinline__ int block_min(int i, int* s_w) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) i = min(i, __shfl_xor(i, o, 64));
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) s_w[threadIdx.x >> 6] = i;
-  __syncthreads();
-  return min(min(s_w[0], s_w[1]), min(s_w[2], s_w[3]));
+  before = readlane_d(front, l);
+  return __builtin_amdgcn_readlane(found, l);
 }
 
-// ---- pass 3: grid B
+// One wave: the token drawn from r (h.j's row), from its pieces' sums
+template <typename E>
+__device__ int64_t draw(const Args& a, int b, const Head& h, const double* pr) {
+  constexpr int N = Vec<E>::N;
+  Rest<E> f(a, b, h);
+  double total = 0.0;
+  const int lane = threadIdx.x & 63;
+  for (int i = lane; i < a.npc; i += 64) total += pr[i];
+  total = wave_sum_d(total);
+  const double u = (double)a.u[(int64_t)b * (a.T + 1) + a.T];
+  double before = 0.0;
+  int first, last;
+  if (total > 0.0) {
+    first = search<0>(a.npc, [&](int i, int) { return pr[i]; }, u * total, before);
+    last = first + 1;
+  } else {  // r = 0 everywhere: the target's own distribution, whose total is 1, from the first piece on
+    if (!(h.ip > 0.0)) return -1;
+    f.y = nullptr;
+    total = 1.0;
+    first = 0;
+    last = a.npc;
+  }
+  int token = -1;
+  const double want = u * total;
+  for (int pc = first; pc < last; ++pc) {
+    double v[N], front = before, sum = 0.0;
+    f.vec(pc, a.V, v);
+#pragma unroll
+    for (int e = 0; e < N; ++e) sum += v[e];
+    sum = wave_sum_d(sum);
+    const int i = search<N>(piece<E>(), [&](int, int k) {
+      double w = v[0];
+#pragma unroll
+      for (int e = 1; e < N; ++e) w = k == e ? v[e] : w;
+      return w;
+    }, want, front);
+    if (i >= 0) token = pc * piece<E>() + i;
+    before += sum;
+    if (before > want && token >= 0) break;
+  }
+  return token;
+}
+// by one wave: the kept tokens, the next one, then -1
+__device__ __forceinline__ void put(const Args& a, int b, int j, int64_t next) {
+  const int lane = threadIdx.x & 63;
+  if (lane <= a.T)
+    a.out[(int64_t)b * (a.T + 1) + lane] = lane < j ? a.tokens[(int64_t)b * a.T + lane] : lane == j ? next : -1;
+  if (lane == 0) a.accepted[b] = j;
+}
+
+// ---- pass 3: grid B; one wave (greedy: one workgroup)
+template <typename E>
+__global__ void __launch_bounds__(64) verify_draw_kernel(Args a) {
+  const int b = blockIdx.x;
+  const Head h = a.head[b];
+  put(a, b, h.j, draw<E>(a, b, h, a.pr + (int64_t)b * a.npc));
+}
+template <typename E>
+__global__ void __launch_bounds__(kT) verify_greedy_kernel(Args a) {
+  __shared__ float s_m[kMaxRows];
+  __shared__ double s_s[kMaxRows];
+  __shared__ int s_j[1];
+  const int b = blockIdx.x, j = decide<E, true>(a, b, s_m, s_s, s_j);
+  if (threadIdx.x < 64) put(a, b, j, (int64_t)s_s[j]);
+}
+
+// ---- all of it for a small problem: grid B. A wave takes every fourth row, twice (maximum, then sum: the row is in cache).
 template <typename E, bool GREEDY>
-__global__ void __launch_bounds__(kT) verify_pick_kernel(Args a) {
-  __shared__ double s_w[kT / 64];
-  __shared__ int s_i[kT / 64];
-  const int b = blockIdx.x, t = threadIdx.x;
-  int j;
-  int64_t next = -1;
-  if constexpr (GREEDY) {
-    __shared__ float s_m[kMaxRows];
-    __shared__ double s_s[kMaxRows];
-    j = decide<E, true>(a, b, s_m, s_s, s_i);
-    next = (int64_t)s_s[j];
-  } else {
-    constexpr int PER = kPiece / kT;  // consecutive logits of a thread
-    const Head h = a.head[b];
-    Rest<E> f(a, b, h);
-    j = h.j;
-    const double* pr = a.pr + (int64_t)b * a.npc;
-    // runs over groups of kT pieces, the last run one past the pieces that hold the answer
-    double total = 0.0, part;
-    for (int g = 0; g < a.npc; g += kT) {
-      block_scan(g + t < a.npc ? pr[g + t] : 0.0, s_w, part);
-      total += part;
-    }
-    const bool none = !(total > 0.0);  // r = 0 everywhere: the target's own distribution, by its chunks
-    if (none) {
-      f.y = nullptr;
-      total = f.ip > 0.0 ? 1.0 : 0.0;
-    }
-    if (total > 0.0) {
-      const int64_t o = ((int64_t)b * (2 * a.T + 1) + j) * a.nch;
-      const int n = none ? a.nch : a.npc, size = none ? kChunk : kPiece;
-      const double want = (double)a.u[(int64_t)b * (a.T + 1) + a.T] * total;
-      // the piece that `want` falls into; past the last sum (u >= 1, rounding): the last piece with anything in it
-      double run = 0.0, before = 0.0;
-      int at = 0x7fffffff, last = -1;
-      double last_before = 0.0;
-      for (int g = 0; g < n && at == 0x7fffffff; g += kT) {
-        const int i = g + t;
-        double v = 0.0;
-        if (i < n) v = none ? a.ps[o + i] * weight(a.pm[o + i], f.mp, f.c) * f.ip : pr[i];
-        if (none && i < n && a.pm[o + i] == -INFINITY) v = 0.0;
-        const double inc = run + block_scan(v, s_w, part);
-        at = block_min(i < n && v > 0.0 && inc > want ? i : 0x7fffffff, s_i);
-        const int nz = block_min(v > 0.0 ? -i : 0x7fffffff, s_i);  // minus the group's last piece with anything in it
-        const int pick = at != 0x7fffffff ? at : nz != 0x7fffffff ? -nz : -1;
-        if (pick >= 0) {
-          __syncthreads();
-          if (i == pick) s_w[0] = inc - v;
-          __syncthreads();
-          last = pick;
-          last_before = s_w[0];
-          __syncthreads();
-        }
-        run += part;
-      }
-      before = last_before;
-      // inside it: PER consecutive logits a thread, so that the order is that of the indexes
-      int hit = 0x7fffffff, tail = -1;
-      const int lo = last * size, hi = min(a.V, lo + size);
-      for (int base = lo; base < hi && hit == 0x7fffffff; base += kPiece) {
-        double v[PER], mine = 0.0;
-        const int i0 = base + t * PER;
+__global__ void __launch_bounds__(kT) verify_small_kernel(Args a) {
+  constexpr int N = Vec<E>::N;
+  __shared__ float s_m[kMaxRows];
+  __shared__ double s_s[kMaxRows], s_pr[kOneRow / piece<E>() + 1];
+  __shared__ int s_j[1];
+  const int b = blockIdx.x, t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int nd = drafts(a, b);
+  const Drafted d = drafted<E, GREEDY>(a, b, nd);
+  for (int r = wv; r < (GREEDY ? a.T + 1 : 2 * a.T + 1); r += kT / 64) {
+    if (idle(a, r, nd)) continue;
+    const E* x = row_ptr<E>(a, b, r);
+    float m = -INFINITY;
+    int at = 0x7fffffff;
+    for (int i = lane * N; i < a.V; i += 64 * N) {
+      Vec<E> v;
+      v.load(x, i, a.V);
 #pragma unroll
-        for (int e = 0; e < PER; ++e) {
-          const bool in = i0 + e < hi;
-          v[e] = in ? f.r(ld1(f.x + i0 + e), f.y ? ld1(f.y + i0 + e) : 0.f) : 0.0;
-          mine += v[e];
-        }
-        const double inc = block_scan(mine, s_w, part);
-        double at_e = before + (inc - mine);
-        int h = 0x7fffffff, l = 0x7fffffff;
-#pragma unroll
-        for (int e = 0; e < PER; ++e) {
-          at_e += v[e];
-          if (v[e] > 0.0) {
-            l = -(i0 + e);
-            if (h == 0x7fffffff && at_e > want) h = i0 + e;
-          }
-        }
-        hit = block_min(h, s_i);
-        l = block_min(l, s_i);
-        if (l != 0x7fffffff) tail = -l;
-        before += part;
+      for (int e = 0; e < N; ++e) {
+        const float z = v.get(e);
+        at = z > m ? i + e : at;
+        m = fmaxf(m, z);
       }
-      next = hit != 0x7fffffff ? hit : tail;
+    }
+    const float mine = m;
+    m = wave_max(m);
+    double s = 0.0;
+    if constexpr (GREEDY) {
+      at = wave_min_i(mine == m ? at : 0x7fffffff);
+      s = m > -INFINITY ? (double)at : -1.0;
+    } else {
+      m = fminf(m, FLT_MAX);
+      if (m > -INFINITY)
+        for (int i = lane * N; i < a.V; i += 64 * N) {
+          Vec<E> v;
+          v.load(x, i, a.V);
+#pragma unroll
+          for (int e = 0; e < N; ++e) s += weight(v.get(e), m, a.c);
+        }
+      s = wave_sum_d(s);
+    }
+    if (lane == 0) {
+      s_m[r] = m;
+      s_s[r] = s;
     }
   }
-  for (int i = t; i <= a.T; i += kT)
-    a.out[(int64_t)b * (a.T + 1) + i] = i < j ? a.tokens[(int64_t)b * a.T + i] : i == j ? next : -1;
-  if (t == 0) a.accepted[b] = j;
+  __syncthreads();
+  const int j = accept<E, GREEDY>(a, d, nd, s_m, s_s, s_j);
+  if constexpr (GREEDY) {
+    if (t < 64) put(a, b, j, (int64_t)s_s[j]);
+  } else {
+    const Head h = head_of(a, b, j, s_m, s_s);
+    const Rest<E> f(a, b, h);
+    for (int pc = wv; pc < a.npc; pc += kT / 64) piece_sums<1>(a, f, pc, s_pr);
+    __syncthreads();
+    if (t < 64) put(a, b, j, draw<E>(a, b, h, s_pr));
+  }
 }
 
 template <typename E>
 int launch(const Args& a, bool greedy, hipStream_t stream) {
-  const dim3 rows(a.nch, greedy ? a.T + 1 : 2 * a.T + 1, a.B);
-  if (greedy) {
-    verify_stats_kernel<E, true><<<rows, kT, 0, stream>>>(a);
-    verify_pick_kernel<E, true><<<a.B, kT, 0, stream>>>(a);
+  const int nrow = greedy ? a.T + 1 : 2 * a.T + 1;
+  // one workgroup per sequence is short of threads for long rows, three launches cost more than they do for short ones
+  if (a.V <= kOneRow && (int64_t)nrow * a.V <= kOneLaunch) {
+    if (greedy) verify_small_kernel<E, true><<<a.B, kT, 0, stream>>>(a);
+    else verify_small_kernel<E, false><<<a.B, kT, 0, stream>>>(a);
   } else {
-    verify_stats_kernel<E, false><<<rows, kT, 0, stream>>>(a);
-    verify_rest_kernel<E><<<dim3((a.npc + kT / 64 - 1) / (kT / 64), a.B), kT, 0, stream>>>(a);
-    verify_pick_kernel<E, false><<<a.B, kT, 0, stream>>>(a);
+    const dim3 rows(a.nch, nrow, a.B);
+    if (greedy) {
+      verify_stats_kernel<E, true><<<rows, kT, 0, stream>>>(a);
+      verify_greedy_kernel<E><<<a.B, kT, 0, stream>>>(a);
+    } else {
+      verify_stats_kernel<E, false><<<rows, kT, 0, stream>>>(a);
+      constexpr int per = kT / 64 * kPieces;
+      verify_rest_kernel<E><<<dim3((a.npc + per - 1) / per, a.B), kT, 0, stream>>>(a);
+      verify_draw_kernel<E><<<a.B, 64, 0, stream>>>(a);
+    }
   }
   return hipGetLastError() == hipSuccess ? 0 : -9;
 }
 inline int64_t chunks(int V) { return (V + kChunk - 1) / kChunk; }
-inline int64_t pieces(int V) { return (V + kPiece - 1) / kPiece; }
+inline int64_t pieces(int V, bool f32) { return (V + (f32 ? piece<float>() : piece<bf16_t>()) - 1) / (f32 ? piece<float>() : piece<bf16_t>()); }
 }  // namespace
 
-int64_t verify_draft_workspace(int B, int T, int V) {
-  return (int64_t)B * (2 * T + 1) * chunks(V) * (8 + 4) + (int64_t)B * (pieces(V) * 8 + sizeof(Head));
+int64_t verify_draft_workspace(int B, int T, int V, bool f32) {
+  return (int64_t)B * (2 * T + 1) * chunks(V) * (8 + 4) + (int64_t)B * (pieces(V, f32) * 8 + sizeof(Head));
 }
 
 int verify_draft(const void* target, int64_t ts_b, int64_t ts_t, const void* draft, int64_t ds_b, int64_t ds_t, bool f32,
@@ -463,7 +570,7 @@ int verify_draft(const void* target, int64_t ts_b, int64_t ts_t, const void* dra
   a.ts_b = ts_b, a.ts_t = ts_t, a.ds_b = ds_b, a.ds_t = ds_t;
   a.tokens = tokens, a.u = u, a.n_draft = n_draft;
   a.B = B, a.T = T, a.V = V;
-  a.nch = (int)chunks(V), a.npc = (int)pieces(V);
+  a.nch = (int)chunks(V), a.npc = (int)pieces(V, f32);
   a.c = temp > 0.0 ? 1.4426950408889634 / temp : 0.0;
   const int64_t n = (int64_t)B * (2 * T + 1) * a.nch;
   a.ps = reinterpret_cast<double*>(workspace);

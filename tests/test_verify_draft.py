@@ -90,7 +90,9 @@ def check(target, draft, tokens, u, temp, n_draft=None):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("B,T,V,temp", [(1, 0, 1, 1.0), (1, 0, 33, 1.0), (3, 1, 5, 1.0), (5, 3, 511, 0.7), (4, 4, 8192, 1.0),
                                         (2, 2, 8193, 1.3), (2, 8, 50257, 0.3), (2, 3, 128256, 1.0), (3, 32, 300, 1.0),
-                                        (4, 3, 1000, 0.0), (2, 5, 50304, 0.0), (1, 0, 128256, 0.0)])
+                                        (4, 3, 1000, 0.0), (2, 5, 50304, 0.0), (1, 0, 128256, 0.0), (3, 3, 4096, 1.0),
+                                        (3, 3, 4097, 1.0), (2, 4, 3640, 0.8), (2, 4, 3641, 0.8), (3, 2, 4096, 0.0),
+                                        (2, 1, 300001, 1.0), (70, 2, 255, 1.0)])
 def test_matches_plain(dev, dtype, B, T, V, temp):
     for seed in range(3):
         check(*make(B, T, V, dev, dtype, seed, temp), temp)
