@@ -237,6 +237,30 @@ __global__ void __launch_bounds__(kT) lora_up_kernel(const bf16_t* y, int64_t ys
     }
   }
   __syncthreads();
+  const int ng = (cnt + 15) / 16;
+  int n0 = blockIdx.y * chunks * 256 + wv * 64;
+  u32x4 yv[2], yn[2];
+  auto load_y = [&](int q, u32x4* v) {  // columns n0 + 8 g .. + 7 and + 32 .. + 39 of the group's rows
+    const int nc = n0 + 8 * g;
+    if (16 * q + col >= cnt) return;
+    const bf16_t* yr = y + (int64_t)s_list[16 * q + col] * ys + nc;
+    if (nc < N) v[0] = *reinterpret_cast<const u32x4*>(yr);
+    if (nc + 32 < N) v[1] = *reinterpret_cast<const u32x4*>(yr + 32);
+  };
+  bf16x8 bf[4][RS];
+  auto load_b = [&](int aj) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int nr = n0 + 8 * (col >> 2) + (col & 3) + 4 * (c & 1) + 32 * (c >> 1);
+      const bf16_t* br = b + ((int64_t)aj * N + nr) * r + 8 * g;
+#pragma unroll
+      for (int s = 0; s < RS; ++s) bf[c][s] = nr < N && 32 * s + 8 * g < r ? ld8(br + 32 * s) : zero8();
+    }
+  };
+  // the first columns' operands are on their way while the low-rank values are put together
+  int cur = GROUP && (int)blockIdx.x < n ? (int)blockIdx.x : -1;  // the adapter whose b operands are loaded
+  if (cur >= 0) load_b(cur);
+  load_y(0, yv);
   // low-rank values, scaled, as a bf16 value and its remainder; zeros past the rank
   for (int i = t; i < ((cnt + 15) & ~15) * 4 * RS; i += kT) {
     const int q = i / (4 * RS), k = 8 * (i % (4 * RS)), aj = s_j[q];
@@ -265,21 +289,13 @@ __global__ void __launch_bounds__(kT) lora_up_kernel(const bf16_t* y, int64_t ys
     *reinterpret_cast<u32x4*>(s_lo + q * PADR + k) = pack8(h);
   }
   __syncthreads();
-  const int ng = (cnt + 15) / 16;
-  for (int ch = 0; ch < chunks; ++ch) {
-    const int n0 = (blockIdx.y * chunks + ch) * 256 + wv * 64;
+  for (int ch = 0; ch < chunks; ++ch, n0 += 256) {
     if (n0 >= N) break;
-    const int nc = n0 + 8 * g;  // the lane's columns nc .. nc + 7 and nc + 32 .. nc + 39
-    u32x4 yv[2], yn[2];
-    auto load_y = [&](int q, u32x4* v) {
-      if (16 * q + col >= cnt) return;
-      const bf16_t* yr = y + (int64_t)s_list[16 * q + col] * ys + nc;
-      if (nc < N) v[0] = *reinterpret_cast<const u32x4*>(yr);
-      if (nc + 32 < N) v[1] = *reinterpret_cast<const u32x4*>(yr + 32);
-    };
-    int cur = -1;  // the adapter whose b operands are loaded
-    bf16x8 bf[4][RS];
-    load_y(0, yv);
+    if (ch > 0) {
+      cur = GROUP && (int)blockIdx.x < n ? (int)blockIdx.x : -1;
+      if (cur >= 0) load_b(cur);
+      load_y(0, yv);
+    }
     for (int q = 0; q < ng; ++q) {
       if (q + 1 < ng) load_y(q + 1, yn);
       const int j = s_j[16 * q + col];
@@ -300,13 +316,7 @@ __global__ void __launch_bounds__(kT) lora_up_kernel(const bf16_t* y, int64_t ys
           todo &= ~__ballot(match);
           if (aj != cur) {
             cur = aj;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const int nr = n0 + 8 * (col >> 2) + (col & 3) + 4 * (c & 1) + 32 * (c >> 1);
-              const bf16_t* br = b + ((int64_t)aj * N + nr) * r + 8 * g;
-#pragma unroll
-              for (int s = 0; s < RS; ++s) bf[c][s] = nr < N && 32 * s + 8 * g < r ? ld8(br + 32 * s) : zero8();
-            }
+            load_b(aj);
           }
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -321,6 +331,7 @@ __global__ void __launch_bounds__(kT) lora_up_kernel(const bf16_t* y, int64_t ys
           }
         }
       }
+      const int nc = n0 + 8 * g;
       if (16 * q + col < cnt) {
         bf16_t* orow = out + (int64_t)s_list[16 * q + col] * os + nc;
 #pragma unroll
