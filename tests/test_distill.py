@@ -190,6 +190,21 @@ def test_lmhead_gradients(dev):
 
 
 @pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """Logits of more than 2^31 elements, in place: the last rows against the formula."""
+    N, V, K = 17000, 128256, 4
+    rows, index, teacher, _ = make(3, V, K, "cuda")
+    logits = torch.zeros(N, V, dtype=torch.bfloat16, device="cuda")
+    logits[-3:] = rows
+    idx, tea = index[:1].repeat(N, 1), teacher[:1].repeat(N, 1)
+    idx[-3:], tea[-3:] = index, teacher
+    want = oracle(rows, index, teacher, 1.0, None)
+    loss, grad = kf.distill_topk(logits, idx, tea, 1.0, None, out=logits)
+    assert ((loss[-3:].double().cpu() - want[0]).abs() - want[2]).max() <= 0
+    assert ((grad[-3:].double().cpu() - want[1]).abs() - want[3]).max() <= 0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("V", [1000, 50304, 128256])
 def test_captured_call_replays_and_another_stream(V):
     logits, index, teacher, weight = make(6, V, 9, "cuda")

@@ -153,6 +153,21 @@ def test_refusals(dev):
 
 
 @pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """Outputs of more than 2^31 elements, written in place: the last rows against the formula, a row in front untouched."""
+    M, N = 280000, 8192
+    _, x, a, b, _, scale = make(64, 3, 8, 64, N, "cuda")
+    y = torch.zeros(M, N, dtype=torch.bfloat16, device="cuda")
+    index = torch.full((M,), -1, dtype=torch.int32, device="cuda")
+    index[-64:] = torch.randint(0, 3, (64,), dtype=torch.int32, device="cuda")
+    xs = x[:1].expand(M, 64).clone()
+    xs[-64:] = x
+    kf.lora_add(y, xs, a, b, index, scale, out=y)
+    want, tol = oracle(torch.zeros(64, N), x, a, b, index[-64:], scale)
+    assert ((y[-64:].double().cpu() - want).abs() - tol).max() <= 0 and not y[:-64].any()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("M", [24, 800])
 def test_captured_call_replays_and_another_stream(M):
     args = make(M, 6, 16, 512, 256, "cuda")

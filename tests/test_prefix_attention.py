@@ -153,6 +153,40 @@ def test_large_scores():
     run(8, 2, 8, 2, 128, 700, [2, 40, 90, 128, 129, 200, 300, 256], "cuda", size=32.0)
 
 
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1.0])
+@pytest.mark.parametrize("B,T", [(3, 2), (20, 9)])
+def test_other_scales(dev, scale, B, T):
+    """Any sign: maxima are taken before scaling; scale 0 weighs every key that is seen alike."""
+    qkv, kp, vp, kc, vc = make(B, T, 4, 2, 64, 70, 90, dev)
+    lens = torch.randint(0, 91, (B,), generator=torch.Generator().manual_seed(1)).to(torch.int32).to(dev)
+    q = 0.3 * qkv[:, : 4 * 64]
+    want, tol = oracle(q, kp, vp, kc, vc, lens, 90, T, scale)
+    got = kf.prefix_attention(q, kp, vp, kc, vc, lens, 90, T, scale)
+    assert ((got.double().cpu() - want).abs() - tol).max() <= 0
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """A cache and a prefix of more than 2^31 elements each; the queries match keys near the end."""
+    Hkv, D, n = 8, 128, (1 << 21) + 4097
+    g = torch.Generator(device="cuda").manual_seed(0)
+    caches = [torch.zeros(1, Hkv, n, D, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    at = n - 77
+    for t in caches:
+        t[:, :, at:] = torch.randn(1, Hkv, n - at, D, device="cuda", generator=g).bfloat16()
+    q = 4 * caches[0][0, :, at + 5].reshape(1, Hkv * D)
+    for kp, vp, kc, vc, lens in ((caches[0][0], caches[1][0], caches[0][:, :, :64].contiguous(), caches[1][:, :, :64].contiguous(), 0),
+                                 (caches[0][0, :, :0], caches[1][0, :, :0], caches[0], caches[1], n)):
+        got = kf.prefix_attention(q, kp, vp, kc, vc, torch.tensor([lens], dtype=torch.int32, device="cuda"), kc.shape[2])
+        # zero keys have score 0 and value 0: they only add to the normaliser
+        s = (caches[0][0, :, at:].double() @ q.view(Hkv, D, 1).double()).squeeze(-1) / math.sqrt(D)
+        e = torch.exp(s - s.amax(-1, keepdim=True))
+        want = (e.unsqueeze(1) @ caches[1][0, :, at:].double()).squeeze(1) / (
+            e.sum(-1) + (at) * torch.exp(-s.amax(-1))).unsqueeze(-1)
+        assert (got.double().view(Hkv, D) - want).abs().max() <= 3 * 2.0 ** -8 * float(caches[1].abs().max())
+
+
 @pytest.mark.gpu
 def test_agrees_with_decode_attention():
     """Without a prefix and for one token it is the framework's decode attention; with the prefix copied in front of every
