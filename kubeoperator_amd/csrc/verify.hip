@@ -16,6 +16,12 @@
 // sequence's refusal, again); the pick inside the one piece that u_T falls into. A workgroup that needs the acceptance
 // re-derives it from the chunk statistics (a few hundred numbers): no atomics, no order-dependent sums. Small problems, whose
 // time is all launches, do the same in one: a workgroup per sequence.
+//
+// 64 sequences, 4 drafts, 128256 fp32 logits: 60 us for the first pass (295 MB, 4.9 TB/s, what a copy reaches), 20 for the second
+// (128 rows again, mostly from cache; 16 million fp64 exponentials), 5.6 for the pick. One sequence, 3 drafts, 50304 logits:
+// 4.9 + 6.3 + 3.6 us, each a launch and its chain of loads. Joining the pick to the second pass (the sequence's last workgroup,
+// told by a counter) costs more than the launch it saves: a fence for the whole device writes each XCD's L2 back (the two
+// together 219 instead of 28 us for 64 sequences, 12.3 instead of 10.3 for one).
 #include <float.h>
 
 #include "common.h"
@@ -30,6 +36,7 @@ constexpr int kChunk = 8192;  // logits per workgroup of the first pass: 32 per 
 template <typename E>
 constexpr int piece() { return 64 * 16 / (int)sizeof(E); }
 constexpr int kPieces = 4;        // pieces per wave of the second pass
+constexpr int kHeld = 16;           // pieces of a row per lane of the draw that are held in registers
 constexpr int kOneRow = 4096, kOneLaunch = 32768;  // logits per row and sequence up to which one launch does everything
 constexpr int kMaxRows = 2 * kVerifyMaxDraft + 1;
 
@@ -174,7 +181,9 @@ __device__ __forceinline__ const E* row_ptr(const Args& a, int b, int r) {
 // whether sequence b's row r is one that none of its drafted tokens needs
 __device__ __forceinline__ bool idle(const Args& a, int r, int nd) { return r <= a.T ? r > nd : r - a.T - 1 >= nd; }
 
-// ---- pass 1: grid (chunks, rows, B); greedy needs the target's T+1 rows only
+// ---- pass 1: grid (chunks, rows, B); greedy needs the target's T+1 rows only. Bound by memory: a chunk is loaded at once, 8
+// (bf16: 4) 16-byte loads a thread, and its exponentials run while other workgroups load. Greedy, 32 x 8 rows of 128256 bf16
+// logits: 12.9 us, 5.1 TB/s.
 template <typename E, bool GREEDY>
 __global__ void __launch_bounds__(kT) verify_stats_kernel(Args a) {
   constexpr int N = Vec<E>::N, NV = kChunk / (kT * N);
@@ -359,7 +368,8 @@ __device__ __forceinline__ void piece_sums(const Args& a, const Rest<E>& f, int 
   }
 }
 
-// ---- pass 2 (not greedy): grid (pieces / (4 kPieces), B)
+// ---- pass 2 (not greedy): grid (pieces / (4 kPieces), B). A piece is what a wave reads at once, so that its sum is one fold of
+// the wave; 4 pieces a wave share one derivation of the acceptance. Bound by the fp64 exponentials (about 0.8 per ps).
 template <typename E>
 __global__ void __launch_bounds__(kT) verify_rest_kernel(Args a) {
   __shared__ float s_m[kMaxRows];
@@ -375,13 +385,13 @@ __global__ void __launch_bounds__(kT) verify_rest_kernel(Args a) {
 // One wave: the smallest of n items whose running sum, from `before` on, passes `want` -- past the last sum (u >= 1, rounding) the
 // last item that is more than 0, -1 if there is none. Lane l owns items l * per .. and gives their values through `at`.
 // `before` becomes the running sum in front of the item.
-template <int PER, typename F>  // PER: items of a lane, 0: as many as n takes
-__device__ __forceinline__ int search(int n, F at, double want, double& before) {
-  const int lane = threadIdx.x & 63, per = PER > 0 ? PER : (n + 63) / 64;
+template <int PER, typename F>  // PER: `per` is at most that, and the loops over a lane's items are unrolled; 0: any number
+__device__ __forceinline__ int search(int per, int n, F at, double want, double& before) {
+  const int lane = threadIdx.x & 63, lim = PER > 0 ? PER : per;
+  auto item = [&](int k) { return k < per && lane * per + k < n ? at(lane * per + k, k) : 0.0; };
   double mine = 0.0;
 #pragma unroll
-  for (int k = 0; k < per; ++k)
-    if (lane * per + k < n) mine += at(lane * per + k, k);
+  for (int k = 0; k < lim; ++k) mine += item(k);
   const double inc = before + wave_scan_d(mine);
   const uint64_t over = __ballot(mine > 0.0 && inc > want), some = __ballot(mine > 0.0);
   if (!some) {
@@ -393,8 +403,8 @@ __device__ __forceinline__ int search(int n, F at, double want, double& before) 
   int found = -1;
   bool hit = false;
 #pragma unroll
-  for (int k = 0; k < per; ++k) {
-    const double v = lane * per + k < n ? at(lane * per + k, k) : 0.0;
+  for (int k = 0; k < lim; ++k) {
+    const double v = item(k);
     const bool take = v > 0.0 && !hit;
     found = take ? lane * per + k : found;
     front = take ? run : front;
@@ -411,14 +421,22 @@ __device__ int64_t draw(const Args& a, int b, const Head& h, const double* pr) {
   constexpr int N = Vec<E>::N;
   Rest<E> f(a, b, h);
   double total = 0.0;
-  const int lane = threadIdx.x & 63;
-  for (int i = lane; i < a.npc; i += 64) total += pr[i];
-  total = wave_sum_d(total);
+  const int lane = threadIdx.x & 63, per = (a.npc + 63) / 64;
   const double u = (double)a.u[(int64_t)b * (a.T + 1) + a.T];
+  // up to kHeld sums a lane (rows of 262144 fp32 logits) in registers, loaded at once: one round trip to memory and not one a sum
+  double held[kHeld];
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) held[k] = per <= kHeld && k < per && lane * per + k < a.npc ? pr[lane * per + k] : 0.0;
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) total += held[k];
+  if (per > kHeld)
+    for (int i = lane; i < a.npc; i += 64) total += pr[i];
+  total = wave_sum_d(total);
   double before = 0.0;
   int first, last;
   if (total > 0.0) {
-    first = search<0>(a.npc, [&](int i, int) { return pr[i]; }, u * total, before);
+    if (per <= kHeld) first = search<kHeld>(per, a.npc, [&](int, int k) { return held[k]; }, u * total, before);
+    else first = search<0>(per, a.npc, [&](int i, int) { return pr[i]; }, u * total, before);
     last = first + 1;
   } else {  // r = 0 everywhere: the target's own distribution, whose total is 1, from the first piece on
     if (!(h.ip > 0.0)) return -1;
@@ -435,12 +453,7 @@ __device__ int64_t draw(const Args& a, int b, const Head& h, const double* pr) {
 #pragma unroll
     for (int e = 0; e < N; ++e) sum += v[e];
     sum = wave_sum_d(sum);
-    const int i = search<N>(piece<E>(), [&](int, int k) {
-      double w = v[0];
-#pragma unroll
-      for (int e = 1; e < N; ++e) w = k == e ? v[e] : w;
-      return w;
-    }, want, front);
+    const int i = search<N>(N, piece<E>(), [&](int, int k) { return v[k]; }, want, front);
     if (i >= 0) token = pc * piece<E>() + i;
     before += sum;
     if (before > want && token >= 0) break;
@@ -455,7 +468,7 @@ __device__ __forceinline__ void put(const Args& a, int b, int j, int64_t next) {
   if (lane == 0) a.accepted[b] = j;
 }
 
-// ---- pass 3: grid B; one wave (greedy: one workgroup)
+// ---- pass 3: grid B; one wave (greedy: one workgroup). Bound by its chain of loads: head, sums, the piece's logits.
 template <typename E>
 __global__ void __launch_bounds__(64) verify_draw_kernel(Args a) {
   const int b = blockIdx.x;
