@@ -613,6 +613,7 @@ Tensor prefix_attn(const Tensor& q, const Tensor& k_prefix, const Tensor& v_pref
   }
   const int64_t P = k_prefix.size(1);
   TORCH_CHECK(D == 64 || D == 128, "prefix_attention: head dim must be 64 or 128");
+  TORCH_CHECK(Hkv >= 1, "prefix_attention: the cache has no heads");
   TORCH_CHECK(tokens >= 1 && q.size(0) == B * tokens && lens.numel() == B,
               "prefix_attention: q must have B * tokens rows and lens B entries");
   TORCH_CHECK(q.size(1) % D == 0 && q.size(1) > 0 && (q.size(1) / D) % Hkv == 0,
@@ -774,6 +775,7 @@ std::vector<Tensor> distill_topk(const Tensor& logits, const Tensor& index, cons
     out = *out_;
     check_bf16(out, "out");
     check_same_device(out, logits, "out");
+    check_no_grad(out, "distill_topk");
     TORCH_CHECK(out.sizes() == logits.sizes() && (out.stride(1) == 1 || V == 1) && (out.stride(0) >= V || N <= 1),
                 "out must have logits' shape, contiguous rows and no overlap");
     if (!(out.data_ptr() == logits.data_ptr() && out.strides() == logits.strides()))

@@ -128,6 +128,7 @@ def prefix_attention_ref(q, k_prefix, v_prefix, k_cache, v_cache, lens, max_len,
         require(t.dim() == 3 and t.shape == (Hkv, k_prefix.shape[1], D),
                 "prefix must be [Hkv, P, D] with the cache's heads and head dim, K and V alike")
     require(D in (64, 128), "prefix_attention: head dim must be 64 or 128")
+    require(Hkv >= 1, "prefix_attention: the cache has no heads")
     require(q.dim() == 2 and tokens >= 1 and q.shape[0] == B * tokens and lens.numel() == B,
             "prefix_attention: q must have B * tokens rows and lens B entries")
     require(lens.dtype == torch.int32, "lens must be contiguous int32")

@@ -234,6 +234,14 @@ def test_refusals(dev):
     assert f(q[:0], kp, vp, kc[:0], vc[:0], lens[:0], 32).shape == (0, Hq * D)
 
 
+@pytest.mark.parametrize("dev", DEVS)
+def test_a_cache_without_heads_is_refused(dev):
+    q = torch.zeros(2, 64, dtype=torch.bfloat16, device=dev)
+    kv, cache = torch.zeros(0, 5, 64, dtype=torch.bfloat16, device=dev), torch.zeros(2, 0, 8, 64, dtype=torch.bfloat16, device=dev)
+    with pytest.raises(RuntimeError, match="no heads"):
+        kf.prefix_attention(q, kv, kv, cache, cache, torch.zeros(2, dtype=torch.int32, device=dev), 8)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("B,T,P", [(4, 1, 500), (48, 4, 700)])
 def test_captured_call_replays_and_another_stream(B, T, P):
