@@ -1007,7 +1007,10 @@ def distill_topk(logits, index, teacher, temperature: float = 1.0, weight=None, 
     outside [0, V) or a teacher logit of -inf / NaN is padding. With p = softmax(teacher / t) over the listed tokens
     and q = softmax(logits / t) over the vocabulary: loss[i] = t^2 w_i sum_k p_k (log p_k - log q_k), and the second
     result is d loss[i] / d logits (``out``: written there, ``logits`` itself for in place). ``weight`` [N] fp32 (default
-    1); rows of weight 0 or of padding only give 0. A token listed twice counts with the sum of its probabilities."""
+    1); rows of weight 0 or of padding only give 0. A token listed twice counts with the sum of its probabilities. The
+    teacher and the weights are constants: they have no gradient."""
+    ref.require(not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (teacher, weight, out))),
+                "distill_topk has no gradient of the teacher or the weights: detach them")
     if not logits.is_cuda:
         return ref.distill_topk_ref(logits, index, teacher, float(temperature), weight, out)
     return tuple(_lib().distill_topk(logits, index, teacher, float(temperature), weight, out))
@@ -1044,7 +1047,10 @@ class _DistillCPU(Function):
 def distill_topk_lmhead(x, w, index, teacher, temperature: float = 1.0, weight=None):
     """Distillation loss of softmax(x @ w^T) against a teacher's top logits (``distill_topk``), summed with ``weight``
     [N] (default 1 / N: the mean). The logits buffer is overwritten by its own gradient, as in
-    ``cross_entropy_lmhead``; index and teacher are [N, K] over the flattened rows of x."""
+    ``cross_entropy_lmhead``; index and teacher are [N, K] over the flattened rows of x. Gradients of x and w; the teacher
+    and the weights are constants."""
+    ref.require(not (torch.is_grad_enabled() and (teacher.requires_grad or (weight is not None and weight.requires_grad))),
+                "distill_topk_lmhead has no gradient of the teacher or the weights: detach them")
     if weight is None:
         n = x.numel() // x.shape[-1]
         weight = torch.full((n,), 1.0 / max(n, 1), dtype=torch.float32, device=x.device)

@@ -165,6 +165,21 @@ def test_refusals(dev):
 
 
 @pytest.mark.parametrize("dev", DEVS)
+def test_teacher_and_weights_have_no_gradient(dev):
+    logits, index, teacher, weight = make(4, 64, 6, dev)
+    x, w = logits.clone(), torch.zeros(64, 64, dtype=torch.bfloat16, device=dev)
+    for f in (lambda t, v: kf.distill_topk(logits, index, t, 1.0, v),
+              lambda t, v: kf.distill_topk_lmhead(x, w, index, t, 1.0, v)):
+        for t, v in ((teacher.clone().requires_grad_(), weight), (teacher, weight.clone().requires_grad_())):
+            with pytest.raises(RuntimeError, match="detach"):
+                f(t, v)
+            with torch.no_grad():
+                f(t, v)
+    with pytest.raises(RuntimeError):
+        kf.distill_topk(logits, index, teacher, 1.0, weight, out=logits.clone().requires_grad_())
+
+
+@pytest.mark.parametrize("dev", DEVS)
 def test_lmhead_gradients(dev):
     """x and w gradients through the LM head against the 64-bit gradient of the logits that the product gives, and an
     upstream factor; grad_fn of the same leaves may be used for several calls."""
