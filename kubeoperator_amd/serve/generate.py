@@ -427,6 +427,8 @@ class LlamaGenerator:
         B, S = ids.shape
         if draft.cfg.vocab_size != self.cfg.vocab_size or not 1 <= drafts <= 32 or max_new_tokens < 1:
             raise ValueError("the draft needs this model's vocabulary; 1 to 32 drafts per round")
+        if draft is self:
+            raise ValueError("the draft needs a generator (a cache) of its own")
         if draft.prefix_len != self.prefix_len:
             raise ValueError("give the draft the same prefix")
         for g in (self, draft):  # the last round may start one token before the end and brings drafts + 1
@@ -440,23 +442,29 @@ class LlamaGenerator:
             none = torch.empty(B, 0, dtype=torch.long, device=self.device)
             return kf.verify_draft(logits.unsqueeze(1), None, none, uniform(B, 1), temperature)[0][:, 0]
 
+        def checked(tokens: list):
+            if min(tokens) < 0:
+                raise RuntimeError("a row of the model's logits gives no token any probability")
+            return tokens
+
         cur = sample(self.prefill(ids))
         draft.prefill(ids)
-        out = [[int(t)] for t in cur.tolist()]
+        out = [[t] for t in checked(cur.tolist())]
         rounds = []
         while min(len(o) for o in out) < max_new_tokens:
             start = list(self.cache.host_lens[:B])
             tok, toks, qs = cur, [], []
             for _ in range(drafts):
                 q = draft.decode(tok)
-                tok = sample(q)
-                toks.append(tok)
+                toks.append(sample(q))  # -1 (no token has any probability) is refused below
+                tok = toks[-1].clamp(min=0)
                 qs.append(q)
             draft.decode(tok)  # the last one's keys: all of them may be kept
             proposed = torch.stack(toks, 1)
-            p = self.extend(torch.cat([cur.unsqueeze(1), proposed], 1))
+            p = self.extend(torch.cat([cur.unsqueeze(1), proposed.clamp(min=0)], 1))
             new, kept = kf.verify_draft(p, torch.stack(qs, 1), proposed, uniform(B, drafts + 1), temperature)
             cur = new.gather(1, kept.long().unsqueeze(1)).squeeze(1)
+            checked(cur.tolist())
             new, kept = new.tolist(), kept.tolist()
             rounds.append(kept)
             for b in range(B):

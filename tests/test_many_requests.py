@@ -182,6 +182,25 @@ def test_speculative_sampling_with_itself_keeps_nearly_everything(dev):
 
 
 @pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("temperature", [0.0, 0.8])
+def test_speculation_with_broken_logits(dev, temperature):
+    """A draft whose logits are all NaN proposes nothing that is kept (and no token outside the vocabulary reaches a model); a
+    target like that is an error, as is a draft that shares the target's cache."""
+    m, bad = model(dev), model(dev)
+    with torch.no_grad():
+        bad.final_norm.fill_(float("nan"))
+    ids = ids_of(m, 2, 10)
+    gen, broken = (LlamaGenerator(x, max_batch=2, max_seq=32) for x in (m, bad))
+    out, rounds = gen.speculate(broken, ids, 6, drafts=3, temperature=temperature)
+    assert out.shape == (2, 16) and rounds == [[0, 0]] * 5
+    assert ((out >= 0) & (out < m.cfg.vocab_size)).all()
+    with pytest.raises(RuntimeError, match="probability"):
+        broken.speculate(gen, ids, 6, drafts=3, temperature=temperature)
+    with pytest.raises(ValueError, match="of its own"):
+        gen.speculate(gen, ids, 6)
+
+
+@pytest.mark.parametrize("dev", DEVS)
 def test_draft_training_gradients(dev):
     """Llama.distill against the logits' formula: the gradient of every parameter against differences of the loss along a
     direction (fp32 master copy, so the differences are those of the same network)."""
