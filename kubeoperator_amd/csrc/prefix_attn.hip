@@ -100,12 +100,13 @@ struct Work {
   int kvh, row0, nrow;   // rows [row0, row0 + nrow) of this KV head
   int slot;              // where its partial goes
   int k0, kend, nkeys;   // keys [k0, kend); no key at or past nkeys is read
-  int lim0;              // own keys: what token 0 of the sequence sees; prefix: nkeys
+  int seen0;             // own keys: what token 0 of the sequence sees (0 or less: nothing)
+  int lim0;              // keys that every row of the tile sees
   bool own;
   const bf16_t *k, *v;
   int ks, vs;            // elements between keys (up to 2^23)
 };
-__device__ __forceinline__ int seen_by(const Args& p, const Work& w, int bt) { return w.own ? w.lim0 + bt % p.T : w.nkeys; }
+__device__ __forceinline__ int seen_by(const Args& p, const Work& w, int bt) { return w.own ? w.seen0 + bt % p.T : w.nkeys; }
 
 // a row's Q^T operand: dims 32 s + 8 g .. + 7 (a negative scale is taken into Q's signs, so that maxima can be taken
 // before scaling)
@@ -672,8 +673,9 @@ __global__ void __launch_bounds__(kThreads, OM == kByRows && D == 128 ? 1 : 2) p
     w.slot = p.np + split;
     w.k0 = split * p.ochunk;
     w.nkeys = min(max(p.lens[b], 0), p.max_len);
-    w.lim0 = w.nkeys - p.T + 1;
-    w.kend = min(w.lim0 + (first + w.nrow - 1) / p.G, w.k0 + p.ochunk);  // up to what the tile's last token sees
+    w.seen0 = w.nkeys - p.T + 1;
+    w.lim0 = w.seen0 + first / p.G;
+    w.kend = min(w.seen0 + (first + w.nrow - 1) / p.G, w.k0 + p.ochunk);  // up to what the tile's last token sees
     w.k = p.kc + ((int64_t)b * p.Hkv + w.kvh) * p.Smax * D;
     w.v = p.vc + ((int64_t)b * p.Hkv + w.kvh) * p.Smax * D;
     w.ks = w.vs = D;
@@ -707,8 +709,9 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attn_short_kernel(Args p) 
       w.vs = (int)p.vps;
     } else {
       w.nkeys = min(max(p.lens[b], 0), p.max_len);
-      w.lim0 = w.nkeys - p.T + 1;
-      w.kend = w.lim0 + (first + w.nrow - 1) / p.G;
+      w.seen0 = w.nkeys - p.T + 1;
+      w.lim0 = w.seen0 + first / p.G;
+      w.kend = w.seen0 + (first + w.nrow - 1) / p.G;
       w.k = p.kc + ((int64_t)b * p.Hkv + w.kvh) * p.Smax * D;
       w.v = p.vc + ((int64_t)b * p.Hkv + w.kvh) * p.Smax * D;
       w.ks = w.vs = D;
