@@ -7,15 +7,23 @@
 // One softmax over both. The rows of ALL sequences meet the prefix together (B T G rows per KV head, G = Hq / Hkv), so its
 // keys leave HBM once per row tile instead of once per sequence, and its products have enough rows for the matrix cores.
 //
-// Pass 1, one launch: a workgroup takes (row tile, key range) of the prefix or of one sequence; its 4 waves take every
-// fourth 32-key block. S^T [keys x rows] = K . Q^T and O^T [dims x rows] += V^T . P^T on v_mfma_f32_16x16x32_bf16:
-//   * the 16 key rows of product b are keys 8 (i >> 2) + 4 b + (i & 3), so that a lane's scores of the two products are
-//     its own P^T operand (keys 8 g .. 8 g + 7 of its row), with no lane exchange;
-//   * V goes through an LDS image filled by LDS-DMA (source chunks XOR-permuted by the row) and is read transposed;
-//   * running maximum and sum per row (fp32), P rounded to bf16 for the matrix cores: 2^-9 relative per key.
-// The next block's K (registers) and V (second LDS image) are in flight while a block is computed; the waves' results
-// meet in LDS, and one fp32 partial (O, max, sum) per row and range goes out.
-// Pass 2: one wave per (row, head) folds the ranges' partials.
+// S^T [keys x rows] = K . Q^T and O^T [dims x rows] += V^T . P^T on v_mfma_f32_16x16x32_bf16, with running maximum and sum
+// per row (fp32), P rounded to bf16 for the matrix cores (half a step: 2^-9 relative per key). The 16 key rows of product b are keys
+// 8 (i >> 2) + 4 b + (i & 3), so that a lane's scores of two products are its own P^T operand (keys 8 g .. 8 g + 7 of its row),
+// with no lane exchange; V goes through an LDS image whose 16-byte chunks are XOR-permuted by the row, and is read transposed.
+// A workgroup works in one of two ways:
+//   * by keys (up to 32 rows): its 4 waves take every fourth 32-key block of all its rows. K goes straight to registers, V through
+//     LDS-DMA; both of the next block are in flight while a block is computed; the waves' results meet in LDS. Bound by memory.
+//   * by rows (128 rows): each wave has 32 rows of its own, and K and V of every 64-key tile come from LDS, where the four share
+//     them. The next tile's scores (matrix cores) run beside this tile's weights (vector ALUs). Bound by those two.
+// and a launch takes one of three forms (make_plan):
+//   * split: workgroups of (row tile, key range) of the prefix, and of one sequence's own keys, write fp32 partials (O, max, sum);
+//     a second launch folds them. Decode (64 sequences, 32/8 heads of 128, 2048 + 500 keys): 23 + 5 us, 3.5 TB/s. Drafts (64 x 5
+//     tokens, 8192 + 1000 keys, prefix by rows): 86 + 7 us; the prefix alone 69, 630 TFLOP/s.
+//   * short contexts, by keys: a workgroup takes prefix and own keys of its rows, one launch, no partials. 4 sequences, 500 + 60
+//     keys: 7.4 us against 10.0 split.
+//   * prompts, by rows: the same for sequences with many tokens. 8 x 1024 tokens behind 2048, 32/8 heads of 128: 448 us, 770
+//     TFLOP/s; one prompt of 4096, no prefix: 175 us, 780 TFLOP/s.
 //
 // A masked key has weight zero exactly: masked scores never enter the maximum or the sum, keys past the last valid one are
 // never read (loads are clamped to it), and in the blocks where some rows see a key and others do not, values that are
@@ -415,21 +423,29 @@ __device__ __forceinline__ void by_keys(const Args& p, F part, char* smem) {
 
 // ---- many rows: each wave takes 32 rows of its own, all 4 take every 64-key tile from LDS (K and V images, two of each:
 // the next tile travels through registers while one is computed)
-template <int D, bool OWN>  // OWN: the keys may be a sequence's own (rows see different numbers of them)
-__device__ __forceinline__ void by_rows(const Args& p, const Work& w, char* smem) {
+// WHOLE: one sequence's rows over its own keys and then over the prefix, no partials; else a range of the prefix
+template <int D, bool WHOLE, typename F>
+__device__ __forceinline__ void by_rows(const Args& p, F part, char* smem) {
   constexpr int ROWB = D * 2, NS = D / 32, NC = D / 16, TK = 64, IMG = TK * ROWB, SLOTS = ROWB / 16, NT = 2;
   constexpr int PER = TK * SLOTS / kThreads;  // 16-byte pieces per thread and image
   static_assert(4 * IMG <= kLds, "LDS");
   const int t = threadIdx.x, lane = t & 63, col = lane & 15, g = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(t >> 6);
-  const bool live = 32 * wv < w.nrow;
+  const Work w0 = part(0);
+  const bool live = 32 * wv < w0.nrow;
   bf16x8 qf[NT][NS];
-  int lim[NT];
+  // the rows' tokens and outputs, kept in LDS: over the loops there is no register to spare for them, of either kind
+  __shared__ int s_bt[kThreads / 64 * 32];
+  __shared__ bf16_t* s_op[WHOLE ? kThreads / 64 * 32 : 1];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const int i = 32 * wv + 16 * n + col, r = w.row0 + (i < w.nrow ? i : 0);
-    load_q<D>(p, w, r, g, qf[n]);
-    lim[n] = seen_by(p, w, r / p.G);
+    const int i = 32 * wv + 16 * n + col, r = w0.row0 + (i < w0.nrow ? i : 0);
+    load_q<D>(p, w0, r, g, qf[n]);
+    const int bt = r / p.G;
+    s_bt[32 * wv + 16 * n + col] = bt;  // the same from all four lanes of a row; read by this wave alone
+    if constexpr (WHOLE)
+      s_op[32 * wv + 16 * n + col] =
+          i >= w0.nrow ? nullptr : p.o + (int64_t)bt * p.os + (int64_t)(w0.kvh * p.G + r % p.G) * D;
   }
   // K image: chunk slots XORed with the row's number in a 16-row operand (8 a + 4 b + q -> 4 a + q), so that its 16 rows'
   // reads of one chunk fall on different banks; V image as in by_keys
@@ -446,181 +462,210 @@ __device__ __forceinline__ void by_rows(const Args& p, const Work& w, char* smem
 #pragma unroll
     for (int c = 0; c <= NC; ++c) acc[n][c] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  // a thread's pieces are rows t / SLOTS + i * RSTEP of the tile, all at chunk t % SLOTS
-  constexpr int RSTEP = kThreads / SLOTS;
-  const int tr = t / SLOTS, ch = t % SLOTS;
-  const uint32_t ko = (uint32_t)(tr * w.ks + 8 * ch) * 2, vo = (uint32_t)(tr * w.vs + 8 * ch) * 2;
-  auto fetch = [&](const bf16_t* src, int64_t stride, uint32_t off, int kb, u32x4* to) {
-    const char* base = reinterpret_cast<const char*>(src + kb * stride);
-    if (kb + TK <= w.nkeys) {
+  auto barrier = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+#pragma unroll 1
+  for (int seg = 0; seg < (WHOLE ? 2 : 1); ++seg) {
+    const Work w = WHOLE ? part(seg) : w0;
+    if (WHOLE && w.k0 >= w.kend) continue;
+    if (seg > 0) barrier();  // the images are free
+    int lim[NT];
 #pragma unroll
-      for (int i = 0; i < PER; ++i) to[i] = *reinterpret_cast<const u32x4*>(base + 2 * RSTEP * i * stride + off);
-    } else {  // rows past the last key: the last key's
+    for (int n = 0; n < NT; ++n) lim[n] = seen_by(p, w, s_bt[32 * wv + 16 * n + col]);
+    // a thread's pieces are rows t / SLOTS + i * RSTEP of the tile, all at chunk t % SLOTS
+    constexpr int RSTEP = kThreads / SLOTS;
+    const int tr = t / SLOTS, ch = t % SLOTS;
+    const uint32_t ko = (uint32_t)(tr * w.ks + 8 * ch) * 2, vo = (uint32_t)(tr * w.vs + 8 * ch) * 2;
+    auto fetch = [&](const bf16_t* src, int step, uint32_t off, int kb, u32x4* to) {
+      if constexpr (WHOLE) asm volatile("" : "+s"(step));  // its multiples are made here, not held over the loop: scalar registers
+      const int64_t stride = step;
+      const char* base = reinterpret_cast<const char*>(src + kb * stride);
+      if (kb + TK <= w.nkeys) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i)
-        to[i] = *reinterpret_cast<const u32x4*>(
-            base + (uint32_t)(min(tr + RSTEP * i, w.nkeys - 1 - kb) * (int)stride + 8 * ch) * 2);
-    }
-  };
-  // where they go in the images: RSTEP rows on, the K swizzle has one of two forms and the V swizzle stays
-  static_assert(RSTEP == 16 || RSTEP == 32, "rows between a thread's pieces");
-  int kw[2];
+        for (int i = 0; i < PER; ++i) to[i] = *reinterpret_cast<const u32x4*>(base + 2 * RSTEP * i * stride + off);
+      } else {  // rows past the last key: the last key's
 #pragma unroll
-  for (int h = 0; h < 2; ++h) kw[h] = tr * ROWB + 16 * (ch ^ kx(tr + RSTEP * h));
-  const int vw = tr * ROWB + 16 * (ch ^ vx<ROWB>(tr));
-  char* const kimg = smem;            // two K images, two V images
-  char* const vimg = smem + 2 * IMG;
-  auto put_k = [&](const u32x4* from, int buf) {
+        for (int i = 0; i < PER; ++i)
+          to[i] = *reinterpret_cast<const u32x4*>(
+              base + (uint32_t)(min(tr + RSTEP * i, w.nkeys - 1 - kb) * (int)stride + 8 * ch) * 2);
+      }
+    };
+    // where they go in the images: RSTEP rows on, the K swizzle has one of two forms and the V swizzle stays
+    static_assert(RSTEP == 16 || RSTEP == 32, "rows between a thread's pieces");
+    int kw[2];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) *reinterpret_cast<u32x4*>(kimg + buf * IMG + kw[i & 1] + i * RSTEP * ROWB) = from[i];
-  };
-  auto put_v = [&](const u32x4* from, int buf) {
+    for (int h = 0; h < 2; ++h) kw[h] = tr * ROWB + 16 * (ch ^ kx(tr + RSTEP * h));
+    const int vw = tr * ROWB + 16 * (ch ^ vx<ROWB>(tr));
+    char* const kimg = smem;            // two K images, two V images
+    char* const vimg = smem + 2 * IMG;
+    auto put_k = [&](const u32x4* from, int buf) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) *reinterpret_cast<u32x4*>(vimg + buf * IMG + vw + i * RSTEP * ROWB) = from[i];
-  };
-  f32x4 sc[NT][4];
-  // a product's addresses, settled before its stretch of code is put in order (address arithmetic would count as work to place)
-  auto k_at = [&](int buf, uint32_t* at) {
+      for (int i = 0; i < PER; ++i) *reinterpret_cast<u32x4*>(kimg + buf * IMG + kw[i & 1] + i * RSTEP * ROWB) = from[i];
+    };
+    auto put_v = [&](const u32x4* from, int buf) {
 #pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      at[s] = (uint32_t)((buf * IMG + ka) ^ (64 * s));
-      asm volatile("" : "+v"(at[s]));
-    }
-  };
-  auto v_at = [&](int buf, uint32_t* at) {
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      at[c] = (uint32_t)((buf * IMG + va) ^ (32 * c));
-      asm volatile("" : "+v"(at[c]));
-    }
-  };
-  auto scores = [&](const uint32_t* at, f32x4 (*s4)[4]) {
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n) s4[n][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < PER; ++i) *reinterpret_cast<u32x4*>(vimg + buf * IMG + vw + i * RSTEP * ROWB) = from[i];
+    };
+    f32x4 sc[NT][4];
+    // a product's addresses, settled before its stretch of code is put in order (address arithmetic would count as work to place)
+    auto k_at = [&](int buf, uint32_t* at) {
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
-        const bf16x8 kf = lds_read8(kimg + at[s] + (32 * (b >> 1) + 4 * (b & 1)) * ROWB);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) s4[n][b] = mfma16(kf, qf[n][s], s4[n][b]);
+        at[s] = (uint32_t)((buf * IMG + ka) ^ (64 * s));
+        asm volatile("" : "+v"(at[s]));
       }
-    }
-  };
-  // One tile: its scores are there. The next tile's scores (matrix cores) are computed beside this one's weights (vector ALUs).
-  auto tile = [&](auto edge_, auto next_, int kb, int buf) {
-    constexpr bool EDGE = decltype(edge_)::value, NEXT = decltype(next_)::value, SIFT = EDGE && OWN;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) raise_max<EDGE, 2, NC>(sc[n], lim[n] - kb - 8 * g, p.sl2, m[n], acc[n]);
-    bf16x8 pf[NT][2];
-    f32x4 nx[NT][4];
-    uint32_t kat[NS], vat[NC];
-    if constexpr (NEXT) k_at(buf ^ 1, kat);
-    __builtin_amdgcn_sched_barrier(0);
-    if constexpr (NEXT) scores(kat, nx);
-#pragma unroll
-    for (int n = 0; n < NT; ++n) weights<EDGE, 2>(sc[n], lim[n] - kb - 8 * g, p.sl2, m[n], pf[n]);
-    if constexpr (NEXT && !EDGE) {
-      // issue order: operands of one 16-key product ahead, and between two matrix instructions what one of them leaves time for
-      __builtin_amdgcn_sched_group_barrier(kDsRead, NS, 0);
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        if (b < 3) __builtin_amdgcn_sched_group_barrier(kDsRead, NS, 0);
-#pragma unroll
-        for (int i = 0; i < NS * NT; ++i) {
-          __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(kTrans, 8 / (NS * NT), 0);
-        }
-      }
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    v_at(buf, vat);
-#pragma unroll
-    for (int n = 0; n < NT; ++n) acc[n][NC] = sum_p(pf[n][1], sum_p(pf[n][0], acc[n][NC]));
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
+    };
+    auto v_at = [&](int buf, uint32_t* at) {
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        const char* vp = vimg + vat[c] + 32 * b * ROWB;
-        const bf16x8 vf = cat44(lds_tr_read(vp), lds_tr_read(vp + 4 * ROWB));
-        if constexpr (SIFT) {
-          bf16x8 pfn[NT];
-          f32x4 an[NT];
-          int left[NT];
+        at[c] = (uint32_t)((buf * IMG + va) ^ (32 * c));
+        asm volatile("" : "+v"(at[c]));
+      }
+    };
+    auto scores = [&](const uint32_t* at, f32x4 (*s4)[4]) {
 #pragma unroll
-          for (int n = 0; n < NT; ++n) pfn[n] = pf[n][b], an[n] = acc[n][c], left[n] = lim[n] - kb - 8 * g - 32 * b;
-          if (!edge_pv<NT>(vf, pfn, left, an)) {
+      for (int b = 0; b < 4; ++b) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n) an[n] = mfma16(vf, pfn[n], an[n]);
-          }
+        for (int n = 0; n < NT; ++n) s4[n][b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int n = 0; n < NT; ++n) acc[n][c] = an[n];
-          __builtin_amdgcn_sched_barrier(0);
-        } else {
+        for (int s = 0; s < NS; ++s) {
+          const bf16x8 kf = lds_read8(kimg + at[s] + (32 * (b >> 1) + 4 * (b & 1)) * ROWB);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) acc[n][c] = mfma16(vf, pf[n][b], acc[n][c]);
+          for (int n = 0; n < NT; ++n) s4[n][b] = mfma16(kf, qf[n][s], s4[n][b]);
         }
       }
-    if constexpr (!SIFT) {  // issue order: three 16-dim blocks' operands ahead
-      __builtin_amdgcn_sched_group_barrier(kDsRead, 6, 0);
+    };
+    // One tile: its scores are there. The next tile's scores (matrix cores) are computed beside this one's weights (vector ALUs), on
+    // an edge afterwards (both at once and the sifting take more registers than two waves per SIMD have).
+    auto tile = [&](auto edge_, auto next_, int kb, int buf) {
+      constexpr bool EDGE = decltype(edge_)::value, NEXT = decltype(next_)::value, SIFT = EDGE && WHOLE;
 #pragma unroll
-      for (int i = 0; i < 2 * NC - 3; ++i) {
-        __builtin_amdgcn_sched_group_barrier(kMfma, NT, 0);
-        __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 0);
+      for (int n = 0; n < NT; ++n) raise_max<EDGE, 2, NC>(sc[n], lim[n] - kb - 8 * g, p.sl2, m[n], acc[n]);
+      bf16x8 pf[NT][2];
+      f32x4 nx[NT][4];
+      uint32_t kat[NS], vat[NC];
+      if constexpr (NEXT && !EDGE) k_at(buf ^ 1, kat);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (NEXT && !EDGE) scores(kat, nx);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) weights<EDGE, 2>(sc[n], lim[n] - kb - 8 * g, p.sl2, m[n], pf[n]);
+      if constexpr (NEXT && !EDGE) {
+        // issue order: operands of one 16-key product ahead, and between two matrix instructions what one of them leaves time for
+        __builtin_amdgcn_sched_group_barrier(kDsRead, NS, 0);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          if (b < 3) __builtin_amdgcn_sched_group_barrier(kDsRead, NS, 0);
+#pragma unroll
+          for (int i = 0; i < NS * NT; ++i) {
+            __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(kTrans, 8 / (NS * NT), 0);
+          }
+        }
       }
-      __builtin_amdgcn_sched_group_barrier(kMfma, 3 * NT, 0);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    if constexpr (NEXT) {
+      __builtin_amdgcn_sched_barrier(0);
+      v_at(buf, vat);
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n) acc[n][NC] = sum_p(pf[n][1], sum_p(pf[n][0], acc[n][NC]));
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int b = 0; b < 4; ++b) sc[n][b] = nx[n][b];
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const char* vp = vimg + vat[c] + 32 * b * ROWB;
+          const bf16x8 vf = cat44(lds_tr_read(vp), lds_tr_read(vp + 4 * ROWB));
+          if constexpr (SIFT) {
+            bf16x8 pfn[NT];
+            f32x4 an[NT];
+            int left[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) pfn[n] = pf[n][b], an[n] = acc[n][c], left[n] = lim[n] - kb - 8 * g - 32 * b;
+            if (!edge_pv<NT>(vf, pfn, left, an)) {
+#pragma unroll
+              for (int n = 0; n < NT; ++n) an[n] = mfma16(vf, pfn[n], an[n]);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[n][c] = an[n];
+            __builtin_amdgcn_sched_barrier(0);
+          } else {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[n][c] = mfma16(vf, pf[n][b], acc[n][c]);
+          }
+        }
+      if constexpr (!SIFT) {  // issue order: three 16-dim blocks' operands ahead
+        __builtin_amdgcn_sched_group_barrier(kDsRead, 6, 0);
+#pragma unroll
+        for (int i = 0; i < 2 * NC - 3; ++i) {
+          __builtin_amdgcn_sched_group_barrier(kMfma, NT, 0);
+          __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(kMfma, 3 * NT, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (NEXT && EDGE) {
+        k_at(buf ^ 1, kat);
+        scores(kat, sc);
+        __builtin_amdgcn_sched_barrier(0);
+      } else if constexpr (NEXT) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int b = 0; b < 4; ++b) sc[n][b] = nx[n][b];
+      }
+    };
+    // Tile i reads V image i and K image i + 1 (both modulo 2); meanwhile V i + 1 and K i + 2 go from registers into the images
+    // that tile i - 1 has left, and V i + 2 and K i + 3 into the registers.
+    u32x4 kr[PER], vr[PER];
+    int kb = w.k0, buf = 0;
+    fetch(w.k, w.ks, ko, kb, kr);
+    fetch(w.v, w.vs, vo, kb, vr);
+    put_k(kr, 0);
+    put_v(vr, 0);
+    if (kb + TK < w.kend) {
+      fetch(w.k, w.ks, ko, kb + TK, kr);
+      put_k(kr, 1);
+      fetch(w.v, w.vs, vo, kb + TK, vr);
     }
-  };
-  // Tile i reads V image i and K image i + 1 (both modulo 2); meanwhile V i + 1 and K i + 2 go from registers into the images
-  // that tile i - 1 has left, and V i + 2 and K i + 3 into the registers.
-  u32x4 kr[PER], vr[PER];
-  int kb = w.k0, buf = 0;
-  auto barrier = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
-  fetch(w.k, w.ks, ko, kb, kr);
-  fetch(w.v, w.vs, vo, kb, vr);
-  put_k(kr, 0);
-  put_v(vr, 0);
-  if (kb + TK < w.kend) {
-    fetch(w.k, w.ks, ko, kb + TK, kr);
-    put_k(kr, 1);
-    fetch(w.v, w.vs, vo, kb + TK, vr);
-  }
-  if (kb + 2 * TK < w.kend) fetch(w.k, w.ks, ko, kb + 2 * TK, kr);
-  barrier();
-  uint32_t kat0[NS];
-  k_at(0, kat0);
-  if (live) scores(kat0, sc);
-  auto stage = [&](auto edge_, auto next_) {
-    // every wave is done with the tile before: image `buf` of K (whose scores are taken) and the other one of V are free
+    if (kb + 2 * TK < w.kend) fetch(w.k, w.ks, ko, kb + 2 * TK, kr);
     barrier();
-    if (kb + TK < w.kend) put_v(vr, buf ^ 1);
-    if (kb + 2 * TK < w.kend) {
-      put_k(kr, buf);
-      fetch(w.v, w.vs, vo, kb + 2 * TK, vr);
-    }
-    if (kb + 3 * TK < w.kend) fetch(w.k, w.ks, ko, kb + 3 * TK, kr);
-    if (live) tile(edge_, next_, kb, buf);
-    kb += TK;
-    buf ^= 1;
-  };
-  while (kb + TK < w.kend && kb + TK <= w.lim0) stage(std::false_type{}, std::true_type{});
-  while (kb + TK < w.kend) stage(std::true_type{}, std::true_type{});
-  stage(std::true_type{}, std::false_type{});
+    uint32_t kat0[NS];
+    k_at(0, kat0);
+    if (live) scores(kat0, sc);
+    auto stage = [&](auto edge_, auto next_) {
+      // every wave is done with the tile before: image `buf` of K (whose scores are taken) and the other one of V are free
+      barrier();
+      if (kb + TK < w.kend) put_v(vr, buf ^ 1);
+      if (kb + 2 * TK < w.kend) {
+        put_k(kr, buf);
+        fetch(w.v, w.vs, vo, kb + 2 * TK, vr);
+      }
+      if (kb + 3 * TK < w.kend) fetch(w.k, w.ks, ko, kb + 3 * TK, kr);
+      if (live) tile(edge_, next_, kb, buf);
+      kb += TK;
+      buf ^= 1;
+    };
+    while (kb + TK < w.kend && kb + TK <= w.lim0) stage(std::false_type{}, std::true_type{});
+    while (kb + TK < w.kend) stage(std::true_type{}, std::true_type{});
+    stage(std::true_type{}, std::false_type{});
+  }
   if (!live) return;
+  if constexpr (WHOLE) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      bf16_t* op = s_op[32 * wv + 16 * n + col];
+      if (!op) continue;
+      const float l = acc[n][NC][0], inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        *reinterpret_cast<u32x2*>(op + 4 * g + 16 * c) =
+            u32x2{pack2(acc[n][c][0] * inv, acc[n][c][1] * inv), pack2(acc[n][c][2] * inv, acc[n][c][3] * inv)};
+    }
+    return;
+  }
   const int RR = p.B * p.T * p.G;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int i = 32 * wv + 16 * n + col;
-    if (i >= w.nrow) continue;
-    const int64_t at = ((int64_t)w.kvh * RR + w.row0 + i) * (p.np + p.ns) + w.slot;
+    if (i >= w0.nrow) continue;
+    const int64_t at = ((int64_t)w0.kvh * RR + w0.row0 + i) * (p.np + p.ns) + w0.slot;
 #pragma unroll
     for (int c = 0; c < NC; ++c) *reinterpret_cast<f32x4*>(p.po + at * D + 16 * c + 4 * g) = acc[n][c];
     if (g == 0) {
@@ -631,17 +676,12 @@ __device__ __forceinline__ void by_rows(const Args& p, const Work& w, char* smem
 }
 
 constexpr int tile_rows(int mode) { return mode == kByRows ? 128 : 16 * mode; }
-template <int D, int MODE, bool OWN>
-__device__ __forceinline__ void run_part(const Args& p, const Work& w, char* smem) {
-  if constexpr (MODE == kByRows) by_rows<D, OWN>(p, w, smem);
-  else by_keys<D, MODE, 1>(p, [&](int) { return w; }, smem);
-}
 }  // namespace
 
-// PM / OM: how the prefix's / the own keys' workgroups work (1, 2: by keys, that many 16-row tiles; kByRows)
-// Two workgroups per CU (256 registers); by rows over own keys at D = 128 takes about 30 more, and one.
+// PM / OM: how the prefix's / the own keys' workgroups work (1, 2: by keys, that many 16-row tiles; the prefix's also kByRows).
+// Two workgroups per CU: 256 registers.
 template <int D, int PM, int OM>
-__global__ void __launch_bounds__(kThreads, OM == kByRows && D == 128 ? 1 : 2) prefix_attn_kernel(Args p) {
+__global__ void __launch_bounds__(kThreads, 2) prefix_attn_kernel(Args p) {
   __shared__ __attribute__((aligned(16))) char smem[kLds];
   Work w;
   int id = blockIdx.x;
@@ -681,44 +721,53 @@ __global__ void __launch_bounds__(kThreads, OM == kByRows && D == 128 ? 1 : 2) p
     w.ks = w.vs = D;
   }
   if (w.k0 >= w.kend) return;  // nothing to see: pass 2 does not read this range's partials
-  if (PM == OM || !w.own) run_part<D, PM, PM == OM>(p, w, smem);
-  else run_part<D, OM, true>(p, w, smem);
+  const auto part = [&](int) { return w; };
+  if (PM == OM || w.own) by_keys<D, OM, 1>(p, part, smem);
+  else if constexpr (PM == kByRows) by_rows<D, false>(p, part, smem);
+  else if constexpr (PM != OM) by_keys<D, PM, 1>(p, part, smem);
 }
 
-// Short contexts: a workgroup per (sequence, row tile, KV head) takes the prefix and the own keys by itself, and no partials
-// are written.
+// What workgroup `id` of a launch without partials takes: a (sequence, tile of ROWS rows, KV head), the prefix (seg 0) or the own
+// keys (seg 1). The last tiles, which see the most, come first.
+template <int D, int ROWS>
+__device__ __forceinline__ Work whole_part(const Args& p, int id, int seg) {
+  Work w;
+  w.kvh = id % p.Hkv;
+  id /= p.Hkv;
+  const int b = id % p.B, first = (p.rto - 1 - id / p.B) * ROWS;
+  w.own = seg != 0;
+  w.row0 = b * p.T * p.G + first;
+  w.nrow = min(ROWS, p.T * p.G - first);
+  w.slot = 0;
+  w.k0 = 0;
+  if (seg == 0) {
+    w.nkeys = w.lim0 = w.kend = p.P;
+    w.k = p.kp + w.kvh * p.kph;
+    w.v = p.vp + w.kvh * p.vph;
+    w.ks = (int)p.kps;
+    w.vs = (int)p.vps;
+  } else {
+    w.nkeys = min(max(p.lens[b], 0), p.max_len);
+    w.seen0 = w.nkeys - p.T + 1;
+    w.lim0 = w.seen0 + first / p.G;
+    w.kend = w.seen0 + (first + w.nrow - 1) / p.G;
+    w.k = p.kc + ((int64_t)b * p.Hkv + w.kvh) * p.Smax * D;
+    w.v = p.vc + ((int64_t)b * p.Hkv + w.kvh) * p.Smax * D;
+    w.ks = w.vs = D;
+  }
+  return w;
+}
+// Short contexts: a workgroup takes the prefix and the own keys by itself, and no partials are written.
 template <int D, int NT>
 __global__ void __launch_bounds__(kThreads, 2) prefix_attn_short_kernel(Args p) {
   __shared__ __attribute__((aligned(16))) char smem[kLds];
-  auto part = [&](int seg) {
-    Work w;
-    int id = blockIdx.x;
-    w.kvh = id % p.Hkv;
-    id /= p.Hkv;
-    const int b = id / p.rto, first = (id % p.rto) * 16 * NT;
-    w.own = seg != 0;
-    w.row0 = b * p.T * p.G + first;
-    w.nrow = min(16 * NT, p.T * p.G - first);
-    w.slot = 0;
-    w.k0 = 0;
-    if (seg == 0) {
-      w.nkeys = w.lim0 = w.kend = p.P;
-      w.k = p.kp + w.kvh * p.kph;
-      w.v = p.vp + w.kvh * p.vph;
-      w.ks = (int)p.kps;
-      w.vs = (int)p.vps;
-    } else {
-      w.nkeys = min(max(p.lens[b], 0), p.max_len);
-      w.seen0 = w.nkeys - p.T + 1;
-      w.lim0 = w.seen0 + first / p.G;
-      w.kend = w.seen0 + (first + w.nrow - 1) / p.G;
-      w.k = p.kc + ((int64_t)b * p.Hkv + w.kvh) * p.Smax * D;
-      w.v = p.vc + ((int64_t)b * p.Hkv + w.kvh) * p.Smax * D;
-      w.ks = w.vs = D;
-    }
-    return w;
-  };
-  by_keys<D, NT, 2>(p, part, smem);
+  by_keys<D, NT, 2>(p, [&](int seg) { return whole_part<D, 16 * NT>(p, blockIdx.x, seg); }, smem);
+}
+// Many tokens per sequence (a prompt): the same, by rows.
+template <int D>
+__global__ void __launch_bounds__(kThreads, 2) prefix_attn_long_kernel(Args p) {
+  __shared__ __attribute__((aligned(16))) char smem[kLds];
+  by_rows<D, true>(p, [&](int seg) { return whole_part<D, tile_rows(kByRows)>(p, blockIdx.x, 1 - seg); }, smem);
 }
 
 // one wave per (row, KV head): the ranges that its row sees, then o = sum O 2^(m - M) / sum l 2^(m - M)
@@ -761,14 +810,20 @@ namespace {
 struct Plan {
   int pm, om;               // how each part's workgroups work
   int rtp, rto, np, pchunk, ns, ochunk;
-  bool whole;               // both parts by one workgroup, without partials
+  bool whole;               // both parts by one workgroup, without partials (om: kByRows too)
 };
 inline int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 inline int mode_of(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : kByRows; }
 Plan make_plan(int B, int T, int G, int Hkv, int P, int max_len) {
   Plan q;
   const int64_t rows = (int64_t)B * T * G;
-  q.om = mode_of((int64_t)T * G);
+  // Prompts: sequences whose own rows fill a 128-row tile, with a workgroup for every CU, take both parts by rows in one launch.
+  // Against the split form (64 sequences, 32/8 heads of 128, 2048 + 500 keys): 31 tokens 109 us and 154, 24 tokens 111 and 119, 16
+  // tokens (half a tile) 104 and 86; one sequence of 512 tokens behind 8192 (128 workgroups) 211 and 108.
+  q.whole = (int64_t)T * G >= 96 && (int64_t)B * Hkv * cdiv((int64_t)T * G, tile_rows(kByRows)) >= 256;
+  // Otherwise own keys go by keys, also where 32-row tiles read them more than once: by rows (64 x 16 tokens, 8192 + 1000 keys) 313
+  // us against 230.
+  q.om = q.whole ? kByRows : std::min(2, mode_of((int64_t)T * G));
   q.pm = P > 0 ? mode_of(rows) : q.om;
   q.rtp = P > 0 ? cdiv(rows, tile_rows(q.pm)) : 0;
   q.rto = cdiv((int64_t)T * G, tile_rows(q.om));
@@ -780,17 +835,17 @@ Plan make_plan(int B, int T, int G, int Hkv, int P, int max_len) {
     chunk = cdiv(cdiv(keys, n), 128) * 128;
     return cdiv(keys, chunk);
   };
-  // At most 8 steps of 128 keys per wave, and a prefix that it does not hurt to read once per sequence: one step long, or at most
+  // Short contexts: at most 8 steps of 128 keys per wave, and a prefix that it does not hurt to read once per sequence: one step long, or at most
   // one workgroup per CU. Saves the second launch (4 sequences x 4 heads, 500 + 60 keys: 7.4 us against 10.0).
   const int64_t groups = (int64_t)B * Hkv * q.rto;
-  q.whole = q.om != kByRows && cdiv(P, 128) + cdiv(max_len, 128) <= 8 && (P <= 128 || groups <= 256) &&
-            (max_len <= 256 || groups >= 128);
+  q.whole = q.whole || (cdiv(P, 128) + cdiv(max_len, 128) <= 8 && (P <= 128 || groups <= 256) &&
+                        (max_len <= 256 || groups >= 128));
   if (q.whole) {
     q.np = q.ns = q.pchunk = q.ochunk = 0;
     return q;
   }
   q.np = ranges(P, (int64_t)Hkv * q.rtp, 256, q.pm == kByRows ? 256 : 128, q.pchunk);
-  q.ns = ranges(max_len, (int64_t)B * Hkv * q.rto, 512, q.om == kByRows ? 256 : 128, q.ochunk);
+  q.ns = ranges(max_len, (int64_t)B * Hkv * q.rto, 512, 128, q.ochunk);
   return q;
 }
 }  // namespace
@@ -828,6 +883,10 @@ int prefix_attn(const bf16_t* q, int64_t qs, const bf16_t* kp, int64_t kph, int6
   if (D == DV && pl.om == NT) prefix_attn_short_kernel<DV, NT><<<(unsigned)n, kThreads, 0, stream>>>(a);
     KOP_PS(128, 1) KOP_PS(128, 2) KOP_PS(64, 1) KOP_PS(64, 2)
 #undef KOP_PS
+    if (pl.om == kByRows) {
+      if (D == 128) prefix_attn_long_kernel<128><<<(unsigned)n, kThreads, 0, stream>>>(a);
+      else prefix_attn_long_kernel<64><<<(unsigned)n, kThreads, 0, stream>>>(a);
+    }
     return hipGetLastError() == hipSuccess ? 0 : -9;
   }
   const int64_t grid = (int64_t)Hkv * pl.rtp * pl.np + (int64_t)B * Hkv * pl.rto * pl.ns;
@@ -835,8 +894,8 @@ int prefix_attn(const bf16_t* q, int64_t qs, const bf16_t* kp, int64_t kph, int6
 #define KOP_PA(DV, PM, OM)                                   \
   if (D == DV && pl.pm == PM && pl.om == OM && grid > 0)     \
     prefix_attn_kernel<DV, PM, OM><<<(unsigned)grid, kThreads, 0, stream>>>(a);
-  KOP_PA(128, 1, 1) KOP_PA(128, 2, 1) KOP_PA(128, 2, 2) KOP_PA(128, 4, 1) KOP_PA(128, 4, 2) KOP_PA(128, 4, 4)
-  KOP_PA(64, 1, 1) KOP_PA(64, 2, 1) KOP_PA(64, 2, 2) KOP_PA(64, 4, 1) KOP_PA(64, 4, 2) KOP_PA(64, 4, 4)
+  KOP_PA(128, 1, 1) KOP_PA(128, 2, 1) KOP_PA(128, 2, 2) KOP_PA(128, 4, 1) KOP_PA(128, 4, 2)
+  KOP_PA(64, 1, 1) KOP_PA(64, 2, 1) KOP_PA(64, 2, 2) KOP_PA(64, 4, 1) KOP_PA(64, 4, 2)
 #undef KOP_PA
   const unsigned cg = (unsigned)(((int64_t)B * T * Hq + 3) / 4);
   if (D == 128)

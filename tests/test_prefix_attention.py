@@ -148,6 +148,55 @@ def test_serving_sizes(B, T, Hq, Hkv, D, P, own):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B,T,Hq,Hkv,D,P", [(64, 24, 8, 2, 64, 130), (64, 25, 8, 2, 128, 64), (130, 96, 2, 2, 64, 0), (1, 1500, 32, 8, 128, 65),
+                                            (65, 40, 8, 4, 128, 1), (22, 50, 20, 4, 64, 300), (3, 700, 6, 6, 128, 0)])
+@pytest.mark.parametrize("more", [0, 97])
+def test_prompts(B, T, Hq, Hkv, D, P, more):
+    """Many rows per sequence: own lengths from the tokens alone up to ``more`` keys before them, stale keys of NaN behind."""
+    run(B, T, Hq, Hkv, D, P, [T + (more * b) // max(B - 1, 1) for b in range(B)], "cuda", seed=B)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("P", [0, 70])
+def test_prompts_empty_short_and_overlong(D, P):
+    """As above with lengths of 0, below the token count, past max_len and negative."""
+    B, T, Hq, Hkv = 64, 33, 12, 4
+    qkv, kp, vp, kc, vc = make(B, T, Hq, Hkv, D, P, 150, "cuda")
+    lens = torch.tensor([(0, 1, 32, 33, 34, 500, -3, 96)[b % 8] for b in range(B)], dtype=torch.int32, device="cuda")
+    got = check(qkv[:, : Hq * D], kp, vp, kc, vc, lens, 140, T).view(B, T, -1)
+    if P == 0:
+        assert not got[0].any() and not got[1, :-1].any() and got[1, -1].any() and not got[6].any()
+    none = kf.prefix_attention(qkv[:, : Hq * D], kp, vp, kc, vc, lens, 0, T)
+    if P == 0:
+        assert not none.any()
+    else:
+        check(qkv[:, : Hq * D], kp, vp, kc, vc, lens, 0, T)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_prompts_with_masked_keys_that_are_not_finite(D, bad):
+    """The key of token j holds NaN / inf: the rows of the tokens before it are those of a finite cache, bit for bit."""
+    B, T, Hq, Hkv, P, own = 32, 70, 8, 4, 50, 90
+    qkv, kp, vp, kc, vc = make(B, T, Hq, Hkv, D, P, own, "cuda", seed=1)
+    q, lens = qkv[:, : Hq * D], torch.full((B,), own, dtype=torch.int32, device="cuda")
+    want = kf.prefix_attention(q, kp, vp, kc, vc, lens, own, T).view(B, T, -1)
+    for j in (1, 31, 32, 44, 69):
+        for what in ("k", "v", "both"):
+            k2, v2 = kc.clone(), vc.clone()
+            if what != "v":
+                k2[:, :, own - T + j] = bad
+            if what != "k":
+                v2[:, :, own - T + j] = bad
+            got = kf.prefix_attention(q, kp, vp, k2, v2, lens, own, T).view(B, T, -1)
+            assert torch.equal(got[:, :j], want[:, :j]), (j, what)
+            if what == "v":
+                assert not torch.isfinite(got[:, j:].float()).any()
+
+
+@pytest.mark.gpu
 def test_large_scores():
     """Scores of several hundred: one key holds nearly everything, maxima that move from block to block."""
     run(8, 2, 8, 2, 128, 700, [2, 40, 90, 128, 129, 200, 300, 256], "cuda", size=32.0)
