@@ -817,16 +817,18 @@ inline int mode_of(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : kByR
 Plan make_plan(int B, int T, int G, int Hkv, int P, int max_len) {
   Plan q;
   const int64_t rows = (int64_t)B * T * G;
-  // Prompts: sequences whose own rows fill a 128-row tile, with a workgroup for every CU, take both parts by rows in one launch.
-  // Against the split form (64 sequences, 32/8 heads of 128, 2048 + 500 keys): 31 tokens 109 us and 154, 24 tokens 111 and 119, 16
-  // tokens (half a tile) 104 and 86; one sequence of 512 tokens behind 8192 (128 workgroups) 211 and 108.
-  q.whole = (int64_t)T * G >= 96 && (int64_t)B * Hkv * cdiv((int64_t)T * G, tile_rows(kByRows)) >= 256;
+  // Prompts: with a workgroup for every CU, both parts by rows in one launch where that costs less. In row-keys: by rows, 128-row
+  // tiles over prefix and own keys; split, prefix tiles filled from all sequences, own keys in 32-row tiles at half that rate,
+  // and partials worth 1100 keys a row. Measured (64 sequences, 32/8 heads of 128; split, by rows): 16 tokens behind 2048 + 500 own
+  // 81, 100 us; 24: 119, 111; 48: 231, 194; 33 tokens behind 8192 458, 566; 9 tokens, no prefix, 1000 own 80, 51; 8 tokens 45, 47.
+  const int64_t tg = (int64_t)T * G, rt = cdiv(tg, tile_rows(kByRows)), seen = std::max(max_len - T / 2, 0);
+  q.whole = tg > 32 && B * Hkv * rt >= 256 && 128 * rt * (P + seen) <= tg * (P + (int64_t)1100) + 64 * cdiv(tg, 32) * seen;
   // Otherwise own keys go by keys, also where 32-row tiles read them more than once: by rows (64 x 16 tokens, 8192 + 1000 keys) 313
   // us against 230.
-  q.om = q.whole ? kByRows : std::min(2, mode_of((int64_t)T * G));
+  q.om = q.whole ? kByRows : std::min(2, mode_of(tg));
   q.pm = P > 0 ? mode_of(rows) : q.om;
   q.rtp = P > 0 ? cdiv(rows, tile_rows(q.pm)) : 0;
-  q.rto = cdiv((int64_t)T * G, tile_rows(q.om));
+  q.rto = cdiv(tg, tile_rows(q.om));
   // key ranges of at least `least` keys, as many as make `want` workgroups
   auto ranges = [](int keys, int64_t groups, int want, int least, int& chunk) {
     chunk = least;

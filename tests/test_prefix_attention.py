@@ -149,7 +149,7 @@ def test_serving_sizes(B, T, Hq, Hkv, D, P, own):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("B,T,Hq,Hkv,D,P", [(64, 24, 8, 2, 64, 130), (64, 25, 8, 2, 128, 64), (130, 96, 2, 2, 64, 0), (1, 1500, 32, 8, 128, 65),
-                                            (65, 40, 8, 4, 128, 1), (22, 50, 20, 4, 64, 300), (3, 700, 6, 6, 128, 0)])
+                                            (65, 40, 8, 4, 128, 1), (40, 33, 16, 4, 64, 0), (64, 12, 24, 4, 128, 2000), (22, 50, 20, 4, 64, 300), (3, 700, 6, 6, 128, 0)])
 @pytest.mark.parametrize("more", [0, 97])
 def test_prompts(B, T, Hq, Hkv, D, P, more):
     """Many rows per sequence: own lengths from the tokens alone up to ``more`` keys before them, stale keys of NaN behind."""
