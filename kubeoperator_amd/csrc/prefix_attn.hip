@@ -21,7 +21,7 @@
 //     a second launch folds them. Decode (64 sequences, 32/8 heads of 128, 2048 + 500 keys): 23 + 5 us, 3.5 TB/s. Drafts (64 x 5
 //     tokens, 8192 + 1000 keys, prefix by rows): 86 + 7 us; the prefix alone 69, 630 TFLOP/s.
 //   * short contexts, by keys: a workgroup takes prefix and own keys of its rows, one launch, no partials. 4 sequences, 500 + 60
-//     keys: 7.4 us against 10.0 split.
+//     keys: 7.1 us against 8.3 split.
 //   * prompts, by rows: the same for sequences with many tokens. 8 x 1024 tokens behind 2048, 32/8 heads of 128: 448 us, 770
 //     TFLOP/s; one prompt of 4096, no prefix: 175 us, 780 TFLOP/s.
 //
@@ -838,7 +838,8 @@ Plan make_plan(int B, int T, int G, int Hkv, int P, int max_len) {
     return cdiv(keys, chunk);
   };
   // Short contexts: at most 8 steps of 128 keys per wave, and a prefix that it does not hurt to read once per sequence: one step long, or at most
-  // one workgroup per CU. Saves the second launch (4 sequences x 4 heads, 500 + 60 keys: 7.4 us against 10.0).
+  // one workgroup per CU. Saves the second launch (4 sequences x 4 heads, 500 + 60 keys: 7.1 us against 8.3; 64 x 32/8 heads of 128,
+  // 128 + 200 keys: 14.3 against 20.3; 16 of them, 500 + 200 keys: 11.8 against 14.0; one, 400 + 100: 10.1 against 9.1).
   const int64_t groups = (int64_t)B * Hkv * q.rto;
   q.whole = q.whole || (cdiv(P, 128) + cdiv(max_len, 128) <= 8 && (P <= 128 || groups <= 256) &&
                         (max_len <= 256 || groups >= 128));
@@ -846,8 +847,11 @@ Plan make_plan(int B, int T, int G, int Hkv, int P, int max_len) {
     q.np = q.ns = q.pchunk = q.ochunk = 0;
     return q;
   }
+  // One workgroup per CU for each part: half as many leave CUs without work, more write and fold more partials (64 x 5 tokens
+  // behind 8192 keys, prefix workgroups wanted 128, 256, 512, 1024: 193, 100, 113, 123 us; 16 x 8 tokens behind 4000: 58, 41, 46,
+  // 55; for the own keys all within 4 %).
   q.np = ranges(P, (int64_t)Hkv * q.rtp, 256, q.pm == kByRows ? 256 : 128, q.pchunk);
-  q.ns = ranges(max_len, (int64_t)B * Hkv * q.rto, 512, 128, q.ochunk);
+  q.ns = ranges(max_len, (int64_t)B * Hkv * q.rto, 256, 128, q.ochunk);
   return q;
 }
 }  // namespace

@@ -37,7 +37,8 @@ template <typename E>
 constexpr int piece() { return 64 * 16 / (int)sizeof(E); }
 constexpr int kPieces = 4;        // pieces per wave of the second pass
 constexpr int kHeld = 16;           // pieces of a row per lane of the draw that are held in registers
-constexpr int kOneRow = 4096, kOneLaunch = 32768;  // logits per row and sequence up to which one launch does everything
+// logits per row, and per sequence (sampling, greedy), up to which one launch does everything
+constexpr int kOneRow = 4096, kOneLaunch = 16384, kOneGreedy = 24576;
 constexpr int kMaxRows = 2 * kVerifyMaxDraft + 1;
 
 template <typename E>
@@ -484,7 +485,8 @@ __global__ void __launch_bounds__(kT) verify_greedy_kernel(Args a) {
   if (threadIdx.x < 64) put(a, b, j, (int64_t)s_s[j]);
 }
 
-// ---- all of it for a small problem: grid B. A wave takes every fourth row, twice (maximum, then sum: the row is in cache).
+// ---- all of it for a small problem: grid B. A wave takes every fourth row, twice (maximum, then sum: the row is in cache). Bound
+// by its chain of loads and sums: 64 sequences, 3 drafts, 1000 logits 10.2 us (three launches 17.6).
 template <typename E, bool GREEDY>
 __global__ void __launch_bounds__(kT) verify_small_kernel(Args a) {
   constexpr int N = Vec<E>::N;
@@ -547,8 +549,10 @@ __global__ void __launch_bounds__(kT) verify_small_kernel(Args a) {
 template <typename E>
 int launch(const Args& a, bool greedy, hipStream_t stream) {
   const int nrow = greedy ? a.T + 1 : 2 * a.T + 1;
-  // one workgroup per sequence is short of threads for long rows, three launches cost more than they do for short ones
-  if (a.V <= kOneRow && (int64_t)nrow * a.V <= kOneLaunch) {
+  // One workgroup per sequence is short of threads for long rows, three launches cost more than they do for short ones: sampling, 7
+  // rows of 2048 fp32 logits 13.5 us in one launch and 14.8 in three, of 2500 16.2 and 15.0; greedy, 9 rows of 2000 7.3 and 8.9 in
+  // two, of 4096 11.7 and 8.7.
+  if (a.V <= kOneRow && (int64_t)nrow * a.V <= (greedy ? kOneGreedy : kOneLaunch)) {
     if (greedy) verify_small_kernel<E, true><<<a.B, kT, 0, stream>>>(a);
     else verify_small_kernel<E, false><<<a.B, kT, 0, stream>>>(a);
   } else {

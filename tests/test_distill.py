@@ -80,6 +80,16 @@ def test_matches_the_formula(dev, N, V, K, t):
     check(*make(N, V, K, dev, seed=1)[:3], t, None)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [65545, 128251])
+def test_many_long_rows(V):
+    """More long rows than the chip has CUs take a form of their own."""
+    logits, index, teacher, weight = make(258, V, 8, "cuda")
+    weight[3] = 0
+    logits[7, 100:] = float("-inf")
+    check(logits, index, teacher, 1.5, weight)
+
+
 @pytest.mark.parametrize("dev", DEVS)
 @pytest.mark.parametrize("V", [40, 4099, 50304, 128256])
 def test_padding_weights_repeats_and_masked_logits(dev, V):
