@@ -40,6 +40,9 @@ namespace {
 constexpr int kThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegBig = -3.402823466e38f;
+// A row's reference for exp2 follows its maximum only when that is this much higher: any reference gives the same softmax, weights
+// of up to 2^8 round as well as those of up to 1, and most tiles then need no rescaling of O^T.
+constexpr float kSlack = 8.f;
 constexpr int kLds = 65536;
 constexpr int kByRows = 4;
 constexpr int kTrans = 0x400, kMfma = 0x8, kDsRead = 0x100;  // instruction classes of sched_group_barrier
@@ -151,7 +154,7 @@ __device__ __forceinline__ void raise_max(f32x4* sc, int left, float sl2, float&
   for (int j = 1; j + 1 < 8 * NB; j += 2) mx = vmax(vmax(mx, sc[j >> 2][j & 3]), sc[(j + 1) >> 2][(j + 1) & 3]);
   mx = vmax(mx, sc[2 * NB - 1][3]);
   mx = xor32_max(xor16_max(mx)) * sl2;
-  if (__any(mx > m)) {
+  if (__any(mx > m + kSlack)) {
     const float nm = fmaxf(m, mx);
     const float al = __builtin_amdgcn_exp2f(m - nm);
     m = nm;
