@@ -19,11 +19,11 @@
 // and a launch takes one of three forms (make_plan):
 //   * split: workgroups of (row tile, key range) of the prefix, and of one sequence's own keys, write fp32 partials (O, max, sum);
 //     a second launch folds them. Decode (64 sequences, 32/8 heads of 128, 2048 + 500 keys): 23 + 5 us, 3.5 TB/s. Drafts (64 x 5
-//     tokens, 8192 + 1000 keys, prefix by rows): 86 + 7 us; the prefix alone 69, 630 TFLOP/s.
+//     tokens, 8192 + 1000 keys, prefix by rows): 83 + 7 us; the prefix alone 69, 630 TFLOP/s.
 //   * short contexts, by keys: a workgroup takes prefix and own keys of its rows, one launch, no partials. 4 sequences, 500 + 60
 //     keys: 7.1 us against 8.3 split.
-//   * prompts, by rows: the same for sequences with many tokens. 8 x 1024 tokens behind 2048, 32/8 heads of 128: 448 us, 770
-//     TFLOP/s; one prompt of 4096, no prefix: 175 us, 780 TFLOP/s.
+//   * prompts, by rows: the same for sequences with many tokens. 8 x 1024 tokens behind 2048, 32/8 heads of 128: 413 us, 830
+//     TFLOP/s; one prompt of 4096, no prefix: 151 us, 910 TFLOP/s.
 //
 // A masked key has weight zero exactly: masked scores never enter the maximum or the sum, keys past the last valid one are
 // never read (loads are clamped to it), and in the blocks where some rows see a key and others do not, values that are
@@ -565,6 +565,9 @@ __device__ __forceinline__ void by_rows(const Args& p, F part, char* smem) {
         }
       }
       __builtin_amdgcn_sched_barrier(0);
+      // waves in the vector stretch go first: the other wave of the SIMD has matrix instructions to fill the gaps with (8 x 1024 tokens
+      // behind 4096: 639 us without, 621)
+      __builtin_amdgcn_s_setprio(0);
       v_at(buf, vat);
 #pragma unroll
       for (int n = 0; n < NT; ++n) acc[n][NC] = sum_p(pf[n][1], sum_p(pf[n][0], acc[n][NC]));
@@ -603,6 +606,7 @@ __device__ __forceinline__ void by_rows(const Args& p, F part, char* smem) {
         __builtin_amdgcn_sched_group_barrier(kMfma, 3 * NT, 0);
       }
       __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(1);
       if constexpr (NEXT && EDGE) {
         k_at(buf ^ 1, kat);
         scores(kat, sc);
