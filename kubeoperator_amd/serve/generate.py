@@ -469,7 +469,7 @@ class LlamaGenerator:
             rounds.append(kept)
             for b in range(B):
                 out[b] += new[b][: kept[b] + 1]
-            # a finished sequence stays where this round began: it goes on computing rows that are thrown away
+            # a finished sequence stays where it was before these drafts: it goes on computing rows that are thrown away
             lens = [n if len(o) >= max_new_tokens else n + k + 1 for n, k, o in zip(start, kept, out)]
             for g in (self, draft):
                 g.cache.truncate(lens)

@@ -216,6 +216,12 @@ def test_other_scales(dev, scale, B, T):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1.0])
+def test_prompts_with_other_scales(scale):
+    test_other_scales("cuda", scale, 130, 30)
+
+
+@pytest.mark.gpu
 def test_offsets_past_32_bits():
     """A cache and a prefix of more than 2^31 elements each; the queries match keys near the end."""
     Hkv, D, n = 8, 128, (1 << 21) + 4097
@@ -292,7 +298,7 @@ def test_a_cache_without_heads_is_refused(dev):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("B,T,P", [(4, 1, 500), (48, 4, 700)])
+@pytest.mark.parametrize("B,T,P", [(4, 1, 500), (48, 4, 700), (130, 20, 30)])
 def test_captured_call_replays_and_another_stream(B, T, P):
     Hq, Hkv, D = 8, 2, 128
     qkv, kp, vp, kc, vc = make(B, T, Hq, Hkv, D, P, 200, "cuda")
