@@ -136,15 +136,28 @@ def prefix_attention_ref(q, k_prefix, v_prefix, k_cache, v_cache, lens, max_len,
     require(0 <= max_len <= Smax, "max_len must be in [0, Smax]")
     Hq = q.shape[1] // D
     out = torch.zeros(B * tokens, Hq, D, dtype=q.dtype, device=q.device)
+    P, G = k_prefix.shape[1], Hq // Hkv
     for b in range(B):
         n = min(max(int(lens[b]), 0), max_len)
-        for t in range(tokens):
-            own = max(n - (tokens - 1 - t), 0)
-            k = torch.cat([k_prefix, k_cache[b, :, :own]], 1).float().repeat_interleave(Hq // Hkv, dim=0)
-            v = torch.cat([v_prefix, v_cache[b, :, :own]], 1).float().repeat_interleave(Hq // Hkv, dim=0)
-            if k.shape[1]:
-                s = torch.matmul(k, q[b * tokens + t].float().view(Hq, D, 1)).squeeze(-1) * scale
-                out[b * tokens + t] = torch.matmul(torch.softmax(s, -1).unsqueeze(1), v).squeeze(1).to(q.dtype)
+        k = torch.cat([k_prefix, k_cache[b, :, :n]], 1).float()
+        v = torch.cat([v_prefix, v_cache[b, :, :n]], 1).float()
+        qb = q[b * tokens:(b + 1) * tokens].float().view(tokens, Hkv, G, D).permute(1, 0, 2, 3)  # [Hkv, tokens, G, D]
+        seen = P + (n - tokens + 1 + torch.arange(tokens, device=q.device)).clamp(min=0)  # keys each token sees
+        top, late = int(seen[-1]), int(seen[0])
+        if not top:
+            continue
+        hidden = torch.arange(top, device=q.device) >= seen.unsqueeze(1)  # [tokens, top]
+        # values that only some tokens see: those that are not finite must not reach the others as 0 times NaN
+        bad = ~torch.isfinite(v[:, late:top])
+        v[:, late:top] = v[:, late:top].masked_fill(bad, 0.0)
+        s = torch.matmul(qb.reshape(Hkv, tokens * G, D), k[:, :top].transpose(1, 2)) * scale
+        s = s.view(Hkv, tokens, G, top).masked_fill(hidden.view(1, tokens, 1, top), float("-inf"))
+        o = torch.matmul(torch.softmax(s, -1).view(Hkv, tokens * G, top), v[:, :top]).view(Hkv, tokens, G, D)
+        if bool(bad.any()):
+            hit = torch.matmul((~hidden[:, late:]).float(), bad.float()) > 0  # [Hkv, tokens, D]
+            o = o.masked_fill(hit.unsqueeze(2), float("nan"))
+        o = o.masked_fill((seen == 0).view(1, tokens, 1, 1), 0.0)
+        out[b * tokens:(b + 1) * tokens] = o.permute(1, 0, 2, 3).reshape(tokens, Hq, D).to(q.dtype)
     return out.view(B * tokens, Hq * D)
 
 
