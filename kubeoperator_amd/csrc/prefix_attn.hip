@@ -141,8 +141,8 @@ __device__ __forceinline__ float vmax(float a, float b) { return __builtin_eleme
 
 // One 16-row tile's running softmax over NB blocks of 32 keys: sc[b] = scores of products 2 b, 2 b + 1 (the lane's keys
 // 32 (b / 2) + 8 g + 4 (b % 2) + e). `left`: the lane's keys of block 0 with a number below it are seen (block b:
-// left - 32 b); only looked at on an edge. First the maximum: masked scores leave sc, and where a row's maximum rises, acc (NC
-// blocks of O^T and, last, the row's sum: see sum_p) is scaled down.
+// left - 32 b); only looked at on an edge. First the maximum: masked scores leave sc, and where a row's maximum rises by
+// more than kSlack, acc (NC blocks of O^T and, last, the row's sum: see sum_p) is scaled down.
 template <bool EDGE, int NB, int NC>
 __device__ __forceinline__ void raise_max(f32x4* sc, int left, float sl2, float& m, f32x4* acc) {
   if constexpr (EDGE) {
@@ -777,7 +777,8 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attn_long_kernel(Args p) {
   by_rows<D, true>(p, [&](int seg) { return whole_part<D, tile_rows(kByRows)>(p, blockIdx.x, 1 - seg); }, smem);
 }
 
-// one wave per (row, KV head): the ranges that its row sees, then o = sum O 2^(m - M) / sum l 2^(m - M)
+// one wave per (row, KV head): the ranges that its row sees, then o = sum O 2^(m - M) / sum l 2^(m - M). Bound by its chain of
+// loads: 64 sequences 4.9 us, 64 x 5 tokens (21 MB of partials) 7
 template <int D>
 __global__ void __launch_bounds__(kThreads) prefix_attn_combine_kernel(Args p) {
   constexpr int DPT = D / 64;
@@ -826,7 +827,7 @@ Plan make_plan(int B, int T, int G, int Hkv, int P, int max_len) {
   const int64_t rows = (int64_t)B * T * G;
   // Prompts: with a workgroup for every CU, both parts by rows in one launch where that costs less. In row-keys: by rows, 128-row
   // tiles over prefix and own keys; split, prefix tiles filled from all sequences, own keys in 32-row tiles at half that rate,
-  // and partials worth 1100 keys a row. Measured (64 sequences, 32/8 heads of 128; split, by rows): 16 tokens behind 2048 + 500 own
+  // and partials worth 1100 keys a row; up to 32 rows go by keys. Measured (64 sequences, 32/8 heads of 128; split, by rows): 16 tokens behind 2048 + 500 own
   // 81, 100 us; 24: 119, 111; 48: 231, 194; 33 tokens behind 8192 458, 566; 9 tokens, no prefix, 1000 own 80, 51; 8 tokens 45, 47.
   const int64_t tg = (int64_t)T * G, rt = cdiv(tg, tile_rows(kByRows)), seen = std::max(max_len - T / 2, 0);
   q.whole = tg > 32 && B * Hkv * rt >= 256 && 128 * rt * (P + seen) <= tg * (P + (int64_t)1100) + 64 * cdiv(tg, 32) * seen;
@@ -844,8 +845,8 @@ Plan make_plan(int B, int T, int G, int Hkv, int P, int max_len) {
     chunk = cdiv(cdiv(keys, n), 128) * 128;
     return cdiv(keys, chunk);
   };
-  // Short contexts: at most 8 steps of 128 keys per wave, and a prefix that it does not hurt to read once per sequence: one step long, or at most
-  // one workgroup per CU. Saves the second launch (4 sequences x 4 heads, 500 + 60 keys: 7.1 us against 8.3; 64 x 32/8 heads of 128,
+  // Short contexts: at most 8 steps of 128 keys per wave, and a prefix that it does not hurt to read once per sequence: one step
+  // long, or at most one workgroup per CU. Saves the second launch (4 sequences x 4 heads, 500 + 60 keys: 7.1 us against 8.3; 64 x 32/8 heads of 128,
   // 128 + 200 keys: 14.3 against 20.3; 16 of them, 500 + 200 keys: 11.8 against 14.0; one, 400 + 100: 10.1 against 9.1).
   const int64_t groups = (int64_t)B * Hkv * q.rto;
   q.whole = q.whole || (cdiv(P, 128) + cdiv(max_len, 128) <= 8 && (P <= 128 || groups <= 256) &&

@@ -570,7 +570,10 @@ int launch(const Args& a, bool greedy, hipStream_t stream) {
   return hipGetLastError() == hipSuccess ? 0 : -9;
 }
 inline int64_t chunks(int V) { return (V + kChunk - 1) / kChunk; }
-inline int64_t pieces(int V, bool f32) { return (V + (f32 ? piece<float>() : piece<bf16_t>()) - 1) / (f32 ? piece<float>() : piece<bf16_t>()); }
+inline int64_t pieces(int V, bool f32) {
+  const int n = f32 ? piece<float>() : piece<bf16_t>();
+  return (V + n - 1) / n;
+}
 }  // namespace
 
 int64_t verify_draft_workspace(int B, int T, int V, bool f32) {
