@@ -8,7 +8,10 @@
 // keys leave HBM once per row tile instead of once per sequence, and its products have enough rows for the matrix cores.
 //
 // S^T [keys x rows] = K . Q^T and O^T [dims x rows] += V^T . P^T on v_mfma_f32_16x16x32_bf16, with running maximum and sum
-// per row (fp32), P rounded to bf16 for the matrix cores (half a step: 2^-9 relative per key). The 16 key rows of product b are keys
+// per row (fp32). P goes through the matrix cores as a bf16 value and its bf16 remainder, two products (2^-16 relative per key): a
+// value alone (2^-8) adds as much to the result's error as its own rounding does (0.0023 relative instead of 0.0016), saves nothing
+// where memory is the bound and a sixth to a quarter where the matrix cores are (drafts 86 us, with the remainder 101; prompts 371
+// and 468). The 16 key rows of product b are keys
 // 8 (i >> 2) + 4 b + (i & 3), so that a lane's scores of two products are its own P^T operand (keys 8 g .. 8 g + 7 of its row),
 // with no lane exchange; V goes through an LDS image whose 16-byte chunks are XOR-permuted by the row, and is read transposed.
 // A workgroup works in one of two ways:
@@ -77,16 +80,20 @@ __device__ __forceinline__ void read_v4(const uint32_t* a, bf16x8* v) {
 #pragma unroll
   for (int c = 0; c < 4; ++c) v[c] = cat44(t[2 * c], t[2 * c + 1]);
 }
-// true if one of 8 bf16 values is not finite; `fin` = the values with those replaced by 0, `bad` = 1 in their places, else 0
-__device__ __forceinline__ bool split_finite(bf16x8 v, bf16x8& fin, bf16x8& bad) {
-  bool any = false;
+// the 8 bf16 values with those that are not finite replaced by 0, and 1 in their places, else 0
+__device__ __forceinline__ void split_finite(bf16x8 v, bf16x8& fin, bf16x8& bad) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const bool nf = (v[i] & 0x7f80) == 0x7f80;
-    any |= nf;
     fin[i] = nf ? (short)0 : v[i];
     bad[i] = nf ? (short)0x3f80 : (short)0;
   }
+}
+__device__ __forceinline__ bool not_finite(bf16x8 v) {
+  const u32x4 w = __builtin_bit_cast(u32x4, v);
+  bool any = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) any |= (w[i] & 0x7f80u) == 0x7f80u || (w[i] & 0x7f800000u) == 0x7f800000u;
   return any;
 }
 
@@ -142,9 +149,9 @@ __device__ __forceinline__ float vmax(float a, float b) { return __builtin_eleme
 // One 16-row tile's running softmax over NB blocks of 32 keys: sc[b] = scores of products 2 b, 2 b + 1 (the lane's keys
 // 32 (b / 2) + 8 g + 4 (b % 2) + e). `left`: the lane's keys of block 0 with a number below it are seen (block b:
 // left - 32 b); only looked at on an edge. First the maximum: masked scores leave sc, and where a row's maximum rises by
-// more than kSlack, acc (NC blocks of O^T and, last, the row's sum: see sum_p) is scaled down.
+// more than kSlack, acc (NC blocks of O^T) and l (the sum of the lane's own weights) are scaled down.
 template <bool EDGE, int NB, int NC>
-__device__ __forceinline__ void raise_max(f32x4* sc, int left, float sl2, float& m, f32x4* acc) {
+__device__ __forceinline__ void raise_max(f32x4* sc, int left, float sl2, float& m, float& l, f32x4* acc) {
   if constexpr (EDGE) {
 #pragma unroll
     for (int j = 0; j < 8 * NB; ++j) sc[j >> 2][j & 3] = 32 * (j >> 3) + (j & 7) < left ? sc[j >> 2][j & 3] : kNegBig;
@@ -158,47 +165,55 @@ __device__ __forceinline__ void raise_max(f32x4* sc, int left, float sl2, float&
     const float nm = fmaxf(m, mx);
     const float al = __builtin_amdgcn_exp2f(m - nm);
     m = nm;
+    l *= al;
 #pragma unroll
-    for (int c = 0; c <= NC; ++c)
+    for (int c = 0; c < NC; ++c)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[c][e] *= al;
   }
 }
-// Then the weights, P^T, rounded to bf16.
+// Then the weights, P^T: their sum into l, in fp32, and each as a bf16 value and the bf16 remainder (off by 2^-16 of it at most).
 template <bool EDGE, int NB>
-__device__ __forceinline__ void weights(const f32x4* sc, int left, float sl2, float m, bf16x8* pf) {
-  float v[8 * NB];
-#pragma unroll
-  for (int j = 0; j < 8 * NB; ++j) v[j] = __builtin_amdgcn_exp2f(fmaf(sc[j >> 2][j & 3], sl2, -m));
-  if constexpr (EDGE) {
-#pragma unroll
-    for (int j = 0; j < 8 * NB; ++j) v[j] = 32 * (j >> 3) + (j & 7) < left ? v[j] : 0.f;
-  }
+__device__ __forceinline__ void weights(const f32x4* sc, int left, float sl2, float m, float& l, bf16x8* hi, bf16x8* lo) {
+  float s[2] = {0.f, 0.f};
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    const float* q = v + 8 * b;
-    pf[b] = __builtin_bit_cast(bf16x8, u32x4{pack2(q[0], q[1]), pack2(q[2], q[3]), pack2(q[4], q[5]), pack2(q[6], q[7])});
+    u32x4 h, r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float v[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int j = 8 * b + 2 * i + k;
+        v[k] = __builtin_amdgcn_exp2f(fmaf(sc[j >> 2][j & 3], sl2, -m));
+        if constexpr (EDGE) v[k] = 32 * (j >> 3) + (j & 7) < left ? v[k] : 0.f;
+        s[k] += v[k];
+      }
+      h[i] = pack2(v[0], v[1]);
+      r[i] = pack2(v[0] - __uint_as_float(h[i] << 16), v[1] - __uint_as_float(h[i] & 0xffff0000u));
+    }
+    hi[b] = __builtin_bit_cast(bf16x8, h);
+    lo[b] = __builtin_bit_cast(bf16x8, r);
   }
+  l += s[0] + s[1];
 }
-// the row's sum of the rounded P on the matrix cores: every lane of the row gets it whole
-__device__ __forceinline__ f32x4 sum_p(bf16x8 pf, f32x4 acc) {
-  constexpr short one = 0x3f80;
-  return mfma16(bf16x8{one, one, one, one, one, one, one, one}, pf, acc);
-}
+// a row's sum from its four lanes'
+__device__ __forceinline__ float row_sum(float l) { return xor32_sum(xor16_sum(l)); }
 
 // acc += V^T . P^T where some rows see a key and others do not: values that are not finite reach only the rows that see them
-// (as NaN). True if there were any; `left` as in softmax_step, of this block.
+// (as NaN). True if there were any; `left` as in weights(), of this block.
 template <int NT>
-__device__ __forceinline__ bool edge_pv(bf16x8 vf, const bf16x8* pf, const int* left, f32x4* acc) {
+__device__ __forceinline__ bool edge_pv(bf16x8 vf, const bf16x8* hi, const bf16x8* lo, const int* left, f32x4* acc) {
+  if (!__any(not_finite(vf))) return false;
   bf16x8 fin, bad;
-  if (!__any(split_finite(vf, fin, bad))) return false;
+  split_finite(vf, fin, bad);
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     bf16x8 ones;
 #pragma unroll
     for (int j = 0; j < 8; ++j) ones[j] = j < left[n] ? (short)0x3f80 : (short)0;
     const f32x4 nb = mfma16(bad, ones, f32x4{0.f, 0.f, 0.f, 0.f});
-    acc[n] = mfma16(fin, pf[n], acc[n]);
+    acc[n] = mfma16(fin, hi[n], mfma16(fin, lo[n], acc[n]));
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[n][e] = nb[e] > 0.f ? __builtin_nanf("") : acc[n][e];
   }
@@ -233,12 +248,13 @@ __device__ __forceinline__ void by_keys(const Args& p, F part, char* smem) {
   for (int c = 0; c < NC; ++c)
     va[c] = lds_addr(vimg) + (8 * g + tq) * ROWB + 8 * (tp & 1) + 16 * ((2 * c + (tp >> 1)) ^ (2 * x));
   float m[NT], l[NT];
-  f32x4 acc[NT][NC + 1];
+  f32x4 acc[NT][NC];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     m[n] = kNegBig;
+    l[n] = 0.f;
 #pragma unroll
-    for (int c = 0; c <= NC; ++c) acc[n][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < NC; ++c) acc[n][c] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 #pragma unroll 1
   for (int seg = 0; seg < SEGS; ++seg) {
@@ -308,14 +324,14 @@ __device__ __forceinline__ void by_keys(const Args& p, F part, char* smem) {
           for (int s = 0; s < NS; ++s) sc[n][bb] = mfma16(kf[bb][s], qf[n][s], sc[n][bb]);
         }
       if (more) load(kb + KSTEP, [&](auto last) { load_k(last, kb + KSTEP, kf); });
-      bf16x8 pf[NT];
+      bf16x8 hi[NT], lo[NT];
       int left[NT];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         left[n] = lim[n] - kb - 8 * g;
-        raise_max<EDGE, 1, NC>(sc[n], left[n], p.sl2, m[n], acc[n]);
-        weights<EDGE, 1>(sc[n], left[n], p.sl2, m[n], &pf[n]);
-        acc[n][NC] = sum_p(pf[n], acc[n][NC]);
+        raise_max<EDGE, 1, NC>(sc[n], left[n], p.sl2, m[n], l[n], acc[n]);
+        if constexpr (EDGE && SEGS == 2) asm volatile("" : "+v"(left[n]));  // (its comparisons are made again, not held: scalar registers)
+        weights<EDGE, 1>(sc[n], left[n], p.sl2, m[n], l[n], &hi[n], &lo[n]);
       }
 #pragma unroll
       for (int c0 = 0; c0 < NC; c0 += 4) {
@@ -330,16 +346,16 @@ __device__ __forceinline__ void by_keys(const Args& p, F part, char* smem) {
             f32x4 an[NT];
 #pragma unroll
             for (int n = 0; n < NT; ++n) an[n] = acc[n][c0 + c];
-            if (!edge_pv<NT>(vf[c], pf, left, an)) {
+            if (!edge_pv<NT>(vf[c], hi, lo, left, an)) {
 #pragma unroll
-              for (int n = 0; n < NT; ++n) an[n] = mfma16(vf[c], pf[n], an[n]);
+              for (int n = 0; n < NT; ++n) an[n] = mfma16(vf[c], hi[n], mfma16(vf[c], lo[n], an[n]));
             }
 #pragma unroll
             for (int n = 0; n < NT; ++n) acc[n][c0 + c] = an[n];
             __builtin_amdgcn_sched_barrier(0);
           } else {
 #pragma unroll
-            for (int n = 0; n < NT; ++n) acc[n][c0 + c] = mfma16(vf[c], pf[n], acc[n][c0 + c]);
+            for (int n = 0; n < NT; ++n) acc[n][c0 + c] = mfma16(vf[c], hi[n], mfma16(vf[c], lo[n], acc[n][c0 + c]));
           }
         }
       }
@@ -350,7 +366,7 @@ __device__ __forceinline__ void by_keys(const Args& p, F part, char* smem) {
   // the 4 waves' (m, l, O^T) -> one partial: waves 2, 3 into 0, 1, then 1 into 0
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    l[n] = acc[n][NC][0];
+    l[n] = row_sum(l[n]);
     if (g == 0) {
       s_ml[wv][16 * n + col][0] = m[n];
       s_ml[wv][16 * n + col][1] = l[n];
@@ -432,8 +448,7 @@ __device__ __forceinline__ void by_rows(const Args& p, F part, char* smem) {
   constexpr int ROWB = D * 2, NS = D / 32, NC = D / 16, TK = 64, IMG = TK * ROWB, SLOTS = ROWB / 16, NT = 2;
   constexpr int PER = TK * SLOTS / kThreads;  // 16-byte pieces per thread and image
   static_assert(4 * IMG <= kLds, "LDS");
-  const int t = threadIdx.x, lane = t & 63, col = lane & 15, g = lane >> 4;
-  const int wv = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Work w0 = part(0);
   const bool live = 32 * wv < w0.nrow;
   bf16x8 qf[NT][NS];
@@ -442,6 +457,7 @@ __device__ __forceinline__ void by_rows(const Args& p, F part, char* smem) {
   __shared__ bf16_t* s_op[WHOLE ? kThreads / 64 * 32 : 1];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
+    const int col = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
     const int i = 32 * wv + 16 * n + col, r = w0.row0 + (i < w0.nrow ? i : 0);
     load_q<D>(p, w0, r, g, qf[n]);
     const int bt = r / p.G;
@@ -453,17 +469,14 @@ __device__ __forceinline__ void by_rows(const Args& p, F part, char* smem) {
   // K image: chunk slots XORed with the row's number in a 16-row operand (8 a + 4 b + q -> 4 a + q), so that its 16 rows'
   // reads of one chunk fall on different banks; V image as in by_keys
   auto kx = [](int r) { return ROWB == 256 ? (((r >> 3) & 3) << 2) | (r & 3) : (((r >> 3) & 3) << 1) | ((r >> 1) & 1); };
-  // chunk 4 s + g of a K row is at ka ^ 64 s, 16-dim block c of V^T at va ^ 32 c
-  const int krow = 8 * (col >> 2) + (col & 3), vrow = 8 * g + ((lane >> 2) & 3), tp = lane & 3;
-  const int ka = krow * ROWB + 16 * (g ^ kx(krow));
-  const int va = vrow * ROWB + 8 * (tp & 1) + 16 * ((tp >> 1) ^ vx<ROWB>(vrow));
-  float m[NT];
-  f32x4 acc[NT][NC + 1];
+  float m[NT], l[NT];
+  f32x4 acc[NT][NC];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     m[n] = kNegBig;
+    l[n] = 0.f;
 #pragma unroll
-    for (int c = 0; c <= NC; ++c) acc[n][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < NC; ++c) acc[n][c] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   auto barrier = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
 #pragma unroll 1
@@ -471,6 +484,13 @@ __device__ __forceinline__ void by_rows(const Args& p, F part, char* smem) {
     const Work w = WHOLE ? part(seg) : w0;
     if (WHOLE && w.k0 >= w.kend) continue;
     if (seg > 0) barrier();  // the images are free
+    int t = threadIdx.x;
+    if constexpr (WHOLE) asm volatile("" : "+v"(t));  // what follows from it is made again for each part, not held over the other one's loop
+    const int lane = t & 63, col = lane & 15, g = lane >> 4;
+    // chunk 4 s + g of a K row is at ka ^ 64 s, 16-dim block c of V^T at va ^ 32 c
+    const int krow = 8 * (col >> 2) + (col & 3), vrow = 8 * g + ((lane >> 2) & 3), tp = lane & 3;
+    const int ka = krow * ROWB + 16 * (g ^ kx(krow));
+    const int va = vrow * ROWB + 8 * (tp & 1) + 16 * ((tp >> 1) ^ vx<ROWB>(vrow));
     int lim[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) lim[n] = seen_by(p, w, s_bt[32 * wv + 16 * n + col]);
@@ -542,25 +562,26 @@ __device__ __forceinline__ void by_rows(const Args& p, F part, char* smem) {
     auto tile = [&](auto edge_, auto next_, int kb, int buf) {
       constexpr bool EDGE = decltype(edge_)::value, NEXT = decltype(next_)::value, SIFT = EDGE && WHOLE;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) raise_max<EDGE, 2, NC>(sc[n], lim[n] - kb - 8 * g, p.sl2, m[n], acc[n]);
-      bf16x8 pf[NT][2];
+      for (int n = 0; n < NT; ++n) raise_max<EDGE, 2, NC>(sc[n], lim[n] - kb - 8 * g, p.sl2, m[n], l[n], acc[n]);
+      bf16x8 hi[NT][2], lo[NT][2];
       f32x4 nx[NT][4];
       uint32_t kat[NS], vat[NC];
       if constexpr (NEXT && !EDGE) k_at(buf ^ 1, kat);
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (NEXT && !EDGE) scores(kat, nx);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) weights<EDGE, 2>(sc[n], lim[n] - kb - 8 * g, p.sl2, m[n], pf[n]);
+      for (int n = 0; n < NT; ++n) weights<EDGE, 2>(sc[n], lim[n] - kb - 8 * g, p.sl2, m[n], l[n], hi[n], lo[n]);
       if constexpr (NEXT && !EDGE) {
-        // issue order: operands of one 16-key product ahead, and between two matrix instructions what one of them leaves time for
+        // issue order: operands of one 16-key product ahead, each read once its register's last value is used, and between two
+        // matrix instructions what one of them leaves time for
         __builtin_amdgcn_sched_group_barrier(kDsRead, NS, 0);
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-          if (b < 3) __builtin_amdgcn_sched_group_barrier(kDsRead, NS, 0);
 #pragma unroll
           for (int i = 0; i < NS * NT; ++i) {
             __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
             __builtin_amdgcn_sched_group_barrier(kTrans, 8 / (NS * NT), 0);
+            if (b < 3 && i % NT == NT - 1) __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
           }
         }
       }
@@ -569,8 +590,6 @@ __device__ __forceinline__ void by_rows(const Args& p, F part, char* smem) {
       // behind 4096: 639 us without, 621)
       __builtin_amdgcn_s_setprio(0);
       v_at(buf, vat);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) acc[n][NC] = sum_p(pf[n][1], sum_p(pf[n][0], acc[n][NC]));
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int b = 0; b < 2; ++b)
@@ -579,31 +598,36 @@ __device__ __forceinline__ void by_rows(const Args& p, F part, char* smem) {
           const char* vp = vimg + vat[c] + 32 * b * ROWB;
           const bf16x8 vf = cat44(lds_tr_read(vp), lds_tr_read(vp + 4 * ROWB));
           if constexpr (SIFT) {
-            bf16x8 pfn[NT];
+            bf16x8 hn[NT], ln[NT];
             f32x4 an[NT];
             int left[NT];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) pfn[n] = pf[n][b], an[n] = acc[n][c], left[n] = lim[n] - kb - 8 * g - 32 * b;
-            if (!edge_pv<NT>(vf, pfn, left, an)) {
+            for (int n = 0; n < NT; ++n) {
+              hn[n] = hi[n][b], ln[n] = lo[n][b], an[n] = acc[n][c], left[n] = lim[n] - kb - 8 * g - 32 * b;
+              asm volatile("" : "+v"(left[n]));  // what is made of it is made where it is used, and not held for all blocks
+            }
+            if (!edge_pv<NT>(vf, hn, ln, left, an)) {
 #pragma unroll
-              for (int n = 0; n < NT; ++n) an[n] = mfma16(vf, pfn[n], an[n]);
+              for (int n = 0; n < NT; ++n) an[n] = mfma16(vf, hn[n], mfma16(vf, ln[n], an[n]));
             }
 #pragma unroll
             for (int n = 0; n < NT; ++n) acc[n][c] = an[n];
             __builtin_amdgcn_sched_barrier(0);
           } else {
 #pragma unroll
-            for (int n = 0; n < NT; ++n) acc[n][c] = mfma16(vf, pf[n][b], acc[n][c]);
+            for (int n = 0; n < NT; ++n) acc[n][c] = mfma16(vf, lo[n][b], acc[n][c]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[n][c] = mfma16(vf, hi[n][b], acc[n][c]);
           }
         }
       if constexpr (!SIFT) {  // issue order: three 16-dim blocks' operands ahead
         __builtin_amdgcn_sched_group_barrier(kDsRead, 6, 0);
 #pragma unroll
         for (int i = 0; i < 2 * NC - 3; ++i) {
-          __builtin_amdgcn_sched_group_barrier(kMfma, NT, 0);
+          __builtin_amdgcn_sched_group_barrier(kMfma, 2 * NT, 0);
           __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 0);
         }
-        __builtin_amdgcn_sched_group_barrier(kMfma, 3 * NT, 0);
+        __builtin_amdgcn_sched_group_barrier(kMfma, 6 * NT, 0);
       }
       __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_setprio(1);
@@ -654,12 +678,15 @@ __device__ __forceinline__ void by_rows(const Args& p, F part, char* smem) {
     stage(std::true_type{}, std::false_type{});
   }
   if (!live) return;
+  const int col = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) l[n] = row_sum(l[n]);
   if constexpr (WHOLE) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       bf16_t* op = s_op[32 * wv + 16 * n + col];
       if (!op) continue;
-      const float l = acc[n][NC][0], inv = l == 0.f ? 0.f : 1.f / l;
+      const float inv = l[n] == 0.f ? 0.f : 1.f / l[n];
 #pragma unroll
       for (int c = 0; c < NC; ++c)
         *reinterpret_cast<u32x2*>(op + 4 * g + 16 * c) =
@@ -677,7 +704,7 @@ __device__ __forceinline__ void by_rows(const Args& p, F part, char* smem) {
     for (int c = 0; c < NC; ++c) *reinterpret_cast<f32x4*>(p.po + at * D + 16 * c + 4 * g) = acc[n][c];
     if (g == 0) {
       p.pml[2 * at] = m[n];
-      p.pml[2 * at + 1] = acc[n][NC][0];
+      p.pml[2 * at + 1] = l[n];
     }
   }
 }
@@ -828,11 +855,12 @@ Plan make_plan(int B, int T, int G, int Hkv, int P, int max_len) {
   // Prompts: with a workgroup for every CU, both parts by rows in one launch where that costs less. In row-keys: by rows, 128-row
   // tiles over prefix and own keys; split, prefix tiles filled from all sequences, own keys in 32-row tiles at half that rate,
   // and partials worth 1100 keys a row; up to 32 rows go by keys. Measured (64 sequences, 32/8 heads of 128; split, by rows): 16 tokens behind 2048 + 500 own
-  // 81, 100 us; 24: 119, 111; 48: 231, 194; 33 tokens behind 8192 458, 566; 9 tokens, no prefix, 1000 own 80, 51; 8 tokens 45, 47.
+  // 101, 108 us; 24: 136, 110; 48: 260, 217; 33 tokens behind 8192 570, 618; 60: 793, 757; 9 tokens, no prefix, 1000 own 81, 51; where it errs
+  // the two are close (9 tokens, 500 + 1000: it splits, 84, 72).
   const int64_t tg = (int64_t)T * G, rt = cdiv(tg, tile_rows(kByRows)), seen = std::max(max_len - T / 2, 0);
   q.whole = tg > 32 && B * Hkv * rt >= 256 && 128 * rt * (P + seen) <= tg * (P + (int64_t)1100) + 64 * cdiv(tg, 32) * seen;
   // Otherwise own keys go by keys, also where 32-row tiles read them more than once: by rows (64 x 16 tokens, 8192 + 1000 keys) 313
-  // us against 230.
+  // us against 256.
   q.om = q.whole ? kByRows : std::min(2, mode_of(tg));
   q.pm = P > 0 ? mode_of(rows) : q.om;
   q.rtp = P > 0 ? cdiv(rows, tile_rows(q.pm)) : 0;
@@ -856,8 +884,8 @@ Plan make_plan(int B, int T, int G, int Hkv, int P, int max_len) {
     return q;
   }
   // One workgroup per CU for each part: half as many leave CUs without work, more write and fold more partials (64 x 5 tokens
-  // behind 8192 keys, prefix workgroups wanted 128, 256, 512, 1024: 193, 100, 113, 123 us; 16 x 8 tokens behind 4000: 58, 41, 46,
-  // 55; for the own keys all within 4 %).
+  // behind 8192 keys, 1000 own, prefix workgroups wanted 128, 256, 512, 1024: 237, 114, 122, 127 us; 16 x 8 tokens behind 4000: 41,
+  // 32, 41, 40; for the own keys all within 3 %, for one token behind 8192 with 8 sequences 29, 26, 30, 32).
   q.np = ranges(P, (int64_t)Hkv * q.rtp, 256, q.pm == kByRows ? 256 : 128, q.pchunk);
   q.ns = ranges(max_len, (int64_t)B * Hkv * q.rto, 256, 128, q.ochunk);
   return q;

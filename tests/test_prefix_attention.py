@@ -322,3 +322,45 @@ def test_captured_call_replays_and_another_stream(B, T, P):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, eager)
+
+
+FORMS = [pytest.param("cuda", *f, marks=pytest.mark.gpu) for f in (
+    (4, 1, 4, 2, 64, 500, 60), (4, 8, 4, 2, 128, 128, 40),          # one launch, 16 and 32 rows by keys
+    (64, 1, 32, 8, 128, 2048, 300), (4, 5, 8, 2, 64, 3000, 900),    # ranges: prefix by rows, own keys of 16 and 32 rows by keys
+    (4, 1, 16, 4, 128, 3000, 900), (1, 2, 16, 1, 64, 3000, 900),    # ranges: both by keys
+    (64, 24, 8, 2, 64, 130, 90), (22, 50, 20, 4, 128, 64, 70))]     # prompts by rows
+FORMS += [("cpu", 4, 1, 4, 2, 64, 500, 60), ("cpu", 2, 8, 4, 2, 128, 128, 40)]
+
+
+@pytest.mark.parametrize("dev,B,T,Hq,Hkv,D,P,own", FORMS)
+def test_weights_lose_nothing_to_the_operands_type(dev, B, T, Hq, Hkv, D, P, own):
+    """A softmax over six keys (the others' scores are too low to count): what the result may be off by, besides the output's one
+    rounding, is the scores' and sums' fp32 and 2^-16 of each weight, not the 2^-8 of a weight in bf16.
+
+    Tolerance, with A = sum_j p_j |v_j| over the six: a weight as a bf16 value and its remainder is off by at most 2^-8 2^-8, in
+    the product with V and in the sum: 2^-16 (A + |o|). A score is off by ((D + 4) sum |q||k| scale + 4 |s|) 2^-24 and the
+    exponential by 2^-22, e relative together; sums of six terms, in up to 32 parts, add 40 2^-24: (e + 40 2^-24) (A + |o|).
+    The other keys' scores are 45 below or lower: 4000 e^-45 < 2^-50. The output's rounding: 2^-8 of what is rounded."""
+    qkv, kp, vp, kc, vc = make(B, T, Hq, Hkv, D, P, own + 3, dev, seed=P)
+    q = qkv[:, : Hq * D].view(B * T, Hq, D)
+    q[:, :, 0] = 8.0
+    near = [(kp, [1, 20, P - 1]), (kc, [0, 1, own - T])]  # what every token sees; two at least of a key range each
+    for k, at in near:
+        rows = k[..., at, :].clone()
+        rows[..., 0] = 0.0
+        k.zero_()
+        k[..., 0] = -8.0 * math.sqrt(D)  # a score of -64
+        k[..., at, :] = rows
+    lens = torch.full((B,), own, dtype=torch.int32, device=dev)
+    got = kf.prefix_attention(qkv[:, : Hq * D], kp, vp, kc, vc, lens, own, T).double().view(B, T, Hq, D)
+    pick = lambda p, c: torch.cat([p[:, near[0][1]].expand(B, Hkv, 3, D), c[:, :, near[1][1]]], 2).double().repeat_interleave(Hq // Hkv, 1)  # noqa: E731
+    k, v, q = pick(kp, kc), pick(vp, vc), q.double().view(B, T, Hq, D).transpose(1, 2)  # [B, Hq, 6 or T, D]
+    s = (k.unsqueeze(2) * q.unsqueeze(3)).sum(-1) / math.sqrt(D)  # [B, Hq, T, 6]
+    mag = (k.abs().unsqueeze(2) * q.abs().unsqueeze(3)).sum(-1) / math.sqrt(D)
+    p = torch.softmax(s, -1).unsqueeze(-1)
+    o, A = (p * v.unsqueeze(2)).sum(3), (p * v.abs().unsqueeze(2)).sum(3)
+    e = ((D + 4) * mag.amax(-1) + 4 * s.abs().amax(-1)) * U + 2.0 ** -22 + 40 * U
+    tol = (2.0 ** -16 + e.unsqueeze(-1)) * (A + o.abs())
+    tol = tol + 2.0 ** -8 * (o.abs() + tol)
+    err = (got.transpose(1, 2) - o).abs()
+    assert (err <= tol).all(), float((err / tol).max())
