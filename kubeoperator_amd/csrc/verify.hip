@@ -206,26 +206,25 @@ __global__ void __launch_bounds__(kT) verify_stats_kernel(Args a) {
   m = wave_max(m);
   if ((t & 63) == 0) s_m[t >> 6] = m;
   __syncthreads();
-  m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  m = fminf(fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3])), FLT_MAX);
   const int64_t o = ((int64_t)b * (2 * a.T + 1) + r) * a.nch + c;
   if constexpr (GREEDY) {
-    int at = 0x7fffffff;  // the lowest index that holds the maximum
-    if (mine == m && m > -INFINITY) {
+    int at = 0x7fffffff;  // the lowest index that holds the maximum, +inf being the largest finite value
+    if (mine >= m && m > -INFINITY) {
 #pragma unroll
       for (int k = NV - 1; k >= 0; --k)
 #pragma unroll
         for (int e = N - 1; e >= 0; --e)
-          if (v[k].get(e) == m) at = lo + (k * kT + t) * N + e;
+          if (v[k].get(e) >= m) at = lo + (k * kT + t) * N + e;
     }
     at = wave_min_i(at);
     if ((t & 63) == 0) s_s[t >> 6] = (double)at;
     __syncthreads();
     if (t == 0) {
-      a.pm[o] = fminf(m, FLT_MAX);
+      a.pm[o] = m;
       a.ps[o] = fmin(fmin(s_s[0], s_s[1]), fmin(s_s[2], s_s[3]));
     }
   } else {
-    m = fminf(m, FLT_MAX);
     double s = 0.0;
     if (m > -INFINITY) {
 #pragma unroll
@@ -506,7 +505,7 @@ __global__ void __launch_bounds__(kT) verify_small_kernel(Args a) {
       v.load(x, i, a.V);
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        const float z = v.get(e);
+        const float z = v.get(e) > FLT_MAX ? FLT_MAX : v.get(e);  // (NaN stays, and is passed over)
         at = z > m ? i + e : at;
         m = fmaxf(m, z);
       }
@@ -518,7 +517,6 @@ __global__ void __launch_bounds__(kT) verify_small_kernel(Args a) {
       at = wave_min_i(mine == m ? at : 0x7fffffff);
       s = m > -INFINITY ? (double)at : -1.0;
     } else {
-      m = fminf(m, FLT_MAX);
       if (m > -INFINITY)
         for (int i = lane * N; i < a.V; i += 64 * N) {
           Vec<E> v;

@@ -219,3 +219,15 @@ def test_captured_call_replays_and_another_stream(temp):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got[0], eager[0]) and torch.equal(got[1], eager[1])
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V,low,high", [(40, 3, 7), (40, 7, 3), (5000, 3, 7), (5000, 7, 3), (20000, 3, 7), (20000, 7, 3), (20000, 3, 9000)])
+def test_infinity_counts_as_the_largest_value(dev, dtype, V, low, high):
+    """+inf and the largest fp32 value are a tie, greedy (the lower index) and sampled (half each); bf16 has no such value."""
+    t, d, k, u = make(4, 2, V, dev, dtype)
+    t[:, :, low], t[:, :, high] = FMAX if dtype == torch.float32 else torch.finfo(dtype).max, float("inf")
+    k[0], k[1], k[2] = min(low, high), max(low, high), torch.tensor([low, high])
+    check(t, d, k, u, 0.0)
+    check(t, d, k, u, 1.0)
