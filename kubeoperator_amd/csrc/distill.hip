@@ -7,6 +7,11 @@
 //   dlogits = t w_i (q - scatter(p))           (d loss_i / d logits; the t^2 keeps its size independent of t)
 // An entry whose index is outside [0, V) or whose teacher logit is -inf or NaN is padding (p_k = 0); a row of padding
 // has p = 0: loss 0 and gradient 0, as has a row of weight 0. Sums and statistics are fp32.
+//
+// q_i = 2^((x_i - m) c) / s with c = log2 e / t, m the row's maximum and s the sum of those powers; log2 q_i = (x_i - m) c - log2 s. The
+// maximum is subtracted before anything is scaled and never joined to the sum: m c + log2 s as one fp32 number is off by half a
+// step of m c, which at low temperatures is percents of q (m = 50: 0.8 % at t = 1e-3), and overflows where logits are masked with
+// the type's lowest value.
 #include "common.h"
 #include "kernels.h"
 
@@ -54,8 +59,8 @@ struct Teacher {
     }
     return block_max<NT / 64>(m, red);
   }
-  // p = softmax; returns the loss in units of log2 without its factors. lse2: log2 of the student's sum, c = log2 e / temp
-  __device__ __forceinline__ float finish(int K, float tm, float c, float lse2, bool some) {
+  // p = softmax; returns the loss in units of log2 without its factors. m, ls2: the student's maximum and log2 of its sum
+  __device__ __forceinline__ float finish(int K, float tm, float c, float m, float ls2, bool some) {
     float s = 0.f;
     for (int k = threadIdx.x; k < K; k += NT) s += idx[k] >= 0 ? __builtin_amdgcn_exp2f((p[k] - tm) * c) : 0.f;
     __syncthreads();  // red may still be read
@@ -66,14 +71,14 @@ struct Teacher {
       const float lp = (p[k] - tm) * c - ls;
       const float e = idx[k] >= 0 ? __builtin_amdgcn_exp2f(lp) : 0.f;
       p[k] = e;
-      if (e > 0.f) part += e * (lp - (some ? fmaf(x[k], c, -lse2) : -INFINITY));
+      if (e > 0.f) part += e * (lp - (some ? (x[k] - m) * c - ls2 : -INFINITY));
     }
     __syncthreads();
     return block_sum<NT / 64>(part, red);
   }
   // the listed tokens' own elements, once every element of the row has been written. A token listed more than once: its
-  // entries' sum, written by the first of them
-  __device__ __forceinline__ void patch(int K, float c, float lse2, float gw, bf16_t* gx) {
+  // entries' sum, written by the first of them. inv: 1 / the student's sum
+  __device__ __forceinline__ void patch(int K, float c, float m, float inv, float gw, bf16_t* gx) {
     __syncthreads();
     for (int k = threadIdx.x; k < K; k += NT) {
       const int i = idx[k];
@@ -86,7 +91,7 @@ struct Teacher {
         sum += same ? p[j] : 0.f;
         first = first && !(same && j < k);
       }
-      if (first) gx[i] = f2bf(gw * (__builtin_amdgcn_exp2f(fmaf(x[k], c, -lse2)) - sum));
+      if (first) gx[i] = f2bf(gw * (__builtin_amdgcn_exp2f((x[k] - m) * c) * inv - sum));
     }
   }
 };
@@ -177,40 +182,40 @@ __global__ void __launch_bounds__(NT, NT >= 512 && CR + CL > 16 ? 4 : 1) distill
   __syncthreads();
   m = block_max<NT / 64>(m, s_t.red);
   const bool some = m > -INFINITY;  // false: every logit is -inf, q = 0
-  const float nb = some ? -m * c : 0.f;
+  m = some ? m : 0.f;
   repack<CR>(v);
-  float s = __builtin_amdgcn_exp2f(fmaf(xt, c, nb));
+  float s = __builtin_amdgcn_exp2f((xt - m) * c);
 #pragma unroll 1
   for (int j = 0; j < CL; ++j) {
     unpack8(s_w[j * NT + t], f);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s += __builtin_amdgcn_exp2f(fmaf(f[e], c, nb));
+    for (int e = 0; e < 8; ++e) s += __builtin_amdgcn_exp2f((f[e] - m) * c);
   }
 #pragma unroll
   for (int j = 0; j < CR; ++j) {
     unpack8(v[j], f);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s += __builtin_amdgcn_exp2f(fmaf(f[e], c, nb));
+    for (int e = 0; e < 8; ++e) s += __builtin_amdgcn_exp2f((f[e] - m) * c);
   }
   __syncthreads();
   s = block_sum<NT / 64>(s, s_t.red);
-  const float lse2 = some ? fmaf(m, c, __log2f(s)) : INFINITY;  // log2 of the student's sum of exp(logit / t)
-  const float part = s_t.finish(a.K, tm, c, lse2, some);
+  const float inv = some ? 1.f / s : 0.f;
+  const float part = s_t.finish(a.K, tm, c, m, __log2f(s), some);
   if (t == 0) a.loss[row] = part * kLn2 * a.temp * a.temp * w;
-  const float gw = a.temp * w;
+  const float gw = a.temp * w, gq = gw * inv;
   repack<CR>(v);
   auto put = [&](u32x4 q, uint32_t i) {
     unpack8(q, f);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = gw * __builtin_amdgcn_exp2f(fmaf(f[e], c, -lse2));
+    for (int e = 0; e < 8; ++e) f[e] = gq * __builtin_amdgcn_exp2f((f[e] - m) * c);
     if (i < V8) store8(gx, i, f);
   };
 #pragma unroll
   for (int j = 0; j < CR; ++j) put(v[j], (j * NT + t) * 8);
 #pragma unroll 1
   for (int j = 0; j < CL; ++j) put(s_w[j * NT + t], ((CR + j) * NT + t) * 8);
-  if (tail) gx[V8 + t] = f2bf(gw * __builtin_amdgcn_exp2f(fmaf(xt, c, -lse2)));
-  s_t.patch(a.K, c, lse2, gw, gx);
+  if (tail) gx[V8 + t] = f2bf(gq * __builtin_amdgcn_exp2f((xt - m) * c));
+  s_t.patch(a.K, c, m, inv, gw, gx);
 }
 
 // Rows longer than that: two passes, running (maximum, sum) in the log2 domain, then the gradient. Bound by memory, with the
@@ -237,30 +242,30 @@ __global__ void __launch_bounds__(NT) distill_long_kernel(Args a) {
     unpack8(load8(x, i), f);
     const float nm = fmaxf(m, max8(f));
     if (nm == -INFINITY) continue;
-    const float nb = -nm * c;
     float add = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) add += __builtin_amdgcn_exp2f(fmaf(f[e], c, nb));
+    for (int e = 0; e < 8; ++e) add += __builtin_amdgcn_exp2f((f[e] - nm) * c);
     s = s * __builtin_amdgcn_exp2f((m - nm) * c) + add;  // m = -inf: times 0
     m = nm;
   }
   __syncthreads();
-  const float M = block_max<NT / 64>(m, s_t.red);
+  float M = block_max<NT / 64>(m, s_t.red);
   __syncthreads();
   s = block_sum<NT / 64>(m == -INFINITY ? 0.f : s * __builtin_amdgcn_exp2f((m - M) * c), s_t.red);
   const bool some = M > -INFINITY;
-  const float lse2 = some ? fmaf(M, c, __log2f(s)) : INFINITY;
-  const float part = s_t.finish(a.K, tm, c, lse2, some);
+  M = some ? M : 0.f;
+  const float inv = some ? 1.f / s : 0.f;
+  const float part = s_t.finish(a.K, tm, c, M, __log2f(s), some);
   if (t == 0) a.loss[row] = part * kLn2 * a.temp * a.temp * w;
-  const float gw = a.temp * w;
+  const float gw = a.temp * w, gq = gw * inv;
   for (uint32_t i = t * 8; i < V8; i += NT * 8) {
     unpack8(load8(x, i), f);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = gw * __builtin_amdgcn_exp2f(fmaf(f[e], c, -lse2));
+    for (int e = 0; e < 8; ++e) f[e] = gq * __builtin_amdgcn_exp2f((f[e] - M) * c);
     store8(gx, i, f);
   }
-  if (tail) gx[V8 + t] = f2bf(gw * __builtin_amdgcn_exp2f(fmaf(xt, c, -lse2)));
-  s_t.patch(a.K, c, lse2, gw, gx);
+  if (tail) gx[V8 + t] = f2bf(gq * __builtin_amdgcn_exp2f((xt - M) * c));
+  s_t.patch(a.K, c, M, inv, gw, gx);
 }
 }  // namespace
 

@@ -261,12 +261,14 @@ def distill_topk_ref(logits, index, teacher, temperature, weight=None, out=None)
     at = torch.where(real, index, 0).long()
     lp = torch.log_softmax(torch.where(real, teacher, float("-inf")) / temperature, -1)
     p = torch.where(real & live.unsqueeze(1), torch.exp(lp), 0.0)
-    z = logits.float() / temperature
-    lse = torch.logsumexp(z, -1, keepdim=True)
-    lse = torch.where(lse == float("-inf"), float("inf"), lse)  # no student probability anywhere: q = 0
-    lq = z.gather(-1, at) - lse
+    m = logits.float().amax(-1, keepdim=True)
+    some = m > float("-inf")  # false: no student probability anywhere, q = 0
+    z = (logits.float() - torch.where(some, m, 0.0)) / temperature  # the maximum goes first: m / t takes z's low bits with it
+    e = torch.exp(z)
+    s = torch.where(some, e.sum(-1, keepdim=True), float("inf"))
+    lq = z.gather(-1, at) - torch.log(s)
     loss = torch.where(p > 0, p * (lp - lq), 0.0).sum(-1) * temperature * temperature * w
-    grad = torch.exp(z - lse).scatter_add(-1, at, -p) * (temperature * w).unsqueeze(1)
+    grad = (e / s).scatter_add(-1, at, -p) * (temperature * w).unsqueeze(1)
     loss = torch.where(live, loss, 0.0)
     grad = torch.where(live.unsqueeze(1), grad, 0.0).to(logits.dtype)
     return loss, grad if out is None else out.copy_(grad)

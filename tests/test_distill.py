@@ -8,6 +8,8 @@ c = max(64, n / 512) plus a 16-step tree (c + 16) u relative -- all terms are po
 E = (3 R ln 2 + c + 24) u relative, log q and log p by E plus 2 R u absolute, and the loss by
 t^2 w sum_k p_k (E |log p_k - log q_k| + 2 E + 4 R u) + (K + 16) u |terms|; the gradient by t w (q + P) E and its
 rounding to bf16, 2^-8 of itself."""
+import math
+
 import pytest
 import torch
 
@@ -250,3 +252,62 @@ def test_captured_call_replays_and_another_stream(V):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got[0], eager[0]) and torch.equal(got[1], eager[1])
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("V", [40, 2055, 50304, 65545, 300001])
+@pytest.mark.parametrize("t", [1e-2, 1e-4])
+@pytest.mark.parametrize("offset", [0.0, 50.0, -50.0])
+def test_low_temperatures(dev, V, t, offset):
+    """What the student's logits have in common, and how large it is next to the temperature, takes nothing from the result: only
+    differences from the row's maximum enter.
+
+    Tolerance: such a difference d, over t, carries 5 roundings (the difference, t, 1 / t, log2 e, the product); where it counts (a
+    weight of 2^-24 of the row's and more) it is at most 24 ln 2 + ln V, so q is off by E = 5 (24 ln 2 + ln V) u, 2 u of the
+    exponential and c + 16 of the sum, relative, q smaller than 2^-24 by 2^-24 altogether; P likewise with T's differences (at
+    most 40 ln 2 before its weight is nothing); log q_k by 5 u |log q_k| + E. Logits a step of bf16 apart (0.25 at 50) are far
+    apart in units of t: the rows get pairs of equal maxima, so that q is not all 0 and 1."""
+    N, K = 6, 9
+    logits, index, teacher, weight = make(N, V, K, dev, seed=7)
+    logits += offset
+    teacher = teacher * t  # the teacher's own distribution keeps its shape
+    top = logits.float().argmax(-1)
+    for i in range(N):
+        for j in range(i):  # rows with 1 + i maxima, some of them listed
+            logits[i, (int(top[i]) + 3 * j + 1) % V] = logits[i, int(top[i])]
+        index[i, 0] = int(top[i])
+        index[i, 1] = (int(top[i]) + 1) % V
+    loss, grad = kf.distill_topk(logits, index, teacher, t, weight)
+    z, T, w = logits.double().cpu() / t, teacher.double().cpu() / t, weight.double().cpu()
+    c = max(64, V / 512)
+    E = (5 * (24 * 0.7 + math.log(V)) + 2 + c + 16) * U
+    EP = (5 * 40 * 0.7 + 2 + K + 16) * U
+    lq, lp = torch.log_softmax(z, -1), torch.log_softmax(T, -1)
+    q, P = lq.exp(), torch.zeros_like(z).scatter_add_(1, index.cpu().long(), lp.exp())
+    g = (q - P) * (t * w).unsqueeze(1)
+    slack = (E * q + 2.0 ** -24 * (q < 2.0 ** -24) + EP * P) * (t * w).unsqueeze(1)
+    err = (grad.double().cpu() - g).abs() - (2.0 ** -8 * (g.abs() + slack) + slack + 2.0 ** -133)
+    assert err.max() <= 0, float(err.max())
+    k = lq.gather(1, index.cpu().long())
+    want = t * t * w * (lp.exp() * (lp - k)).sum(-1)
+    tol = t * t * w * (lp.exp() * (EP * (lp - k).abs() + 5 * U * k.abs() + E + EP + 5 * U * lp.abs())).sum(-1)
+    tol += (K + 16) * U * t * t * w * (lp.exp() * (lp - k).abs()).sum(-1)
+    assert ((loss.double().cpu() - want).abs() <= tol).all(), ((loss.double().cpu() - want).abs() / tol).max()
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("V", [40, 4099, 300001])
+@pytest.mark.parametrize("t", [0.5, 1.0])
+def test_rows_of_the_lowest_value(dev, V, t):
+    """Logits at the type's lowest value (a mask) are finite: a row of nothing else is uniform, beside others they weigh nothing."""
+    logits, index, teacher, _ = make(3, V, 5, dev)
+    logits[0] = torch.finfo(torch.bfloat16).min
+    logits[1, : V // 2] = torch.finfo(torch.bfloat16).min
+    index[1] = torch.arange(V - 5, V, dtype=torch.int32)
+    logits[2] = torch.finfo(torch.bfloat16).max
+    got = kf.distill_topk(logits, index, teacher, t)
+    logits[0] = 0.0
+    logits[1, : V // 2] = float("-inf")
+    logits[2] = 0.0
+    want = kf.distill_topk(logits, index, teacher, t)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
