@@ -405,10 +405,11 @@ class LlamaGenerator:
         return self._graphs[key]
 
     @torch.no_grad()
-    def generate(self, ids: torch.Tensor, max_new_tokens: int) -> torch.Tensor:
-        """Greedy continuation: [B, S] prompt -> [B, S + max_new_tokens] tokens."""
+    def generate(self, ids: torch.Tensor, max_new_tokens: int, adapters: list | None = None) -> torch.Tensor:
+        """Greedy continuation: [B, S] prompt -> [B, S + max_new_tokens] tokens. ``adapters`` as in ``prefill``: each
+        sequence's index, default none."""
         out = [ids]
-        logits = self.prefill(ids)
+        logits = self.prefill(ids, adapters=adapters)
         for _ in range(max_new_tokens):
             nxt = logits.argmax(-1)
             out.append(nxt.unsqueeze(1).to(ids.dtype))
@@ -419,11 +420,12 @@ class LlamaGenerator:
 
     @torch.no_grad()
     def speculate(self, draft: "LlamaGenerator", ids: torch.Tensor, max_new_tokens: int, drafts: int = 4,
-                  temperature: float = 0.0, generator: torch.Generator | None = None):
+                  temperature: float = 0.0, generator: torch.Generator | None = None, adapters: list | None = None):
         """Continuation of ``ids`` [B, S] through a small draft model: it proposes ``drafts`` tokens per round, one ``extend`` of
         this model scores them all, and ``ops.verify_draft`` keeps the first ones and draws the token after them. With
         ``temperature`` 0 the result is this model's greedy continuation, otherwise it is distributed as this model's
-        samples (uniform numbers from ``generator``). Returns ([B, S + max_new_tokens] tokens, kept drafts per round)."""
+        samples (uniform numbers from ``generator``). ``adapters`` as in ``prefill``: each sequence's index into this model's
+        adapters, default none; the draft proposes without any. Returns ([B, S + max_new_tokens] tokens, kept drafts per round)."""
         B, S = ids.shape
         if draft.cfg.vocab_size != self.cfg.vocab_size or not 1 <= drafts <= 32 or max_new_tokens < 1:
             raise ValueError("the draft needs this model's vocabulary; 1 to 32 drafts per round")
@@ -447,7 +449,7 @@ class LlamaGenerator:
                 raise RuntimeError("a row of the model's logits gives no token any probability")
             return tokens
 
-        cur = sample(self.prefill(ids))
+        cur = sample(self.prefill(ids, adapters=adapters))
         draft.prefill(ids)
         out = [[t] for t in checked(cur.tolist())]
         rounds = []

@@ -284,3 +284,42 @@ def test_adapter_refusals():
     for i, x, y in ((2, a[0], b[0]), (0, a[0, :8], b[0]), (0, a[0, :, :64], b[0]), (-1, a[0], b[0])):
         with pytest.raises(ValueError):
             ad.set(i, 0, "wo", x, y)
+
+
+def is_greedy(dev, gen, ids, got, n, adapters=None):
+    """Every one of the n tokens behind ``ids`` is the best one after those before it, up to the rounding of two paths on the GPU."""
+    S = ids.shape[1]
+    logits = gen.prefill(ids, adapters=adapters)
+    for t in range(n):
+        top = logits.max(-1).values - logits.gather(1, got[:, S + t].unsqueeze(1)).squeeze(1)
+        assert (top <= (0.0 if dev == "cpu" else 3e-2) * logits.abs().max()).all(), (t, top)
+        logits = gen.decode(got[:, S + t])
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("graph", [False, True])
+def test_speculation_and_generation_with_an_adapter_per_request(dev, graph):
+    """Requests bring adapters and speculate together: the tokens are those of step-by-step decoding with the same adapters, a
+    captured draft (and target) included, and not the base model's."""
+    m = model(dev, size=0.08)
+    ad, which = adapters(m, 3, 16), [2, -1, 0]
+    ids, n = ids_of(m, 3, 11), 10
+    new = lambda g: LlamaGenerator(m, max_batch=3, max_seq=40, graph=g)  # noqa: E731
+    gen, draft, steps = new(graph), new(graph), new(False)
+    for g in (gen, steps):
+        g.set_adapters(ad)
+    for _ in range(2):  # the second time on captured graphs
+        got, _ = gen.speculate(draft, ids, n, drafts=3, adapters=which)
+        assert gen.slot_adapter.tolist() == which
+        is_greedy(dev, steps, ids, got, n, which)
+    got = gen.generate(ids, n, adapters=which)
+    is_greedy(dev, steps, ids, got, n, which)
+    base, _ = gen.speculate(draft, ids, n, drafts=3)  # none named: none
+    is_greedy(dev, new(False), ids, base, n)
+    assert not torch.equal(base[0], got[0])
+    with pytest.raises(ValueError):
+        gen.speculate(draft, ids, n, adapters=[0, 1])
+    with pytest.raises(ValueError):
+        gen.generate(ids, n, adapters=[0, 1, 3])
+    with pytest.raises(ValueError):
+        draft.generate(ids, n, adapters=which)
