@@ -444,14 +444,22 @@ class LlamaGenerator:
             none = torch.empty(B, 0, dtype=torch.long, device=self.device)
             return kf.verify_draft(logits.unsqueeze(1), None, none, uniform(B, 1), temperature)[0][:, 0]
 
-        def checked(tokens: list):
-            if min(tokens) < 0:
-                raise RuntimeError("a row of the model's logits gives no token any probability")
-            return tokens
+        out: list = [[] for _ in range(B)]
+
+        def add(new: list, last: torch.Tensor):
+            """Each unfinished sequence's new tokens into ``out``; the tokens that the next round starts with (a finished sequence
+            computes rows that are thrown away: any token will do)."""
+            for o, more in zip(out, new):
+                if len(o) >= max_new_tokens:
+                    continue
+                o += more
+                if o[:max_new_tokens][-1] < 0:
+                    raise RuntimeError("a row of the model's logits gives no token any probability")
+            return last.clamp(min=0)
 
         cur = sample(self.prefill(ids, adapters=adapters))
         draft.prefill(ids)
-        out = [[t] for t in checked(cur.tolist())]
+        cur = add([[t] for t in cur.tolist()], cur)
         rounds = []
         while min(len(o) for o in out) < max_new_tokens:
             start = list(self.cache.host_lens[:B])
@@ -465,12 +473,10 @@ class LlamaGenerator:
             proposed = torch.stack(toks, 1)
             p = self.extend(torch.cat([cur.unsqueeze(1), proposed.clamp(min=0)], 1))
             new, kept = kf.verify_draft(p, torch.stack(qs, 1), proposed, uniform(B, drafts + 1), temperature)
-            cur = new.gather(1, kept.long().unsqueeze(1)).squeeze(1)
-            checked(cur.tolist())
-            new, kept = new.tolist(), kept.tolist()
+            last = new.gather(1, kept.long().unsqueeze(1)).squeeze(1)
+            kept = kept.tolist()
             rounds.append(kept)
-            for b in range(B):
-                out[b] += new[b][: kept[b] + 1]
+            cur = add([row[: k + 1] for row, k in zip(new.tolist(), kept)], last)
             # a finished sequence stays where it was before these drafts: it goes on computing rows that are thrown away
             lens = [n if len(o) >= max_new_tokens else n + k + 1 for n, k, o in zip(start, kept, out)]
             for g in (self, draft):

@@ -323,3 +323,30 @@ def test_speculation_and_generation_with_an_adapter_per_request(dev, graph):
         gen.generate(ids, n, adapters=[0, 1, 3])
     with pytest.raises(ValueError):
         draft.generate(ids, n, adapters=which)
+
+
+def test_a_finished_sequence_cannot_stop_the_others(monkeypatch):
+    """A row that has all its tokens goes on computing rows that are thrown away: one without any probability there (-1), or right
+    behind the last token, is not an error, and no -1 reaches the embedding."""
+    from kubeoperator_amd.serve import generate
+
+    m = model("cpu")
+    gen, draft = (LlamaGenerator(m, max_batch=2, max_seq=40) for _ in range(2))
+    ids, n, verify, calls = ids_of(m, 2, 10), 8, kf.verify_draft, []
+
+    def stub(target, d, tokens, u, temperature=1.0, n_draft=None):
+        """Checks of drafts: row 0 keeps all three, row 1 none; row 0 finds no token behind its eighth (the second round)
+        and later."""
+        if tokens.shape[1] == 0:
+            return verify(target, d, tokens, u, temperature, n_draft)
+        calls.append(0)
+        best = target.argmax(-1)
+        out = torch.full((2, 4), -1)
+        out[0, :3], out[0, 3], out[1, 0] = tokens[0], best[0, 3] if len(calls) < 2 else -1, best[1, 0]
+        return out, torch.tensor([3, 0], dtype=torch.int32)
+
+    monkeypatch.setattr(generate.kf, "verify_draft", stub)
+    out, rounds = gen.speculate(draft, ids, n, drafts=3)
+    assert len(rounds) == 7 and ((out >= 0) & (out < m.cfg.vocab_size)).all()
+    monkeypatch.undo()
+    is_greedy("cpu", LlamaGenerator(m, 2, 40), ids, out, n)
