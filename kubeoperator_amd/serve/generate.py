@@ -425,7 +425,8 @@ class LlamaGenerator:
         this model scores them all, and ``ops.verify_draft`` keeps the first ones and draws the token after them. With
         ``temperature`` 0 the result is this model's greedy continuation, otherwise it is distributed as this model's
         samples (uniform numbers from ``generator``). ``adapters`` as in ``prefill``: each sequence's index into this model's
-        adapters, default none; the draft proposes without any. Returns ([B, S + max_new_tokens] tokens, kept drafts per round)."""
+        adapters, default none; the draft proposes without any. Returns ([B, S + max_new_tokens] tokens, kept drafts per round);
+        both caches then hold all of them but the last, as after ``generate``."""
         B, S = ids.shape
         if draft.cfg.vocab_size != self.cfg.vocab_size or not 1 <= drafts <= 32 or max_new_tokens < 1:
             raise ValueError("the draft needs this model's vocabulary; 1 to 32 drafts per round")
@@ -433,7 +434,7 @@ class LlamaGenerator:
             raise ValueError("the draft needs a generator (a cache) of its own")
         if draft.prefix_len != self.prefix_len:
             raise ValueError("give the draft the same prefix")
-        for g in (self, draft):  # the last round may start one token before the end and brings drafts + 1
+        for g in (self, draft):  # a finished sequence, all but its last token cached, goes through rounds of drafts + 1 more
             if B > g.cache.batch or S + max_new_tokens + drafts > g.cache.max_seq:
                 raise ValueError("KV cache too small for the continuation and one round of drafts")
 
@@ -462,7 +463,7 @@ class LlamaGenerator:
         cur = add([[t] for t in cur.tolist()], cur)
         rounds = []
         while min(len(o) for o in out) < max_new_tokens:
-            start = list(self.cache.host_lens[:B])
+            start = self.cache.host_lens[:B]
             tok, toks, qs = cur, [], []
             for _ in range(drafts):
                 q = draft.decode(tok)
@@ -477,8 +478,8 @@ class LlamaGenerator:
             kept = kept.tolist()
             rounds.append(kept)
             cur = add([row[: k + 1] for row, k in zip(new.tolist(), kept)], last)
-            # a finished sequence stays where it was before these drafts: it goes on computing rows that are thrown away
-            lens = [n if len(o) >= max_new_tokens else n + k + 1 for n, k, o in zip(start, kept, out)]
+            # everything but the last token; a finished sequence's rows from then on are thrown away
+            lens = [min(n + k + 1, S + max_new_tokens - 1) for n, k in zip(start, kept)]
             for g in (self, draft):
                 g.cache.truncate(lens)
         res = torch.tensor([o[:max_new_tokens] for o in out], dtype=ids.dtype, device=ids.device)

@@ -350,3 +350,28 @@ def test_a_finished_sequence_cannot_stop_the_others(monkeypatch):
     assert len(rounds) == 7 and ((out >= 0) & (out < m.cfg.vocab_size)).all()
     monkeypatch.undo()
     is_greedy("cpu", LlamaGenerator(m, 2, 40), ids, out, n)
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("n", [1, 2, 13])
+@pytest.mark.parametrize("prefix", [0, 30])
+def test_caches_after_speculation(dev, n, prefix):
+    """They hold what generate() leaves there, everything but the last token returned, for each sequence and in both models: decoding
+    goes on from it."""
+    m, other = model(dev, size=0.08), model(dev, size=0.08, seed=1)
+    with torch.no_grad():  # sequences that keep different numbers of drafts
+        for p, q in zip(other.parameters(), m.parameters()):
+            p.copy_(0.97 * q + 0.03 * p)
+    ids = ids_of(m, 3, 12)
+    new = lambda x: LlamaGenerator(x, max_batch=3, max_seq=40)  # noqa: E731
+    gens = [new(m), new(other)]
+    for g in gens:
+        if prefix:
+            g.set_prefix(ids_of(m, 1, prefix, seed=9)[0])
+    got, _ = gens[0].speculate(gens[1], ids, n, drafts=3)
+    for g, x in zip(gens, (m, other)):
+        assert g.cache.host_lens == [12 + n - 1] * 3 == g.cache.lens.tolist()
+        fresh = new(x)
+        if prefix:
+            fresh.set_prefix(ids_of(m, 1, prefix, seed=9)[0])
+        close(g.decode(got[:, -1]), fresh.prefill(got))
