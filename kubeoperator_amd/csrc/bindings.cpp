@@ -656,6 +656,7 @@ Tensor lora_add(const Tensor& y, const Tensor& x, const Tensor& a, const Tensor&
   check_same_device(scale, y, "scale");
   const int64_t M = x.size(0), K = x.size(1), N = y.size(1), n = a.size(0), r = a.size(1);
   TORCH_CHECK(y.size(0) == M && index.dim() == 1 && index.numel() == M, "lora_add: x, y and index disagree on the rows");
+  TORCH_CHECK(M <= kop::kLoraMaxRows, "lora_add: too many rows");
   TORCH_CHECK(a.size(2) == K && b.size(0) == n && b.size(1) == N && b.size(2) == r,
               "lora_add: a must be [n, r, K] and b [n, N, r]");
   TORCH_CHECK(scale.dim() == 1 && scale.numel() == n && scale.is_contiguous(), "lora_add: scale must be [n]");

@@ -59,8 +59,10 @@ int verify_draft(const void* target, int64_t ts_b, int64_t ts_t, const void* dra
 
 // lora.hip: out[i] = y[i] + scale[j] b[j] (a[j] x[i]) with j = index[i] (rows whose j is outside [0, n): out = y);
 // x [M, K], y / out [M, N] rows, a [n, r, K], b [n, N, r] contiguous, index [M] int32, scale [n] fp32.
-// workspace: lora_workspace() bytes. K, N, r multiples of 8, r <= kLoraMaxRank
+// workspace: lora_workspace() bytes. K, N, r multiples of 8, r <= kLoraMaxRank, M <= kLoraMaxRows (32 rows per workgroup of 256 in a
+// launch of less than 2^32 work-items; the kernels hold row numbers in 32 bits)
 constexpr int kLoraMaxRank = 128;
+constexpr int64_t kLoraMaxRows = 32 * ((int64_t(1) << 24) - 1);
 int64_t lora_workspace(int64_t M, int K, int N, int n, int r);
 int lora_add(const bf16_t* y, int64_t ys, const bf16_t* x, int64_t xs, const bf16_t* a, const bf16_t* b,
              const int* index, const float* scale, bf16_t* out, int64_t os, int64_t M, int K, int N, int n, int r,

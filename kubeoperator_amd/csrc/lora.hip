@@ -402,7 +402,7 @@ int lora_add(const bf16_t* y, int64_t ys, const bf16_t* x, int64_t xs, const bf1
              const int* index, const float* scale, bf16_t* out, int64_t os, int64_t M, int K, int N, int n, int r,
              void* workspace, hipStream_t stream) {
   if (K < 8 || K % 8 || N < 8 || N % 8 || r < 8 || r % 8 || r > kLoraMaxRank || n < 0 || M < 0 || xs % 8 || ys % 8 ||
-      os % 8 || (M + 31) / 32 > 0x7fffffff || (N + 255) / 256 > 65535)
+      os % 8 || M > kLoraMaxRows || (N + 255) / 256 > 65535)
     return -1;
   if (M == 0) return 0;
   const Plan p = make_plan(M, K, N, n, r);

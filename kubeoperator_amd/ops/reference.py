@@ -167,6 +167,7 @@ def lora_add_ref(y, x, a, b, index, scale, out=None):
     require(y.dim() == 2 and x.dim() == 2 and a.dim() == 3 and b.dim() == 3, "adapters must be contiguous a [n, r, K] and b [n, N, r]")
     n, r, K = a.shape
     require(x.shape == (y.shape[0], K) and index.shape == (y.shape[0],), "lora_add: x, y and index disagree on the rows")
+    require(y.shape[0] <= 32 * (2 ** 24 - 1), "lora_add: too many rows")
     require(b.shape == (n, y.shape[1], r), "lora_add: a must be [n, r, K] and b [n, N, r]")
     require(scale.shape == (n,) and scale.dtype == torch.float32, "lora_add: scale must be [n]")
     require(index.dtype == torch.int32, "index must be contiguous int32")

@@ -188,3 +188,14 @@ def test_captured_call_replays_and_another_stream(M):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, eager)
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("M", [2 ** 29, 2 ** 31 + 64])
+def test_more_rows_than_a_launch_can_have_are_refused(dev, M):
+    """Row numbers inside the kernels are 32 bits wide, and a launch has at most 2^32 work-items: refused before anything is allocated
+    or launched (rows that are all the same one, so that only the index list takes memory)."""
+    row, low = torch.zeros(1, 8, dtype=torch.bfloat16, device=dev), torch.zeros(1, 8, 8, dtype=torch.bfloat16, device=dev)
+    index = torch.empty(M, dtype=torch.int32, device=dev) if dev == "cuda" else torch.zeros(1, dtype=torch.int32).expand(M)
+    with pytest.raises(RuntimeError, match="too many rows"):
+        kf.lora_add(row.expand(M, 8), row.expand(M, 8), low, low, index, torch.ones(1, device=dev))
