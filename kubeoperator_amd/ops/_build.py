@@ -5,7 +5,8 @@ compiled by ``hipcc --offload-arch=gfx950`` (they include no PyTorch headers, so
 ``bindings.cpp`` is compiled once as host C++ against the PyTorch headers, and the objects are linked
 into one shared object next to the package so it travels with the source tree (``gpurun`` snapshots it).
 
-Incremental: an object is rebuilt only when its source or any ``csrc/*.h`` header is newer.
+Incremental: an object is rebuilt when its source or any ``csrc/*.h`` header is newer, or when it was made by another command
+line than today's (recorded beside it): flags that results depend on reach every object.
 """
 from __future__ import annotations
 
@@ -45,11 +46,25 @@ def _newest_header() -> float:
     return max((os.path.getmtime(h) for h in hs), default=0.0)
 
 
-def _needs(obj: str, src: str, hdr_mtime: float) -> bool:
-    if not os.path.exists(obj):
+def _command(cmd: list[str]) -> str:
+    """A compilation's command line, without the place of the tree: it may be moved or copied with its objects."""
+    return " ".join(cmd).replace(PKG_DIR, "")
+
+
+def _needs(obj: str, src: str, hdr_mtime: float, cmd: list[str]) -> bool:
+    if not os.path.exists(obj) or not os.path.exists(obj + ".cmd"):
         return True
+    with open(obj + ".cmd") as f:
+        if f.read() != _command(cmd):
+            return True
     m = os.path.getmtime(obj)
     return m < os.path.getmtime(src) or m < hdr_mtime
+
+
+def _compile(cmd: list[str]) -> None:
+    _run(cmd)
+    with open(cmd[cmd.index("-o") + 1] + ".cmd", "w") as f:
+        f.write(_command(cmd))
 
 
 def _run(cmd: list[str]) -> None:
@@ -86,26 +101,26 @@ def build(verbose: bool = False, jobs: int | None = None, force: bool = False) -
     for src in hip_srcs:
         obj = os.path.join(BUILD_DIR, os.path.basename(src) + ".o")
         objs.append(obj)
-        if force or _needs(obj, src, hdr):
-            jobs_list.append([hipcc, f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics",
-                              abi, *BASE_HIPFLAGS, *FILE_FLAGS.get(os.path.basename(src), []), *EXTRA_HIPFLAGS, "-I", CSRC, "-c", src,
-                              "-o", obj])
+        cmd = [hipcc, f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics", abi, *BASE_HIPFLAGS,
+               *FILE_FLAGS.get(os.path.basename(src), []), *EXTRA_HIPFLAGS, "-I", CSRC, "-c", src, "-o", obj]
+        if force or _needs(obj, src, hdr, cmd):
+            jobs_list.append(cmd)
     bsrc = os.path.join(CSRC, "bindings.cpp")
     bobj = os.path.join(BUILD_DIR, "bindings.cpp.o")
     objs.append(bobj)
-    if force or _needs(bobj, bsrc, hdr):
-        py_inc = sysconfig.get_paths()["include"]
-        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", abi, "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-               f"-DTORCH_EXTENSION_NAME={os.environ.get('KOP_EXT_NAME', '_C')}", "-DTORCH_API_INCLUDE_EXTENSION_H", "-w",
-               "-I", CSRC, "-I", os.path.join(ROCM, "include"), "-I", py_inc]
-        for i in tinc:
-            cmd += ["-I", i]
-        cmd += ["-c", bsrc, "-o", bobj]
+    py_inc = sysconfig.get_paths()["include"]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", abi, "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           f"-DTORCH_EXTENSION_NAME={os.environ.get('KOP_EXT_NAME', '_C')}", "-DTORCH_API_INCLUDE_EXTENSION_H", "-w",
+           "-I", CSRC, "-I", os.path.join(ROCM, "include"), "-I", py_inc]
+    for i in tinc:
+        cmd += ["-I", i]
+    cmd += ["-c", bsrc, "-o", bobj]
+    if force or _needs(bobj, bsrc, hdr, cmd):
         jobs_list.append(cmd)
     if jobs_list:
         n = jobs or min(len(jobs_list), int(os.environ.get("MAX_JOBS", "8")))
         with cf.ThreadPoolExecutor(max_workers=max(1, n)) as ex:
-            for cmd, fut in [(c, ex.submit(_run, c)) for c in jobs_list]:
+            for cmd, fut in [(c, ex.submit(_compile, c)) for c in jobs_list]:
                 if verbose:
                     print("[kop-build]", os.path.basename(cmd[-3] if cmd[-2] == "-o" else cmd[-1]), file=sys.stderr)
                 fut.result()
