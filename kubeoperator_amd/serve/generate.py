@@ -387,7 +387,7 @@ class LlamaGenerator:
 
                     load().decode_rope_append_(row, self.cos, self.sin, pt, self.cache.k[i], self.cache.v[i], Hq)
                 else:
-                    row.copy_(ref.rope_ref(row, self.cos, self.sin, 1, Hq + Hkv, D, pos=pt))
+                    kf.rope_positions_(row, self.cos, self.sin, pt, Hq + Hkv, D)
                     self.cache.k[i][rows, :, pt.long()] = row[:, a:kc].reshape(B, Hkv, D)
                     self.cache.v[i][rows, :, pt.long()] = row[:, kc:].reshape(B, Hkv, D)
             o = self._attend(i, qkv[:, :a], self.cache.k[i][:B], self.cache.v[i][:B], lens, max_len, T)
