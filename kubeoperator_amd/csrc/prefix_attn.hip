@@ -8,7 +8,7 @@
 // keys leave HBM once per row tile instead of once per sequence, and its products have enough rows for the matrix cores.
 //
 // S^T [keys x rows] = K . Q^T and O^T [dims x rows] += V^T . P^T on v_mfma_f32_16x16x32_bf16, with running maximum and sum
-// per row (fp32). P goes through the matrix cores as a bf16 value and its bf16 remainder, two products (2^-16 relative per key): a
+// per row (fp32). P goes through the matrix cores as a bf16 value and its bf16 remainder, two products (2^-15 relative per key): a
 // value alone (2^-8) adds as much to the result's error as its own rounding does (0.0023 relative instead of 0.0016), saves nothing
 // where memory is the bound and a sixth to a quarter where the matrix cores are (drafts 86 us, with the remainder 101; prompts 371
 // and 468). The 16 key rows of product b are keys
@@ -172,7 +172,8 @@ __device__ __forceinline__ void raise_max(f32x4* sc, int left, float sl2, float&
       for (int e = 0; e < 4; ++e) acc[c][e] *= al;
   }
 }
-// Then the weights, P^T: their sum into l, in fp32, and each as a bf16 value and the bf16 remainder (off by 2^-16 of it at most).
+// Then the weights, P^T: their sum into l, in fp32, and each as a bf16 value (cut, not rounded) and the bf16 remainder. 2^-20 of the
+// weight goes into the remainder, so that one of a weight above 0 is above 0 too: times an infinite value, the two add up to inf.
 template <bool EDGE, int NB>
 __device__ __forceinline__ void weights(const f32x4* sc, int left, float sl2, float m, float& l, bf16x8* hi, bf16x8* lo) {
   float s[2] = {0.f, 0.f};
@@ -189,8 +190,11 @@ __device__ __forceinline__ void weights(const f32x4* sc, int left, float sl2, fl
         if constexpr (EDGE) v[k] = 32 * (j >> 3) + (j & 7) < left ? v[k] : 0.f;
         s[k] += v[k];
       }
-      h[i] = pack2(v[0], v[1]);
-      r[i] = pack2(v[0] - __uint_as_float(h[i] << 16), v[1] - __uint_as_float(h[i] & 0xffff0000u));
+      const uint32_t x = __float_as_uint(v[0]), y = __float_as_uint(v[1]);
+      constexpr float up = 1.f + 0x1p-20f;
+      const uint32_t xh = x & 0xffff0000u, yh = y & 0xffff0000u;
+      h[i] = NB == 1 ? yh | (x >> 16) : __builtin_amdgcn_perm(y, x, 0x07060302u);  // (by keys no scalar register is left for the constant)
+      r[i] = pack2(fmaf(v[0], up, -__uint_as_float(xh)), fmaf(v[1], up, -__uint_as_float(yh)));
     }
     hi[b] = __builtin_bit_cast(bf16x8, h);
     lo[b] = __builtin_bit_cast(bf16x8, r);

@@ -335,10 +335,10 @@ FORMS += [("cpu", 4, 1, 4, 2, 64, 500, 60), ("cpu", 2, 8, 4, 2, 128, 128, 40)]
 @pytest.mark.parametrize("dev,B,T,Hq,Hkv,D,P,own", FORMS)
 def test_weights_lose_nothing_to_the_operands_type(dev, B, T, Hq, Hkv, D, P, own):
     """A softmax over six keys (the others' scores are too low to count): what the result may be off by, besides the output's one
-    rounding, is the scores' and sums' fp32 and 2^-16 of each weight, not the 2^-8 of a weight in bf16.
+    rounding, is the scores' and sums' fp32 and 2^-15 of each weight, not the 2^-8 of a weight in bf16.
 
-    Tolerance, with A = sum_j p_j |v_j| over the six: a weight as a bf16 value and its remainder is off by at most 2^-8 2^-8, in
-    the product with V and in the sum: 2^-16 (A + |o|). A score is off by ((D + 4) sum |q||k| scale + 4 |s|) 2^-24 and the
+    Tolerance, with A = sum_j p_j |v_j| over the six: a weight cut to a bf16 value leaves a remainder below 2^-7 of it, which is
+    rounded to bf16 (2^-8) after 2^-20 of the weight went into it: 2^-15 A + 2^-20 A, and as much of |o| for good measure. A score is off by ((D + 4) sum |q||k| scale + 4 |s|) 2^-24 and the
     exponential by 2^-22, e relative together; sums of six terms, in up to 32 parts, add 40 2^-24: (e + 40 2^-24) (A + |o|).
     The other keys' scores are 45 below or lower: 4000 e^-45 < 2^-50. The output's rounding: 2^-8 of what is rounded."""
     qkv, kp, vp, kc, vc = make(B, T, Hq, Hkv, D, P, own + 3, dev, seed=P)
@@ -360,7 +360,23 @@ def test_weights_lose_nothing_to_the_operands_type(dev, B, T, Hq, Hkv, D, P, own
     p = torch.softmax(s, -1).unsqueeze(-1)
     o, A = (p * v.unsqueeze(2)).sum(3), (p * v.abs().unsqueeze(2)).sum(3)
     e = ((D + 4) * mag.amax(-1) + 4 * s.abs().amax(-1)) * U + 2.0 ** -22 + 40 * U
-    tol = (2.0 ** -16 + e.unsqueeze(-1)) * (A + o.abs())
+    tol = (2.0 ** -15 + 2.0 ** -20 + e.unsqueeze(-1)) * (A + o.abs())
     tol = tol + 2.0 ** -8 * (o.abs() + tol)
     err = (got.transpose(1, 2) - o).abs()
     assert (err <= tol).all(), float((err / tol).max())
+
+
+@pytest.mark.parametrize("dev,B,T,Hq,Hkv,D,P,own", FORMS)
+def test_infinite_values_that_every_row_sees(dev, B, T, Hq, Hkv, D, P, own):
+    """A value of inf whose weight is not 0 makes its dimension inf, not NaN, in every row that sees it: a weight's remainder is never
+    0 times inf, nor of the other sign."""
+    for bad in (float("inf"), -float("inf")):
+        qkv, kp, vp, kc, vc = make(B, T, Hq, Hkv, D, P, own + 3, dev, seed=P)
+        lens = torch.full((B,), own, dtype=torch.int32, device=dev)
+        args = (kc, vc, lens, own, T)
+        want = kf.prefix_attention(qkv[:, : Hq * D], kp, vp, *args).view(B * T, Hq, D)
+        vp[:, 3, 5] = bad
+        qkv[:, 0] = 0.0  # a score of 0 against every key of one row: weights that bf16 holds
+        kp[:, :, 1:] = 0.0
+        got = kf.prefix_attention(qkv[:, : Hq * D], kp, vp, *args).view(B * T, Hq, D)
+        assert (got[:, :, 5] == bad).all() and torch.isfinite(got[:, :, [0, 4, 6, D - 1]]).all() and torch.isfinite(want).all()
