@@ -105,7 +105,7 @@ __device__ __forceinline__ float max32(const f32x16& a, const f32x16& b) {
   for (int j = 1; j < 16; ++j) m = max3f(m, a[j], b[j]);
   return m;
 }
-// sum of the 32 values of two accumulators with packed adds (v_pk_add_f32: two lanes' worth per issue)
+// sum of the 32 values of two accumulators, eight chains side by side
 __device__ __forceinline__ float sum32(const f32x16& a, const f32x16& b) {
   typedef float f2 __attribute__((ext_vector_type(2)));
   f2 acc[4];
@@ -117,8 +117,8 @@ __device__ __forceinline__ float sum32(const f32x16& a, const f32x16& b) {
   const f2 s = (acc[0] + acc[1]) + (acc[2] + acc[3]);
   return s[0] + s[1];
 }
-// s = s * c + b over one accumulator with packed FMAs (v_pk_fma_f32: two values per issue, half the VALU
-// slots of 16 v_fma_f32 in the softmax's exponent argument)
+// s = s * c + b over one accumulator (the softmax's exponent argument), written two values at a time; the build compiles
+// it without packed fp32 instructions, to 16 v_fma_f32
 __device__ __forceinline__ void fma_pk16(f32x16& s, float c, float b) {
   typedef float f2 __attribute__((ext_vector_type(2)));
   const f2 c2 = {c, c}, b2 = {b, b};

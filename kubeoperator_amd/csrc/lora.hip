@@ -4,11 +4,12 @@
 //   x [M, K], y / out [M, N] bf16 rows; a [n, r, K], b [n, N, r] bf16; index [M] int32; scale [n] fp32
 //
 // Two launches: the rows' products with a (K split over workgroups, fp32 partials), then their products with b added to y.
-// Both take up to 64 rows per workgroup as 16-column operands of v_mfma_f32_16x16x32_bf16, in one of two forms:
-//   * by adapter (few rows: a decode step): a workgroup collects the rows of ONE adapter from the index list, so every
-//     adapter that occurs is read once, however its rows are scattered; one more "adapter" collects the rows without any;
-//   * by rows (many rows: a prefill): consecutive rows, the adapters that occur among them taken one after another
-//     (lowest row first), each row keeping the result of its own only -- by selection, not by a zero factor, so a request's
+// Both take rows as 16-column operands of v_mfma_f32_16x16x32_bf16, in one of two forms:
+//   * by adapter (few rows: a decode step): a workgroup collects up to 64 rows (ranks above 64: 32; second launch: 128) of ONE
+//     adapter from the index list, so every adapter that occurs is read once, however its rows are scattered; one more "adapter"
+//     collects the rows without any;
+//   * by rows (many rows: a prefill): 32 (second launch: 64) consecutive rows, the adapters that occur among them taken one after
+//     another (lowest row first), each row keeping the result of its own only -- by selection, not by a zero factor, so a request's
 //     NaN weights stay with its own rows.
 // The low-rank values enter the second product as a bf16 pair (value and remainder: 2^-16 relative), so the only rounding
 // that counts is the output's.

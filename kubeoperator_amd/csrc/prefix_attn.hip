@@ -10,8 +10,8 @@
 // S^T [keys x rows] = K . Q^T and O^T [dims x rows] += V^T . P^T on v_mfma_f32_16x16x32_bf16, with running maximum and sum
 // per row (fp32). P goes through the matrix cores as a bf16 value and its bf16 remainder, two products (2^-15 relative per key): a
 // value alone (2^-8) adds as much to the result's error as its own rounding does (0.0023 relative instead of 0.0016), saves nothing
-// where memory is the bound and a sixth to a quarter where the matrix cores are (drafts 86 us, with the remainder 101; prompts 371
-// and 468). The 16 key rows of product b are keys
+// where memory is the bound and a sixth to a quarter elsewhere (drafts 86 us, with the remainder 103; 8 x 1024 tokens behind 2048
+// 371 and 468). The 16 key rows of product b are keys
 // 8 (i >> 2) + 4 b + (i & 3), so that a lane's scores of two products are its own P^T operand (keys 8 g .. 8 g + 7 of its row),
 // with no lane exchange; V goes through an LDS image whose 16-byte chunks are XOR-permuted by the row, and is read transposed.
 // A workgroup works in one of two ways:
@@ -21,12 +21,12 @@
 //     them. The next tile's scores (matrix cores) run beside this tile's weights (vector ALUs). Bound by those two.
 // and a launch takes one of three forms (make_plan):
 //   * split: workgroups of (row tile, key range) of the prefix, and of one sequence's own keys, write fp32 partials (O, max, sum);
-//     a second launch folds them. Decode (64 sequences, 32/8 heads of 128, 2048 + 500 keys): 23 + 5 us, 3.5 TB/s. Drafts (64 x 5
-//     tokens, 8192 + 1000 keys, prefix by rows): 83 + 7 us; the prefix alone 69, 630 TFLOP/s.
+//     a second launch folds them. Decode (64 sequences, 32/8 heads of 128, 2048 + up to 500 keys): 23 + 5 us, 3.3 TB/s in the
+//     first. Drafts (64 x 5 tokens, 8192 + up to 1000 keys, prefix by rows): 96 + 7 us; the prefix alone 99, 435 TFLOP/s.
 //   * short contexts, by keys: a workgroup takes prefix and own keys of its rows, one launch, no partials. 4 sequences, 500 + 60
-//     keys: 7.1 us against 8.3 split.
-//   * prompts, by rows: the same for sequences with many tokens. 8 x 1024 tokens behind 2048, 32/8 heads of 128: 413 us, 830
-//     TFLOP/s; one prompt of 4096, no prefix: 151 us, 910 TFLOP/s.
+//     keys: 7.3 us against 8.3 split.
+//   * prompts, by rows: the same for sequences with many tokens. 8 x 1024 tokens behind 2048, 32/8 heads of 128: 470 us, 730
+//     TFLOP/s; one prompt of 4096, no prefix: 200 us, 690 TFLOP/s (matrix cores 47-53 % busy, vector ALUs 54-60 %).
 //
 // A masked key has weight zero exactly: masked scores never enter the maximum or the sum, keys past the last valid one are
 // never read (loads are clamped to it), and in the blocks where some rows see a key and others do not, values that are
@@ -591,7 +591,7 @@ __device__ __forceinline__ void by_rows(const Args& p, F part, char* smem) {
       }
       __builtin_amdgcn_sched_barrier(0);
       // waves in the vector stretch go first: the other wave of the SIMD has matrix instructions to fill the gaps with (8 x 1024 tokens
-      // behind 4096: 639 us without, 621)
+      // behind 4096: 858 us without, 847)
       __builtin_amdgcn_s_setprio(0);
       v_at(buf, vat);
       __builtin_amdgcn_sched_barrier(0);
@@ -863,8 +863,8 @@ Plan make_plan(int B, int T, int G, int Hkv, int P, int max_len) {
   // the two are close (9 tokens, 500 + 1000: it splits, 84, 72).
   const int64_t tg = (int64_t)T * G, rt = cdiv(tg, tile_rows(kByRows)), seen = std::max(max_len - T / 2, 0);
   q.whole = tg > 32 && B * Hkv * rt >= 256 && 128 * rt * (P + seen) <= tg * (P + (int64_t)1100) + 64 * cdiv(tg, 32) * seen;
-  // Otherwise own keys go by keys, also where 32-row tiles read them more than once: by rows (64 x 16 tokens, 8192 + 1000 keys) 313
-  // us against 256.
+  // Otherwise own keys go by keys, also where 32-row tiles read them more than once: by rows (64 x 16 tokens, 8192 + 1000 keys,
+  // measured before P had its remainder) 313 us against 230.
   q.om = q.whole ? kByRows : std::min(2, mode_of(tg));
   q.pm = P > 0 ? mode_of(rows) : q.om;
   q.rtp = P > 0 ? cdiv(rows, tile_rows(q.pm)) : 0;
@@ -878,8 +878,8 @@ Plan make_plan(int B, int T, int G, int Hkv, int P, int max_len) {
     return cdiv(keys, chunk);
   };
   // Short contexts: at most 8 steps of 128 keys per wave, and a prefix that it does not hurt to read once per sequence: one step
-  // long, or at most one workgroup per CU. Saves the second launch (4 sequences x 4 heads, 500 + 60 keys: 7.1 us against 8.3; 64 x 32/8 heads of 128,
-  // 128 + 200 keys: 14.3 against 20.3; 16 of them, 500 + 200 keys: 11.8 against 14.0; one, 400 + 100: 10.1 against 9.1).
+  // long, or at most one workgroup per CU. Saves the second launch (4 sequences x 4 heads, 500 + 60 keys: 7.3 us against 8.3; 64 x 32/8 heads of 128,
+  // 128 + 200 keys: 14.6 against 20.6; 16 of them, 500 + 200 keys: 12.1 against 15.4; one, 400 + 100: 10.1 against 9.3).
   const int64_t groups = (int64_t)B * Hkv * q.rto;
   q.whole = q.whole || (cdiv(P, 128) + cdiv(max_len, 128) <= 8 && (P <= 128 || groups <= 256) &&
                         (max_len <= 256 || groups >= 128));

@@ -17,8 +17,9 @@
 // re-derives it from the chunk statistics (a few hundred numbers): no atomics, no order-dependent sums. Small problems, whose
 // time is all launches, do the same in one: a workgroup per sequence.
 //
-// 64 sequences, 4 drafts, 128256 fp32 logits: 60 us for the first pass (295 MB, 4.9 TB/s, what a copy reaches), 20 for the second
-// (128 rows again, mostly from cache; 16 million fp64 exponentials), 5.6 for the pick. One sequence, 3 drafts, 50304 logits:
+// 64 sequences, 4 drafts, 128256 fp32 logits: 61 us for the first pass (295 MB, 4.9 TB/s, what a copy reaches; vector ALUs 73 %
+// busy, and as long for bf16 logits, which are half the bytes), 20 for the second (128 rows again, mostly from cache; 16 million fp64
+// exponentials), 5.2 for the pick. One sequence, 3 drafts, 50304 logits:
 // 4.9 + 6.3 + 3.6 us, each a launch and its chain of loads. Joining the pick to the second pass (the sequence's last workgroup,
 // told by a counter) costs more than the launch it saves: a fence for the whole device writes each XCD's L2 back (the two
 // together 219 instead of 28 us for 64 sequences, 12.3 instead of 10.3 for one).
@@ -369,7 +370,8 @@ __device__ __forceinline__ void piece_sums(const Args& a, const Rest<E>& f, int 
 }
 
 // ---- pass 2 (not greedy): grid (pieces / (4 kPieces), B). A piece is what a wave reads at once, so that its sum is one fold of
-// the wave; 4 pieces a wave share one derivation of the acceptance. Bound by the fp64 exponentials (about 0.8 per ps).
+// the wave; 4 pieces a wave share one derivation of the acceptance. 16 million exponentials in 20 us (64 sequences of 128256; the first pass,
+// which also reads its logits from memory, does 1.2 per ps): vector ALUs 62 % busy, after a chain of loads for the acceptance.
 template <typename E>
 __global__ void __launch_bounds__(kT) verify_rest_kernel(Args a) {
   __shared__ float s_m[kMaxRows];
