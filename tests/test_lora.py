@@ -199,3 +199,9 @@ def test_more_rows_than_a_launch_can_have_are_refused(dev, M):
     index = torch.empty(M, dtype=torch.int32, device=dev) if dev == "cuda" else torch.zeros(1, dtype=torch.int32).expand(M)
     with pytest.raises(RuntimeError, match="too many rows"):
         kf.lora_add(row.expand(M, 8), row.expand(M, 8), low, low, index, torch.ones(1, device=dev))
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("M,n", [(1, 700), (64, 700), (130, 1500)])
+def test_more_adapters_than_rows(dev, M, n):
+    check(make(M, n, 16, 128, 72, dev, seed=n))
