@@ -3,7 +3,7 @@
 No hipify step and no ``torch.utils.cpp_extension`` JIT cache: every ``csrc/*.hip`` translation unit is
 compiled by ``hipcc --offload-arch=gfx950`` (they include no PyTorch headers, so each takes seconds),
 ``bindings.cpp`` is compiled once as host C++ against the PyTorch headers, and the objects are linked
-into one shared object next to the package so it travels with the source tree (``gpurun`` snapshots it).
+into one shared object next to the package so it travels with the source tree.
 
 Incremental: an object is rebuilt when its source or any ``csrc/*.h`` header is newer, or when it was made by another command
 line than today's (recorded beside it): flags that results depend on reach every object.
